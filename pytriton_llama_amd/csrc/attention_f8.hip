@@ -1,0 +1,535 @@
+// Attention over a paged cache that is held in 8 bits: the formulas, the tables and the mask of attention.hip (causal, window,
+// sink), over keys and values that stand for e4m3(code) * scale with one scale, a power of two, for the keys and one for the values
+// of every (page, kv head). Codes [pages, Hkv, page_size, D], scales float32 [pages, Hkv].
+//
+// e4m3 times a power of two is a bfloat16 number as it is: the matrix-core kernels below turn codes into bfloat16 with the scale in
+// the converting instruction and lose nothing there.
+#include "attention.h"
+#include "common.h"
+#include "device.h"
+#include "mfma.h"
+#include <math.h>
+
+// What all kernels here are given.
+struct F8Cache {
+  const uint8_t *k, *v;
+  const float *k_scale, *v_scale;
+};
+struct F8Tables {
+  const int32_t *q_start, *ctx_len, *block_table;
+  int bt_stride;
+};
+
+// ===========================================================================
+// ptl_attention_generic_f8: float32 arithmetic on the vector units, for every type of query, head size (up to 640), page size
+// and number of heads. A workgroup has one query row of one head; its four waves take the keys 64 at a time in turn, a lane a key
+// for the scores and a lane every 64th column for the values.
+template <typename T, int NACC>
+__global__ void __launch_bounds__(256)
+attn_generic_f8_kernel(T* __restrict__ out, long out_stride, const T* __restrict__ q, long q_stride, F8Cache cache, F8Tables tab,
+                       const int32_t* __restrict__ work_seq, const int32_t* __restrict__ work_qoff, int Hq, int Hkv, int D,
+                       int page_size, int window, const float* __restrict__ sink, float scale) {
+  extern __shared__ float lds[];
+  __shared__ float ps[4][64];              // a tile's probabilities times the values' scales
+  __shared__ long at[4][64];               // where its value rows lie
+  __shared__ float ends[4][2];
+  float* qs = lds;                         // [D]
+  float* sums = lds + D;                   // [4][D]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int item = blockIdx.x >> 4, head = blockIdx.y;
+  const int seq = work_seq[item], r = work_qoff[item] + (blockIdx.x & 15);
+  const int first = tab.q_start[seq], rows = tab.q_start[seq + 1] - first, ctx = tab.ctx_len[seq];
+  if (r >= rows) return;
+  const int row = first + r, pos = ctx - rows + r, kvh = head / (Hq / Hkv);
+  const int32_t* bt = tab.block_table + (size_t)seq * tab.bt_stride;
+  for (int d = threadIdx.x; d < D; d += 256) qs[d] = to_float<T>(q[(size_t)row * q_stride + (size_t)head * D + d]);
+  __syncthreads();
+  const int lo = window > 0 ? max(0, pos - window + 1) : 0;
+  float m = -INFINITY, l = 0.f, acc[NACC];
+#pragma unroll
+  for (int a = 0; a < NACC; ++a) acc[a] = 0.f;
+  const bool words = D % 4 == 0;
+  for (int k0 = lo + 64 * wave; k0 <= pos; k0 += 256) {
+    const int key = k0 + lane, n = min(64, pos + 1 - k0);
+    float s = -INFINITY, vs = 0.f;
+    long row_at = 0;
+    if (lane < n) {
+      const int slot = key / page_size, page = bt[slot];
+      const size_t block = (size_t)page * Hkv + kvh;
+      row_at = (block * page_size + (key - slot * page_size)) * D;
+      const uint8_t* kr = cache.k + row_at;
+      float dot = 0.f;
+      if (words) {
+        for (int d = 0; d < D; d += 4) {
+          const int x = *reinterpret_cast<const int*>(kr + d);
+          const auto e = __builtin_amdgcn_cvt_pk_f32_fp8(x, false), f = __builtin_amdgcn_cvt_pk_f32_fp8(x, true);
+          dot = fmaf(e[0], qs[d], dot);
+          dot = fmaf(e[1], qs[d + 1], dot);
+          dot = fmaf(f[0], qs[d + 2], dot);
+          dot = fmaf(f[1], qs[d + 3], dot);
+        }
+      } else {
+        for (int d = 0; d < D; ++d) dot = fmaf(__builtin_amdgcn_cvt_f32_fp8((int)kr[d], 0), qs[d], dot);
+      }
+      s = dot * cache.k_scale[block] * scale;
+      vs = cache.v_scale[block];
+    }
+    const float top = fmaxf(m, wave_max(s));
+    const float to = top == -INFINITY ? 0.f : top, keep = expf(m - to);
+    const float p = lane < n ? expf(s - to) : 0.f;
+    l = l * keep + wave_sum(p);
+    m = top;
+    ps[wave][lane] = p * vs;
+    at[wave][lane] = row_at;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");       // (a wave's own LDS: written above, read below)
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int a = 0; a < NACC; ++a) acc[a] *= keep;
+    for (int j = 0; j < n; ++j) {
+      const float pj = ps[wave][j];
+      const uint8_t* vr = cache.v + at[wave][j];
+#pragma unroll
+      for (int a = 0; a < NACC; ++a) {
+        const int d = lane + 64 * a;
+        if (d < D) acc[a] = fmaf(__builtin_amdgcn_cvt_f32_fp8((int)vr[d], 0), pj, acc[a]);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+#pragma unroll
+  for (int a = 0; a < NACC; ++a)
+    if (lane + 64 * a < D) sums[wave * D + lane + 64 * a] = acc[a];
+  if (lane == 0) { ends[wave][0] = m; ends[wave][1] = l; }
+  __syncthreads();
+  float top = sink ? sink[head] : -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) top = fmaxf(top, ends[w][0]);
+  const float to = top == -INFINITY ? 0.f : top;
+  float total = sink ? expf(sink[head] - to) : 0.f, f[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = expf(ends[w][0] - to);
+    total += ends[w][1] * f[w];
+  }
+  const float inv = total == 0.f ? 0.f : 1.0f / total;            // (a row without keys: zeros)
+  for (int d = threadIdx.x; d < D; d += 256) {
+    float a = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) a = fmaf(sums[w * D + d], f[w], a);
+    out[(size_t)row * out_stride + (size_t)head * D + d] = from_float<T>(a * inv);
+  }
+}
+
+extern "C" int ptl_attention_generic_f8(void* out, long out_stride, const void* q, long q_stride, const uint8_t* k, const uint8_t* v,
+                                        const float* k_scale, const float* v_scale, const int32_t* q_start, const int32_t* ctx_len,
+                                        const int32_t* block_table, int bt_stride, const int32_t* work_seq, const int32_t* work_qoff,
+                                        int n_work, int Hq, int Hkv, int D, int page_size, int window, const float* sink, float scale,
+                                        int dtype, hipStream_t stream) {
+  if (n_work <= 0) return PTL_OK;
+  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq > 65535 || D <= 0 || D > 640 || page_size <= 0 || n_work >= 1 << 26 || window < 0)
+    return PTL_ERR_ARG;
+  const F8Cache cache{k, v, k_scale, v_scale};
+  const F8Tables tab{q_start, ctx_len, block_table, bt_stride};
+  const dim3 grid(16 * n_work, Hq);
+  const size_t lds = 5 * (size_t)D * sizeof(float);
+  auto go = [&](auto kernel, auto* o, auto* x) {
+    kernel<<<grid, 256, lds, stream>>>(o, out_stride, x, q_stride, cache, tab, work_seq, work_qoff, Hq, Hkv, D, page_size, window,
+                                       sink, scale);
+  };
+  if (dtype == PTL_DTYPE_F32) {
+    auto *o = (float*)out; auto* x = (const float*)q;
+    if (D <= 128) go(attn_generic_f8_kernel<float, 2>, o, x);
+    else if (D <= 256) go(attn_generic_f8_kernel<float, 4>, o, x);
+    else go(attn_generic_f8_kernel<float, 10>, o, x);
+  } else if (dtype == PTL_DTYPE_BF16) {
+    auto *o = (bf16_t*)out; auto* x = (const bf16_t*)q;
+    if (D <= 128) go(attn_generic_f8_kernel<bf16_t, 2>, o, x);
+    else if (D <= 256) go(attn_generic_f8_kernel<bf16_t, 4>, o, x);
+    else go(attn_generic_f8_kernel<bf16_t, 10>, o, x);
+  } else {
+    return PTL_ERR_ARG;
+  }
+  return ptl_launch_status();
+}
+
+// ===========================================================================
+// The matrix-core kernels: bfloat16 queries, head sizes of 32, 64, 96 and 128, pages of 16 rows and more (a power of two).
+// D = 64 A + 32 B. A 16-byte piece of a key row holds, for lane group lg = lane / 16, elements 64 c + 16 lg .. +15 (c < A): the k-values of
+// two matrix instructions (which k-value stands where is free, as long as the queries' agree); the last 32 elements come as
+// 8 bytes, 64 A + 8 lg .. +7.
+
+// two codes (the low or the high half of x) times a power of two, as bfloat16: exact
+__device__ __forceinline__ uint32_t two_bf16(uint32_t x, float scale, bool high) {
+  const auto r = high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x, scale, true)
+                      : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x, scale, false);
+  return __builtin_bit_cast(uint32_t, r);
+}
+__device__ __forceinline__ bf16x8_t eight_bf16(uint32_t x, uint32_t y, float scale) {
+  Frag8 f;
+  f.u = make_uint4(two_bf16(x, scale, false), two_bf16(x, scale, true), two_bf16(y, scale, false), two_bf16(y, scale, true));
+  return f.v;
+}
+// the low (high) halves of two words, side by side
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// ===========================================================================
+// ptl_attention_decode_f8: the sequences of a step that bring one token each.
+//
+// The keys of a (sequence, kv head) pair are cut into parts of ``piece`` units of 128 keys, the same piece for all sequences: as
+// long as lets the parts of all of them fit the launch, which has room for ``cuts`` parts beside one a sequence
+// (sum of ceil(n_s / piece) <= sum of n_s / piece + sequences). Every workgroup finds the piece and its own part from the context
+// lengths on the device, so a recorded launch suits whatever contexts it is replayed with. A pair's parts are merged by the
+// workgroup that is done last (a ticket), in the order of the keys.
+//
+// A workgroup has four waves, which take tiles of 32 keys in turn. Both products are transposed, as in attention_decode.h:
+//   S^T[key, head] = K . Q^T        A = K: lane (ln, lg) has key ln's k-values, straight from memory
+//   O^T[d, head]  += V^T . P^T      B = P^T: what a lane has of S^T; A = V^T[d, key]
+// For the second a lane needs one d of the 8 keys that its P^T values belong to. It loads D / 16 neighbouring elements of each of those
+// keys, which are D / 16 matrix instructions' d, and pairs the keys' halves up after the conversion (two
+// v_perm_b32 for two words): no LDS between memory and the matrix cores, and nothing to wait for but the loads.
+struct DecodeF8Parts {
+  float *acc, *ml;                 // [part][kv head][heads of a kv head][D] sums, [..][2] their maximum and denominator
+  int* tickets;                    // [sequence][kv head][head tile][TICKET]
+};
+
+constexpr int UNIT_F8 = 128;       // keys of a workgroup's turn
+
+template <int A, int B>
+__global__ void __launch_bounds__(256)
+attn_decode_f8_kernel(const int32_t* __restrict__ ctx_len, const int32_t* __restrict__ block_table, const uint8_t* __restrict__ k_cache,
+                      const uint8_t* __restrict__ v_cache, int n_seq, int Hkv, int cuts, int bt_stride, int page_shift,
+                      const bf16_t* __restrict__ q, long q_stride, const float* __restrict__ k_scale,
+                      const float* __restrict__ v_scale, int Hq, bf16_t* __restrict__ out, long out_stride,
+                      const int32_t* __restrict__ q_start, DecodeF8Parts parts, int window, const float* __restrict__ sink,
+                      float scale_log2) {
+  constexpr int D = 64 * A + 32 * B, NT = D / 16, STEPS = D / 32;
+  constexpr int REGION = 16 * D + 32;               // floats of a wave's sums
+  __shared__ __attribute__((aligned(16))) float regions[4][REGION];
+  __shared__ int last;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 15, lg = lane >> 4;
+  const int G = Hq / Hkv, tiles = (G + 15) / 16, tile = blockIdx.y, GT = min(16, G - 16 * tile);
+  const int kvh = blockIdx.x % Hkv, u = blockIdx.x / Hkv;
+
+  // ---- which part of which sequence ----
+  auto units_of = [&](int s) {
+    const int c = ctx_len[s], lo = window > 0 ? max(0, c - window) : 0;
+    return c > 0 ? (c - (lo & ~15) + UNIT_F8 - 1) / UNIT_F8 : 0;
+  };
+  int total = 0;
+  for (int s0 = 0; s0 < n_seq; s0 += 64) total += s0 + lane < n_seq ? units_of(s0 + lane) : 0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+  const int piece = max(1, (total + cuts - 1) / cuts);
+  int seq = -1, split = 0, n_parts = 0, before = 0;
+  for (int s0 = 0; s0 < n_seq && seq < 0; s0 += 64) {
+    const int mine = s0 + lane < n_seq ? max(1, (units_of(s0 + lane) + piece - 1) / piece) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(upto, o, 64);
+      upto += lane >= o ? x : 0;
+    }
+    const unsigned long long here = __ballot(before + upto > u);
+    if (here) {
+      const int at = __ffsll(here) - 1;
+      seq = s0 + at;
+      n_parts = __builtin_amdgcn_readlane(mine, at);
+      split = u - (before + __builtin_amdgcn_readlane(upto, at) - n_parts);
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  if (seq < 0) return;                              // (more room than parts)
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  const int ctx = ctx_len[seq], row = q_start[seq];
+  const int k_lo = window > 0 ? max(0, ctx - window) : 0;
+  const int k_first = (k_lo & ~15) + split * piece * UNIT_F8;
+  const int k_end = min(ctx, k_first + piece * UNIT_F8);
+  const int head0 = kvh * G + 16 * tile;
+  const int32_t* bt = block_table + (size_t)seq * bt_stride;
+  const uint32_t page_bytes = (uint32_t)(Hkv * D) << page_shift;          // < 4 GiB, checked by the host
+  const uint8_t* k_head = k_cache + ((size_t)(kvh * D) << page_shift);
+  const uint8_t* v_head = v_cache + ((size_t)(kvh * D) << page_shift);
+
+  Frag8 qf[STEPS];
+  {
+    const bf16_t* qr = q + (size_t)row * q_stride + (size_t)(head0 + min(ln, GT - 1)) * D;
+#pragma unroll
+    for (int c = 0; c < A; ++c) {
+      qf[2 * c].u = load16(qr + 64 * c + 16 * lg);
+      qf[2 * c + 1].u = load16(qr + 64 * c + 16 * lg + 8);
+    }
+    if (B) qf[2 * A].u = load16(qr + 64 * A + 8 * lg);
+  }
+  Frag8 ones;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ones.v[j] = (__bf16)1.0f;
+
+  struct Tile {
+    uint4 k[2][A ? A : 1];
+    uint2 kb[2];
+    uint32_t v[2][4][A ? A : 1], vb[2][4];
+    float ks[2], vs[2];
+  };
+  const int turns = (k_end - k_first + UNIT_F8 - 1) / UNIT_F8;          // (0: no keys)
+  auto first_key = [&](int turn) { return k_first + turn * UNIT_F8 + 32 * wave; };
+  // the page of the 16 keys from kp on (one page: pages hold a multiple of 16); of keys that are none, that of one that is
+  auto page_at = [&](int kp) {
+    const int at = __builtin_amdgcn_readfirstlane(min(max(kp, k_lo), k_end - 1) >> page_shift);
+    return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(bt + at);
+  };
+  auto load = [&](Tile& t, int turn, const int (&page)[2]) __attribute__((always_inline)) {
+    const int kc = first_key(turn);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int in_page = (kc + 16 * h) & ((1 << page_shift) - 1);
+      const uint64_t at = (uint64_t)(uint32_t)page[h] * page_bytes + (uint32_t)(in_page * D);
+      const uint8_t *kr = k_head + at, *vr = v_head + at;
+      const size_t block = (size_t)page[h] * Hkv + kvh;
+      t.ks[h] = *(const __attribute__((address_space(4))) float*)(uintptr_t)(k_scale + block);
+      t.vs[h] = *(const __attribute__((address_space(4))) float*)(uintptr_t)(v_scale + block);
+#pragma unroll
+      for (int c = 0; c < A; ++c) t.k[h][c] = load_once(kr + ln * D + 64 * c + 16 * lg);
+      if (B) t.kb[h] = *reinterpret_cast<const uint2*>(kr + ln * D + 64 * A + 8 * lg);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* x = vr + (4 * lg + i) * D;
+        if constexpr (A == 1) t.v[h][i][0] = *reinterpret_cast<const uint32_t*>(x + 4 * ln);
+        if constexpr (A == 2) {
+          const uint2 w = *reinterpret_cast<const uint2*>(x + 8 * ln);
+          t.v[h][i][0] = w.x;
+          t.v[h][i][1] = w.y;
+        }
+        if (B) t.vb[h][i] = *reinterpret_cast<const uint16_t*>(x + 64 * A + 2 * ln);
+      }
+    }
+  };
+
+  f32x4_t o[NT + 1];                                // (the last one: the denominator, of ones for values)
+#pragma unroll
+  for (int t = 0; t <= NT; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m_run = -INFINITY;
+  auto use = [&](Tile& t, int turn) __attribute__((always_inline)) {
+    const int kc = first_key(turn);
+    if (kc >= k_end) return;                        // (wave-uniform)
+    const bool whole = kc >= k_lo && kc + 32 <= k_end;
+    if (!whole) {
+      // rows that are no keys: what lies there may be a NaN, and zero times NaN is one
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = kc + 16 * h + 4 * lg + i;
+          const bool in = key >= k_lo && key < k_end;
+#pragma unroll
+          for (int c = 0; c < A; ++c) t.v[h][i][c] = in ? t.v[h][i][c] : 0;
+          if (B) t.vb[h][i] = in ? t.vb[h][i] : 0;
+        }
+    }
+    f32x4_t st[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      st[h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < A; ++c) {
+        st[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16(t.k[h][c].x, t.k[h][c].y, t.ks[h]), qf[2 * c].v, st[h], 0, 0, 0);
+        st[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16(t.k[h][c].z, t.k[h][c].w, t.ks[h]), qf[2 * c + 1].v, st[h], 0, 0, 0);
+      }
+      if (B) st[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16(t.kb[h].x, t.kb[h].y, t.ks[h]), qf[2 * A].v, st[h], 0, 0, 0);
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float s = st[h][i] * scale_log2;
+        if (!whole) {
+          const int key = kc + 16 * h + 4 * lg + i;
+          s = key >= k_lo && key < k_end ? s : -INFINITY;
+        }
+        st[h][i] = s;
+        top = __builtin_elementwise_maximum(top, s);
+      }
+    top = max_with_lane_xor32(max_with_lane_xor16(top));
+    // the maximum follows only when the scores pass it by 2^8: until then float32 sums and bfloat16 probabilities hold as well
+    if (top > m_run + 8.0f) {
+      const float keep = __builtin_amdgcn_exp2f(m_run - top);
+      m_run = top;
+#pragma unroll
+      for (int n = 0; n <= NT; ++n) { o[n][0] *= keep; o[n][1] *= keep; o[n][2] *= keep; o[n][3] *= keep; }
+    }
+    const float to = m_run == -INFINITY ? 0.f : m_run;
+    Frag8 p;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p.v[4 * h + i] = (__bf16)__builtin_amdgcn_exp2f(st[h][i] - to);
+    // V^T: word w of a lane's 8 keys holds two neighbouring d of each
+    auto products = [&](int n, const uint32_t (&w)[8]) __attribute__((always_inline)) {
+      Frag8 f;
+      f.u = make_uint4(low_halves(w[0], w[1]), low_halves(w[2], w[3]), low_halves(w[4], w[5]), low_halves(w[6], w[7]));
+      o[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.v, p.v, o[n], 0, 0, 0);
+      f.u = make_uint4(high_halves(w[0], w[1]), high_halves(w[2], w[3]), high_halves(w[4], w[5]), high_halves(w[6], w[7]));
+      o[n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.v, p.v, o[n + 1], 0, 0, 0);
+    };
+#pragma unroll
+    for (int c = 0; c < A; ++c)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = two_bf16(t.v[i >> 2][i & 3][c], t.vs[i >> 2], half);
+        products(4 * c + 2 * half, w);
+      }
+    if (B) {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = two_bf16(t.vb[i >> 2][i & 3], t.vs[i >> 2], false);
+      products(4 * A, w);
+    }
+    o[NT] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones.v, p.v, o[NT], 0, 0, 0);
+  };
+
+  if (turns > 0) {
+    Tile ta, tb;
+    int page[2];
+    auto pages = [&](int turn) {
+      const int kc = first_key(turn);
+      page[0] = page_at(kc);
+      page[1] = page_at(kc + 16);
+    };
+    pages(0);
+    load(ta, 0, page);
+    pages(1);
+    for (int turn = 0; turn < turns; turn += 2) {
+      if (turn + 1 < turns) { load(tb, turn + 1, page); pages(turn + 2); }
+      use(ta, turn);
+      if (turn + 1 < turns) {
+        if (turn + 2 < turns) { load(ta, turn + 2, page); pages(turn + 3); }
+        use(tb, turn + 1);
+      }
+    }
+  }
+
+  // ---- the waves' sums meet ----
+  float* const region = regions[wave];
+  if (ln < GT) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 4 * lg + i;                  // row of the result tile: tile n holds d = 4 A r + n, the last ones 64 A + 2 r + n - 4 A
+        region[ln * D + (n < 4 * A ? 4 * A * r + n : 64 * A + 2 * r + n - 4 * A)] = o[n][i];
+      }
+    if (lg == 0) { region[16 * D + 2 * ln] = m_run; region[16 * D + 2 * ln + 1] = o[NT][0]; }
+  }
+  __syncthreads();
+  auto write = [&](int h, int d, float m, float l, float a) {
+    const int head = head0 + h;
+    if (sink) {
+      const float s = sink[head] * 1.4426950408889634f, to = fmaxf(m, s), f = __builtin_amdgcn_exp2f(m - to);
+      l = l * f + __builtin_amdgcn_exp2f(s - to);
+      a *= f;
+    }
+    out[(size_t)row * out_stride + (size_t)head * D + d] = float_to_bf16(l == 0.f ? 0.f : a / l);       // (no keys: zeros)
+  };
+  const size_t group = ((size_t)u * Hkv + kvh) * G + 16 * tile;             // this part's first head
+  for (int i = threadIdx.x; i < GT * D; i += 256) {
+    const int h = i / D, d = i - h * D;
+    float m = -INFINITY, l = 0.f, a = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, regions[w][16 * D + 2 * h]);
+    const float to = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f(regions[w][16 * D + 2 * h] - to);
+      l = fmaf(regions[w][16 * D + 2 * h + 1], f, l);
+      a = fmaf(regions[w][h * D + d], f, a);
+    }
+    if (n_parts == 1) {
+      write(h, d, m, l, a);
+    } else {
+      put_shared(parts.acc + (group + h) * D + d, a);
+      if (d == 0) { put_shared(parts.ml + (group + h) * 2, m); put_shared(parts.ml + (group + h) * 2 + 1, l); }
+    }
+  }
+  if (n_parts == 1) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // this wave's share of the part has reached memory
+  __syncthreads();
+  if (threadIdx.x == 0) last = last_part(parts.tickets + (((size_t)seq * Hkv + kvh) * tiles + tile) * TICKET, n_parts);
+  __syncthreads();
+  if (!last) return;
+  const size_t part_heads = (size_t)Hkv * G, first = group - (size_t)split * part_heads;
+  constexpr int AHEAD = 8;                                  // parts that are asked for at once: they lie a long way off
+  for (int i = threadIdx.x; i < GT * D; i += 256) {
+    const int h = i / D, d = i - h * D;
+    const float *acc = parts.acc + (first + h) * D + d, *ml = parts.ml + (first + h) * 2;
+    float m = -INFINITY, l = 0.f, a = 0.f;
+    for (int s0 = 0; s0 < n_parts; s0 += AHEAD) {
+      float av[AHEAD];
+      float2 e[AHEAD];
+#pragma unroll
+      for (int s = 0; s < AHEAD; ++s) {
+        const size_t at = min(s0 + s, n_parts - 1) * part_heads;
+        e[s] = get_shared2(ml + 2 * at);
+        av[s] = get_shared(acc + at * D);
+      }
+      float top = m;
+#pragma unroll
+      for (int s = 0; s < AHEAD; ++s) top = fmaxf(top, e[s].x);
+      const float to = top == -INFINITY ? 0.f : top, keep = __builtin_amdgcn_exp2f(m - to);
+      l *= keep;
+      a *= keep;
+#pragma unroll
+      for (int s = 0; s < AHEAD; ++s) {
+        const float f = s0 + s < n_parts ? __builtin_amdgcn_exp2f(e[s].x - to) : 0.f;
+        l = fmaf(e[s].y, f, l);
+        a = fmaf(av[s], f, a);
+      }
+      m = top;
+    }
+    write(h, d, m, l, a);
+  }
+}
+
+static bool f8_matrix_sizes(int Hq, int Hkv, int D, int page_size) {
+  return Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 1024 && D > 0 && D % 32 == 0 && D <= 128 && page_size >= 16 &&
+         (page_size & (page_size - 1)) == 0 && (long)Hkv * D * page_size < 1l << 31;
+}
+
+// Room for parts beside one a sequence: what fills the compute units a few times over.
+extern "C" int ptl_attention_decode_f8_cuts(int n_seq, int Hkv, int Hq) {
+  if (n_seq <= 0 || Hkv <= 0 || Hq < Hkv) return 0;
+  const int tiles = (Hq / Hkv + 15) / 16, want = 3 * compute_units() / (Hkv * tiles);
+  return max(1, want > n_seq ? want - n_seq : n_seq);
+}
+
+extern "C" int ptl_attention_decode_f8(void* out, long out_stride, const void* q, long q_stride, const uint8_t* k, const uint8_t* v,
+                                       const float* k_scale, const float* v_scale, const int32_t* q_start, const int32_t* ctx_len,
+                                       const int32_t* block_table, int bt_stride, float* acc, float* ml, int* tickets, int cuts,
+                                       int n_seq, int Hq, int Hkv, int D, int page_size, int window, const float* sink, float scale,
+                                       hipStream_t stream) {
+  if (n_seq <= 0) return PTL_OK;
+  if (!f8_matrix_sizes(Hq, Hkv, D, page_size) || cuts <= 0 || window < 0 || !acc || !ml || !tickets ||
+      ((uintptr_t)ml % 8) || ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 || q_stride % 8)
+    return PTL_ERR_ARG;
+  const long groups = ((long)n_seq + cuts) * Hkv;
+  if (groups >= 1l << 31) return PTL_ERR_ARG;
+  const dim3 grid((unsigned)groups, (Hq / Hkv + 15) / 16);
+  int shift = 0;
+  while (1 << shift < page_size) ++shift;
+  const DecodeF8Parts parts{acc, ml, tickets};
+  auto go = [&](auto kernel) {
+    kernel<<<grid, 256, 0, stream>>>(ctx_len, block_table, k, v, n_seq, Hkv, cuts, bt_stride, shift, (const bf16_t*)q, q_stride, k_scale,
+                                     v_scale, Hq, (bf16_t*)out, out_stride, q_start, parts, window, sink, scale * 1.4426950408889634f);
+  };
+  if (D == 32) go(attn_decode_f8_kernel<0, 1>);
+  else if (D == 64) go(attn_decode_f8_kernel<1, 0>);
+  else if (D == 96) go(attn_decode_f8_kernel<1, 1>);
+  else go(attn_decode_f8_kernel<2, 0>);
+  return ptl_launch_status();
+}

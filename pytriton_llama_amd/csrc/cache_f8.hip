@@ -1,0 +1,327 @@
+// Pages of a cache: the store of a step's keys and values into pages held in 8 bits, and copies of pages.
+//
+// A block is what a page holds of one kv head, page_size rows of D; keys and values have blocks, and scales, of their own.
+// A block stands for the numbers e4m3(code) * scale, scale = 2^e the smallest power of two, e >= -126, with |x| <= 448 scale
+// for every finite x that was stored into it. (A number of e4m3's normal range, |x| >= 2^-6 scale, is then rounded to four
+// significant bits whatever the scale is: what the other tokens of a block change of it lies below 2^-14 of the block's
+// largest number. With a scale of largest / 448 all numbers of a block would move with its largest.) What is not finite is
+// stored as NaN and takes no part in the scale.
+#include "common.h"
+#include "device.h"
+
+// 2^e for -126 <= e <= 127
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
+
+// The exponent of the scale of numbers up to ``largest`` (finite, not negative): 448 = 1.75 * 2^8.
+__device__ __forceinline__ int scale_exponent(float largest) {
+  const uint32_t u = __float_as_uint(largest);
+  return max(-126, (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0));
+}
+
+// two numbers as e4m3 codes in the low 16 bits: |x| <= 448, or not finite (then NaN). Rounds to nearest even.
+__device__ __forceinline__ uint32_t two_codes(float a, float b) {
+  a = fabsf(a) <= 448.f ? a : __uint_as_float(0x7fc00000u);
+  b = fabsf(b) <= 448.f ? b : __uint_as_float(0x7fc00000u);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
+}
+
+// ===========================================================================
+// ptl_rope_store_f8: the rotation of csrc/rope.hip (same angles, same formula), the queries rounded to their type, the keys and
+// the values into their blocks.
+//
+// The tokens of a page that a call brings are a run: rows one after the other with slots one after the other. A run that
+// begins at its page's first row begins the block anew (the old scale counts no more and the rows behind the run become
+// zeros); one that begins further back takes the block as it is, and where the new tokens need a larger scale the other rows'
+// codes are rounded anew to it. So a block's content does not depend on how often the same run is stored.
+//
+// Workgroups [0, T * chunks): one for every token that begins a run (the others leave) and every chunk of kv heads; two waves take the
+// keys' heads in turn and two the values'. A wave holds the run's numbers of a head, up to HELD items of VEC pairs a lane, finds
+// the largest and then writes; runs with more items read (and rotate) the rest again. A block belongs to one wave: no
+// two waves write one scale. Behind them T workgroups that rotate the queries of one token each.
+constexpr int HELD = 2;
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256)
+rope_store_f8_kernel(T* __restrict__ q_out, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+                     long row_stride, const int32_t* __restrict__ positions, const float* __restrict__ inv_freq,
+                     const int32_t* __restrict__ slots, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
+                     float* __restrict__ k_scale, float* __restrict__ v_scale, int T_, int Hq, int Hkv, int D, int page_size,
+                     int slots_in_all, int chunks) {
+  extern __shared__ float cs[];                 // [2][D / 2]: cosines and sines of a query row's angles
+  struct __attribute__((aligned(sizeof(T) * VEC))) Vec { T e[VEC]; };
+  const int half = D >> 1, per_row = half / VEC;               // items of VEC pairs in a row of D
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int store_groups = slots ? T_ * chunks : 0;
+  if ((int)blockIdx.x >= store_groups) {
+    // ---- queries ----
+    const int t = blockIdx.x - store_groups;
+    const float pos = (float)positions[t];
+    for (int j = threadIdx.x; j < half; j += 256) {
+      float s = 0.f, c = 1.f;
+      if (inv_freq) sincosf(pos * inv_freq[j], &s, &c);
+      cs[j] = c;
+      cs[half + j] = s;
+    }
+    __syncthreads();
+    const T* row = q + (size_t)t * row_stride;
+    T* to = q_out + (size_t)t * Hq * D;
+    for (int i = threadIdx.x; i < Hq * per_row; i += 256) {
+      const int h = i / per_row, j = (i - h * per_row) * VEC;
+      Vec a = *reinterpret_cast<const Vec*>(row + h * D + j), b = *reinterpret_cast<const Vec*>(row + h * D + j + half);
+      if (inv_freq) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float x1 = to_float<T>(a.e[e]), x2 = to_float<T>(b.e[e]), c = cs[j + e], s = cs[half + j + e];
+          a.e[e] = from_float<T>(x1 * c - x2 * s);
+          b.e[e] = from_float<T>(x2 * c + x1 * s);
+        }
+      }
+      *reinterpret_cast<Vec*>(to + h * D + j) = a;
+      *reinterpret_cast<Vec*>(to + h * D + j + half) = b;
+    }
+    return;
+  }
+  // ---- keys and values ----
+  const int t0 = blockIdx.x / chunks, chunk = blockIdx.x - t0 * chunks;
+  const int slot = slots[t0];
+  if (slot < 0 || slot >= slots_in_all) return;
+  const int page = slot / page_size, off = slot - page * page_size;
+  if (off > 0 && t0 > 0 && slots[t0 - 1] == slot - 1) return;      // inside a run
+  int n = 1;                                                     // rows of the run
+  for (const int most = min(page_size - off, T_ - t0); n < most; n += 64) {
+    const bool next = n + lane < most && slots[t0 + n + lane] == slot + n + lane;
+    const unsigned long long stop = ~__ballot(next);
+    if (stop) { n += __ffsll(stop) - 1; break; }
+  }
+  const int items = n * per_row;
+  const bool values = wave >= 2;
+  const T* from = (values ? v : k) + (size_t)t0 * row_stride;
+  uint8_t* cache = values ? v_cache : k_cache;
+  float* scales = values ? v_scale : k_scale;
+  const bool turn = inv_freq && !values;
+
+  // item i of the run: VEC pairs of row i / per_row
+  auto angles = [&](int i, float (&c)[VEC], float (&s)[VEC]) {
+    const int r = i / per_row, j = (i - r * per_row) * VEC;
+    const float pos = (float)positions[t0 + r];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sincosf(pos * inv_freq[j + e], &s[e], &c[e]);
+  };
+  auto load = [&](int h, int i, const float (&c)[VEC], const float (&s)[VEC], float (&a)[VEC], float (&b)[VEC]) {
+    const int r = i / per_row, j = (i - r * per_row) * VEC;
+    const T* at = from + (size_t)r * row_stride + h * D + j;
+    const Vec x = *reinterpret_cast<const Vec*>(at), y = *reinterpret_cast<const Vec*>(at + half);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float x1 = to_float<T>(x.e[e]), x2 = to_float<T>(y.e[e]);
+      a[e] = turn ? x1 * c[e] - x2 * s[e] : x1;
+      b[e] = turn ? x2 * c[e] + x1 * s[e] : x2;
+    }
+  };
+  auto largest_of = [&](const float (&a)[VEC], float m) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float x = fabsf(a[e]);
+      m = x < INFINITY ? fmaxf(m, x) : m;
+    }
+    return m;
+  };
+  float c[HELD][VEC], s[HELD][VEC];
+#pragma unroll
+  for (int it = 0; it < HELD; ++it)
+    if (turn && lane + 64 * it < items) angles(lane + 64 * it, c[it], s[it]);
+
+  const int per_chunk = (Hkv + chunks - 1) / chunks, h_end = min(Hkv, (chunk + 1) * per_chunk);
+  for (int h = chunk * per_chunk + (wave & 1); h < h_end; h += 2) {
+    float a[HELD][VEC], b[HELD][VEC], m = 0.f;
+#pragma unroll
+    for (int it = 0; it < HELD; ++it)
+      if (lane + 64 * it < items) {
+        load(h, lane + 64 * it, c[it], s[it], a[it], b[it]);
+        m = largest_of(b[it], largest_of(a[it], m));
+      }
+    for (int i = lane + 64 * HELD; i < items; i += 64) {
+      float cc[VEC], ss[VEC], aa[VEC], bb[VEC];
+      if (turn) angles(i, cc, ss);
+      load(h, i, cc, ss, aa, bb);
+      m = largest_of(bb, largest_of(aa, m));
+    }
+    m = wave_max(m);
+    const size_t block = (size_t)page * Hkv + h;
+    uint8_t* const rows = cache + block * page_size * D;
+    int e_new = scale_exponent(m);
+    if (off > 0) {
+      const float old = scales[block];
+      const int e_old = max(-126, (int)(__float_as_uint(old) >> 23) - 127);
+      if (e_old >= e_new) {
+        e_new = e_old;
+      } else {
+        // the block's other rows are rounded anew to the larger scale (of numbers below 2^-126 nothing is left in float32)
+        const float f = e_old - e_new < -126 ? 0.f : power_of_two(e_old - e_new);
+        auto again = [&](uint32_t x) {
+          const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)x, false);
+          const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)x, true);
+          return two_codes(lo[0] * f, lo[1] * f) | two_codes(hi[0] * f, hi[1] * f) << 16;
+        };
+        // (the run's own rows are left to the writes below: lanes of a wave would write them in no certain order)
+        auto other = [&](int i) { const int r = i / D; return r < off || r >= off + n; };
+        if (D % 4 == 0) {
+          for (int i = 4 * lane; i < page_size * D; i += 256)
+            if (other(i)) *reinterpret_cast<uint32_t*>(rows + i) = again(*reinterpret_cast<const uint32_t*>(rows + i));
+        } else {                                  // D is even: two neighbours lie in one row
+          for (int i = 2 * lane; i < page_size * D; i += 128)
+            if (other(i)) *reinterpret_cast<uint16_t*>(rows + i) = (uint16_t)again(*reinterpret_cast<const uint16_t*>(rows + i));
+        }
+      }
+    } else {
+      for (int i = n * D + 2 * lane; i < page_size * D; i += 128) *reinterpret_cast<uint16_t*>(rows + i) = 0;
+    }
+    if (lane == 0) scales[block] = power_of_two(e_new);
+    const float f = power_of_two(-e_new);
+    auto put = [&](int i, const float (&x)[VEC], const float (&y)[VEC]) {
+      const int r = i / per_row, j = (i - r * per_row) * VEC;
+      uint8_t* const to = rows + (size_t)(off + r) * D + j;
+      if constexpr (VEC == 8) {
+        uint2 lo, hi;
+        lo.x = two_codes(x[0] * f, x[1] * f) | two_codes(x[2] * f, x[3] * f) << 16;
+        lo.y = two_codes(x[4] * f, x[5] * f) | two_codes(x[6] * f, x[7] * f) << 16;
+        hi.x = two_codes(y[0] * f, y[1] * f) | two_codes(y[2] * f, y[3] * f) << 16;
+        hi.y = two_codes(y[4] * f, y[5] * f) | two_codes(y[6] * f, y[7] * f) << 16;
+        *reinterpret_cast<uint2*>(to) = lo;
+        *reinterpret_cast<uint2*>(to + half) = hi;
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const uint32_t z = two_codes(x[e] * f, y[e] * f);
+          to[e] = (uint8_t)z;
+          to[half + e] = (uint8_t)(z >> 8);
+        }
+      }
+    };
+#pragma unroll
+    for (int it = 0; it < HELD; ++it)
+      if (lane + 64 * it < items) put(lane + 64 * it, a[it], b[it]);
+    for (int i = lane + 64 * HELD; i < items; i += 64) {
+      float cc[VEC], ss[VEC], aa[VEC], bb[VEC];
+      if (turn) angles(i, cc, ss);
+      load(h, i, cc, ss, aa, bb);
+      put(i, aa, bb);
+    }
+  }
+}
+
+extern "C" int ptl_rope_store_f8(void* q_out, const void* q, const void* k, const void* v, long row_stride,
+                                 const int32_t* positions, const float* inv_freq, const int32_t* slots, uint8_t* k_cache,
+                                 uint8_t* v_cache, float* k_scale, float* v_scale, int T, int Hq, int Hkv, int D, int page_size,
+                                 int pages, int dtype, hipStream_t stream) {
+  if (T <= 0) return PTL_OK;
+  if (Hq <= 0 || Hkv <= 0 || D <= 0 || (D & 1) || D > 640 || page_size <= 0 || (long)page_size * D >= 1l << 30) return PTL_ERR_ARG;
+  if (slots && (!k_cache || !v_cache || !k_scale || !v_scale)) return PTL_ERR_ARG;
+  if (((uintptr_t)k_cache | (uintptr_t)v_cache) % 16) return PTL_ERR_ARG;
+  const int in_all = slots ? (int)min((long)pages * page_size, 0x7fffffffl) : 0;
+  const int chunks = min(Hkv, 4);
+  if ((long)T * (chunks + 1) >= 1l << 31) return PTL_ERR_ARG;
+  const int groups = T + (slots ? T * chunks : 0);
+  const size_t lds = (size_t)D * sizeof(float);
+  const bool vec = (D / 2) % 8 == 0 && row_stride % 8 == 0 && ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out) % 16 == 0;
+  if (dtype == PTL_DTYPE_F32) {
+    auto go = [&](auto kernel) {
+      kernel<<<groups, 256, lds, stream>>>((float*)q_out, (const float*)q, (const float*)k, (const float*)v, row_stride, positions,
+                                           inv_freq, slots, k_cache, v_cache, k_scale, v_scale, T, Hq, Hkv, D, page_size, in_all, chunks);
+    };
+    if (vec) go(rope_store_f8_kernel<float, 8>); else go(rope_store_f8_kernel<float, 1>);
+  } else if (dtype == PTL_DTYPE_BF16) {
+    auto go = [&](auto kernel) {
+      kernel<<<groups, 256, lds, stream>>>((bf16_t*)q_out, (const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, row_stride, positions,
+                                           inv_freq, slots, k_cache, v_cache, k_scale, v_scale, T, Hq, Hkv, D, page_size, in_all, chunks);
+    };
+    if (vec) go(rope_store_f8_kernel<bf16_t, 8>); else go(rope_store_f8_kernel<bf16_t, 1>);
+  } else {
+    return PTL_ERR_ARG;
+  }
+  return ptl_launch_status();
+}
+
+// ===========================================================================
+// ptl_copy_pages: page src[i] -> page dst[i] of several pools [layers, pages, page bytes], all layers, one launch. The host has
+// checked that no page is written twice, or read and written. The page numbers travel with the launch (PAIRS of them; more are
+// more launches), so nothing is uploaded and a recorded launch keeps its own.
+constexpr int PAIRS = 256, POOLS = 16;
+struct CopyPool {
+  char* at;
+  long page_bytes, layer_bytes;
+  uint32_t units;                  // pieces of a thread's 16 bytes (or one byte) in a page
+  uint32_t pieces;                 // layers * pairs * units
+  uint32_t first_group;            // the launch's workgroups from here on are this pool's
+};
+struct CopyPages {
+  CopyPool pools[POOLS];
+  int n_pools, n_pairs;
+  int32_t src[PAIRS], dst[PAIRS];
+};
+
+constexpr int COPY_AHEAD = 4;      // pieces that a thread asks for at once
+
+template <typename V>
+__global__ void __launch_bounds__(256) copy_pages_kernel(CopyPages c) {
+  int p = 0;
+  while (p + 1 < c.n_pools && blockIdx.x >= c.pools[p + 1].first_group) ++p;
+  const CopyPool pool = c.pools[p];
+  const uint32_t first = (blockIdx.x - pool.first_group) * (256 * COPY_AHEAD) + threadIdx.x;
+  V held[COPY_AHEAD];
+  char* to[COPY_AHEAD];
+#pragma unroll
+  for (int i = 0; i < COPY_AHEAD; ++i) {
+    const uint32_t piece = min(first + 256 * i, pool.pieces - 1);       // (a thread behind the end copies the last piece too)
+    const uint32_t page = piece / pool.units, unit = piece - page * pool.units;
+    const uint32_t layer = page / c.n_pairs, pair = page - layer * c.n_pairs;
+    char* const in = pool.at + (size_t)layer * pool.layer_bytes + (size_t)unit * sizeof(V);
+    held[i] = *reinterpret_cast<const V*>(in + (size_t)c.src[pair] * pool.page_bytes);
+    to[i] = in + (size_t)c.dst[pair] * pool.page_bytes;
+  }
+#pragma unroll
+  for (int i = 0; i < COPY_AHEAD; ++i) *reinterpret_cast<V*>(to[i]) = held[i];
+}
+
+// pools: n_pools times (address, layers, pages, bytes a page) in host memory; src, dst: n page numbers in host memory.
+extern "C" int ptl_copy_pages(const long* pools, int n_pools, const int32_t* src, const int32_t* dst, int n, hipStream_t stream) {
+  if (n <= 0 || n_pools <= 0) return PTL_OK;
+  if (n_pools > POOLS || !pools || !src || !dst) return PTL_ERR_ARG;
+  bool wide = true;
+  for (int p = 0; p < n_pools; ++p) {
+    const long *d = pools + 4 * p, at = d[0], layers = d[1], pages = d[2], bytes = d[3];
+    if (!at || layers <= 0 || pages <= 0 || bytes <= 0) return PTL_ERR_ARG;
+    wide = wide && at % 16 == 0 && bytes % 16 == 0;
+    for (int i = 0; i < n; ++i)
+      if (src[i] < 0 || src[i] >= pages || dst[i] < 0 || dst[i] >= pages) return PTL_ERR_ARG;
+  }
+  const long size = wide ? 16 : 1;
+  long a_pair = 0, pairs = PAIRS;            // the pieces of a launch are counted in 32 bits
+  for (int p = 0; p < n_pools; ++p) {
+    const long one = pools[4 * p + 1] * (pools[4 * p + 3] / size);
+    if (one >= 1l << 30) return PTL_ERR_ARG;
+    a_pair += one + 256 * COPY_AHEAD;
+  }
+  pairs = min(pairs, max(1l, (1l << 30) / a_pair));
+  for (int first = 0; first < n; first += pairs) {
+    CopyPages c{};
+    c.n_pools = n_pools;
+    c.n_pairs = min((int)pairs, n - first);
+    uint32_t groups = 0;
+    for (int p = 0; p < n_pools; ++p) {
+      const long* d = pools + 4 * p;
+      CopyPool& pool = c.pools[p];
+      pool.at = (char*)d[0];
+      pool.page_bytes = d[3];
+      pool.layer_bytes = d[2] * d[3];
+      pool.units = (uint32_t)(d[3] / size);
+      pool.pieces = (uint32_t)(d[1] * c.n_pairs) * pool.units;
+      pool.first_group = groups;
+      groups += (pool.pieces + 256 * COPY_AHEAD - 1) / (256 * COPY_AHEAD);
+    }
+    for (int i = 0; i < c.n_pairs; ++i) { c.src[i] = src[first + i]; c.dst[i] = dst[first + i]; }
+    if (wide) copy_pages_kernel<ptl_u32x4_t><<<groups, 256, 0, stream>>>(c);
+    else copy_pages_kernel<uint8_t><<<groups, 256, 0, stream>>>(c);
+  }
+  return ptl_launch_status();
+}

@@ -33,7 +33,7 @@ HIPCC_FLAGS = ["--offload-arch=" + ARCH, "-O3", "-fPIC", "-shared", "-std=c++17"
 
 KERNEL_LIBRARIES = ("embedding", "norm", "rope", "attention", "attention_prefill", "attention_step", "activation",
                     "gemm", "gemm_f32", "gemm_rows", "gemm_tile", "blaslt", "sampling", "probe", "stream", "latent", "moe", "prepare", "prompt",
-                    "recurrent", "selective", "linear_scan")
+                    "recurrent", "selective", "linear_scan", "cache_f8", "attention_f8")
 # libraries a source is linked with (after the source on the command line)
 LINK_FLAGS = {"blaslt": ["-lhipblaslt"]}
 

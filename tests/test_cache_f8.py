@@ -1,0 +1,29 @@
+"""What the faces of the 8-bit cache's kernels refuse before anything is launched (no GPU needed: a refusal comes first)."""
+import pytest
+import torch
+
+from pytriton_llama_amd import ops
+
+
+def test_tensors_on_the_host_are_refused():
+    cache = torch.zeros(2, 1, 16, 64).to(ops.CACHE_F8)
+    scale = torch.ones(2, 1)
+    q = torch.zeros(1, 1, 64, dtype=torch.bfloat16)
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ops.KernelError, match="GPU"):
+        ops.rope_store_f8(q, q, q, i[:1], None, i[:1], cache, cache, scale, scale)
+    with pytest.raises(ops.KernelError, match="GPU"):
+        ops.attention_decode_f8(q, q, cache, cache, scale, scale, i, i[:1], i.view(2, 1), 1, 1.0)
+    with pytest.raises(ops.KernelError, match="GPU"):
+        ops.attention_generic_f8(q, q, cache, cache, scale, scale, i, i[:1], i.view(2, 1), i[:1], i[:1], 1.0)
+    with pytest.raises(ops.KernelError, match="GPU"):
+        ops.copy_pages([cache[None]], [0], [1])
+
+
+def test_which_sizes_the_matrix_cores_take():
+    fits = ops.attention_f8_fits
+    for D in (32, 64, 96, 128):
+        assert fits(torch.bfloat16, 32, 8, D, 16) and fits(torch.bfloat16, 40, 1, D, 64)
+        assert not fits(torch.float32, 32, 8, D, 16) and not fits(torch.bfloat16, 32, 8, D, 8)
+        assert not fits(torch.bfloat16, 32, 8, D, 24) and not fits(torch.bfloat16, 7, 2, D, 16)
+    assert not fits(torch.bfloat16, 8, 8, 160, 16) and not fits(torch.bfloat16, 8, 8, 48, 16) and not fits(torch.bfloat16, 8, 0, 64, 16)
