@@ -9,6 +9,7 @@
 #include "device.h"
 #include "mfma.h"
 #include <math.h>
+#include <type_traits>
 
 // What all kernels here are given.
 struct F8Cache {
@@ -293,18 +294,18 @@ attn_decode_f8_kernel(const int32_t* __restrict__ ctx_len, const int32_t* __rest
       t.ks[h] = *(const __attribute__((address_space(4))) float*)(uintptr_t)(k_scale + block);
       t.vs[h] = *(const __attribute__((address_space(4))) float*)(uintptr_t)(v_scale + block);
 #pragma unroll
-      for (int c = 0; c < A; ++c) t.k[h][c] = load_once(kr + ln * D + 64 * c + 16 * lg);
-      if (B) t.kb[h] = *reinterpret_cast<const uint2*>(kr + ln * D + 64 * A + 8 * lg);
+      for (int c = 0; c < A; ++c) t.k[h][c] = load_once(kr + (uint32_t)(ln * D + 64 * c + 16 * lg));
+      if (B) t.kb[h] = *reinterpret_cast<const uint2*>(kr + (uint32_t)(ln * D + 64 * A + 8 * lg));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint8_t* x = vr + (4 * lg + i) * D;
-        if constexpr (A == 1) t.v[h][i][0] = *reinterpret_cast<const uint32_t*>(x + 4 * ln);
+        const uint32_t x = (uint32_t)((4 * lg + i) * D);
+        if constexpr (A == 1) t.v[h][i][0] = *reinterpret_cast<const uint32_t*>(vr + (x + 4 * ln));
         if constexpr (A == 2) {
-          const uint2 w = *reinterpret_cast<const uint2*>(x + 8 * ln);
+          const uint2 w = *reinterpret_cast<const uint2*>(vr + (x + 8 * ln));
           t.v[h][i][0] = w.x;
           t.v[h][i][1] = w.y;
         }
-        if (B) t.vb[h][i] = *reinterpret_cast<const uint16_t*>(x + 64 * A + 2 * ln);
+        if (B) t.vb[h][i] = *reinterpret_cast<const uint16_t*>(vr + (x + 64 * A + 2 * ln));
       }
     }
   };
@@ -531,5 +532,267 @@ extern "C" int ptl_attention_decode_f8(void* out, long out_stride, const void* q
   else if (D == 64) go(attn_decode_f8_kernel<1, 0>);
   else if (D == 96) go(attn_decode_f8_kernel<1, 1>);
   else go(attn_decode_f8_kernel<2, 0>);
+  return ptl_launch_status();
+}
+
+// ===========================================================================
+// ptl_attention_prefill_f8: portions of prompts. A workgroup of four waves takes 64 RT query rows of one head, 16 RT a wave, and walks the
+// keys that they see in tiles of 64. A tile's codes come into registers, are turned into bfloat16 (with their scales) and
+// lie in LDS in two buffers: in the turn in which tile t is used, tile t + 1, which arrived during the turn before, is
+// converted into the other buffer and tile t + 2 sets out. Products, softmax and the layout of LDS are those of
+// attention_prefill.h: S^T = K Q^T, O^T += V^T P^T, sums of the rounded probabilities by one more product with ones.
+// Of a tile every wave brings 16 rows, which lie in one page: page and scales are the wave's, in scalar registers.
+template <int ND, int RT>
+__global__ void __launch_bounds__(256, ND <= 2 ? 3 : 2)
+attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* __restrict__ q, long q_stride, F8Cache cache, F8Tables tab,
+                       const int32_t* __restrict__ work_seq, const int32_t* __restrict__ work_qoff, int n_work, int Hq, int Hkv,
+                       int page_shift, int window, const float* __restrict__ sink, float scale_log2) {
+  constexpr int D = 32 * ND, BN = 64, ROWS = 64 * RT;
+  constexpr int PIECES = D / 8;                     // 8-element pieces of a row: 8 codes, 16 bytes of bfloat16
+  __shared__ __attribute__((aligned(16))) bf16_t Ks[2][BN * D], Vs[2][BN * D];
+  // piece c of row r lies at c ^ swz(r), so that neither product's reads meet in a bank
+  auto swz = [](int r) { return PIECES % 8 == 0 ? (r & 7) : ((r >> 1) & 3); };
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 15, lg = lane >> 4;
+  // heads run along x, which the eight dies take in turn: die c gets heads c Hq / 8 .. of which a kv head's lie together
+  const int head = Hq % 8 == 0 ? (blockIdx.x % 8) * (Hq / 8) + blockIdx.x / 8 : blockIdx.x;
+  const int kvh = head / (Hq / Hkv), page_mask = (1 << page_shift) - 1;
+  const uint32_t page_bytes = (uint32_t)(Hkv * D) << page_shift;
+  const uint8_t* k_head = cache.k + ((size_t)(kvh * D) << page_shift);
+  const uint8_t* v_head = cache.v + ((size_t)(kvh * D) << page_shift);
+  Frag8 ones;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ones.v[j] = (__bf16)1.0f;
+  const float lazy = 8.0f / scale_log2;             // (raw scores: the maximum follows only where they pass it by 2^8)
+  // Wave w brings rows 16 w .. +15 of a tile: 16 D bytes side by side in one page, lane l the 8 codes from 512 i + 8 l on of them
+  int plds[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) {
+    const int r = (64 * i + lane) / PIECES, c = 64 * i + lane - r * PIECES;
+    plds[i] = (16 * wave + r) * D + (c ^ swz(r)) * 8;
+  }
+  // where this lane reads: the first product takes row 16 kt + ln, piece 4 kk + lg; the second points at row
+  // 32 half + 16 j + 4 lg + ln / 4, elements 16 dt + 4 (ln % 4) .. +3
+  int k_at[ND], v_at[2 * ND];
+#pragma unroll
+  for (int kk = 0; kk < ND; ++kk) k_at[kk] = ln * D + 8 * ((4 * kk + lg) ^ swz(ln));
+  {
+    const int r = 4 * lg + (ln >> 2);
+#pragma unroll
+    for (int dt = 0; dt < 2 * ND; ++dt) v_at[dt] = r * D + 8 * ((2 * dt + ((ln & 3) >> 1)) ^ swz(r)) + 4 * (ln & 1);
+  }
+
+  // the list is sorted, most keys first; the workgroups of a head walk it forwards and backwards in turn
+  for (int round = 0;; ++round) {
+    const int item = round * gridDim.y + ((round & 1) ? gridDim.y - 1 - blockIdx.y : blockIdx.y);
+    if (item >= n_work) break;
+    const int seq = work_seq[item], qoff = work_qoff[item];
+    const int first = tab.q_start[seq], qlen = tab.q_start[seq + 1] - first, ctx = tab.ctx_len[seq];
+    const int rows = min(ROWS, qlen - qoff);
+    if (rows <= 0) continue;
+    const int32_t* bt = tab.block_table + (size_t)seq * tab.bt_stride;
+    const int first_q = ctx - qlen + qoff;          // position of the block's first row
+    int qpos[RT], lo[RT];
+    bool row_ok[RT];
+    Frag8 qf[RT][ND];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int mine = 16 * (RT * wave + r) + ln;
+      row_ok[r] = mine < rows;
+      const int qrow = row_ok[r] ? mine : 0;        // (rows behind the end repeat the first; they are not stored)
+      qpos[r] = first_q + qrow;
+      lo[r] = window > 0 ? max(0, qpos[r] - window + 1) : 0;
+      const bf16_t* x = q + (size_t)(first + qoff + qrow) * q_stride + (size_t)head * D + 8 * lg;
+#pragma unroll
+      for (int kk = 0; kk < ND; ++kk) qf[r][kk].u = load16(x + 32 * kk);
+    }
+    const int wave_first = 16 * RT * wave;
+    const bool wave_has_rows = wave_first < rows;
+    const int min_q = first_q + (wave_has_rows ? wave_first : 0), max_q = first_q + min(rows, wave_first + 16 * RT) - 1;
+    const int wave_lo = window > 0 ? max(0, min_q - window + 1) : 0, wave_lo_last = window > 0 ? max(0, max_q - window + 1) : 0;
+    f32x4_t o[RT][2 * ND + 1];
+    float m_run[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      m_run[r] = -INFINITY;
+#pragma unroll
+      for (int t = 0; t <= 2 * ND; ++t) o[r][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    const int k_lo = window > 0 ? max(0, first_q - window + 1) : 0, k_end = min(ctx, first_q + rows);
+    const int k_begin = k_lo / BN * BN, n_tiles = (k_end - k_begin + BN - 1) / BN;
+
+    uint2 kc[ND], vc[ND];
+    float ks, vs;
+    int page;
+    auto load_page = [&](int t) {
+      const int kp = min(max(k_begin + t * BN + 16 * wave, k_lo), max(k_end - 1, 0));     // (of rows that are no keys: of one that is)
+      page = *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)(bt + __builtin_amdgcn_readfirstlane(kp >> page_shift));
+    };
+    auto load = [&](int t) __attribute__((always_inline)) {
+      const uint64_t at = (uint64_t)(uint32_t)page * page_bytes + (uint32_t)(((k_begin + t * BN + 16 * wave) & page_mask) * D);
+      const uint8_t *kr = k_head + at, *vr = v_head + at;
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        kc[i] = *reinterpret_cast<const uint2*>(kr + (uint32_t)(512 * i + 8 * lane));
+        vc[i] = *reinterpret_cast<const uint2*>(vr + (uint32_t)(512 * i + 8 * lane));
+      }
+      const size_t block = (size_t)page * Hkv + kvh;
+      ks = *(const __attribute__((address_space(4))) float*)(uintptr_t)(cache.k_scale + block);
+      vs = *(const __attribute__((address_space(4))) float*)(uintptr_t)(cache.v_scale + block);
+    };
+    auto convert = [&](int t, bf16_t* Kb, bf16_t* Vb) __attribute__((always_inline)) {
+      const int k0 = k_begin + t * BN + 16 * wave;
+      if (k0 < k_lo || k0 + 16 > k_end) {           // rows that are no keys read as zeros (what lies there may be a NaN)
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+          const int k = k0 + (64 * i + lane) / PIECES;
+          if (k < k_lo || k >= k_end) kc[i] = vc[i] = make_uint2(0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        *reinterpret_cast<bf16x8_t*>(Kb + plds[i]) = eight_bf16(kc[i].x, kc[i].y, ks);
+        *reinterpret_cast<bf16x8_t*>(Vb + plds[i]) = eight_bf16(vc[i].x, vc[i].y, vs);
+      }
+    };
+    auto tile = [&](int k0, const bf16_t* Kb, const bf16_t* Vb, auto masked_tag) __attribute__((always_inline)) {
+      constexpr bool MASKED = decltype(masked_tag)::value;
+      f32x4_t st[RT][4];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) st[r][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < ND; ++kk) {
+          Frag8 a;
+          a.u = *reinterpret_cast<const uint4*>(Kb + 16 * kt * D + k_at[kk]);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) st[r][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, qf[r][kk].v, st[r][kt], 0, 0, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      Frag8 p[RT][2];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        if (MASKED) {
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int k = k0 + 16 * kt + 4 * lg + i;
+              st[r][kt][i] = k <= qpos[r] && k < k_end && k >= lo[r] ? st[r][kt][i] : -INFINITY;
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = __builtin_elementwise_maximum(top, st[r][kt][i]);
+        top = max_with_lane_xor32(max_with_lane_xor16(top));
+        if (top > m_run[r] + lazy) {
+          const float keep = __builtin_amdgcn_exp2f((m_run[r] - top) * scale_log2);
+          m_run[r] = top;
+#pragma unroll
+          for (int t = 0; t <= 2 * ND; ++t) { o[r][t][0] *= keep; o[r][t][1] *= keep; o[r][t][2] *= keep; o[r][t][3] *= keep; }
+        }
+        const float mc = (MASKED && m_run[r] == -INFINITY) ? 0.f : -m_run[r] * scale_log2;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              p[r][half].v[4 * t + i] = (__bf16)__builtin_amdgcn_exp2f(fmaf(st[r][2 * half + t][i], scale_log2, mc));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      auto transposed = [&](const bf16_t* x) {
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)x);
+      };
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int dt = 0; dt < 2 * ND; ++dt) {
+          Frag8 a;
+          a.s[0] = transposed(Vb + 32 * half * D + v_at[dt]);
+          a.s[1] = transposed(Vb + (32 * half + 16) * D + v_at[dt]);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, p[r][half].v, o[r][dt], 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) o[r][2 * ND] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones.v, p[r][half].v, o[r][2 * ND], 0, 0, 0);
+      }
+    };
+    auto turn = [&](int t, int buffer) __attribute__((always_inline)) {
+      const int k0 = k_begin + t * BN;
+      if (t + 1 < n_tiles) {
+        convert(t + 1, Ks[1 - buffer], Vs[1 - buffer]);
+        if (t + 2 < n_tiles) { load(t + 2); load_page(t + 3); }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (wave_has_rows && k0 <= max_q && k0 + BN > wave_lo) {
+        const bool need_mask = k0 + BN - 1 > min_q || k0 + BN > k_end || k0 < wave_lo_last;
+        if (need_mask) tile(k0, Ks[buffer], Vs[buffer], std::true_type{});
+        else tile(k0, Ks[buffer], Vs[buffer], std::false_type{});
+      }
+      __syncthreads();
+    };
+    if (n_tiles > 0) {
+      load_page(0);
+      load(0);
+      load_page(1);
+      convert(0, Ks[0], Vs[0]);
+      if (n_tiles > 1) { load(1); load_page(2); }
+    }
+    __syncthreads();
+    for (int t = 0; t < n_tiles; t += 2) {
+      turn(t, 0);
+      if (t + 1 < n_tiles) turn(t + 1, 1);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      float l = o[r][2 * ND][0];
+      if (sink) l += __builtin_amdgcn_exp2f(sink[head] * 1.4426950408889634f - m_run[r] * scale_log2);
+      if (!row_ok[r]) continue;
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      bf16_t* to = out + (size_t)(first + qoff + 16 * (RT * wave + r) + ln) * out_stride + (size_t)head * D + 4 * lg;
+#pragma unroll
+      for (int dt = 0; dt < 2 * ND; ++dt) {
+        union { uint2 u; bf16_t e[4]; } x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.e[i] = float_to_bf16(o[r][dt][i] * inv);
+        *reinterpret_cast<uint2*>(to + 16 * dt) = x.u;
+      }
+    }
+  }
+}
+
+extern "C" int ptl_attention_prefill_f8(void* out, long out_stride, const void* q, long q_stride, const uint8_t* k, const uint8_t* v,
+                                        const float* k_scale, const float* v_scale, const int32_t* q_start, const int32_t* ctx_len,
+                                        const int32_t* block_table, int bt_stride, const int32_t* work_seq, const int32_t* work_qoff,
+                                        int n_work, int groups, int block_rows, int Hq, int Hkv, int D, int page_size, int window,
+                                        const float* sink, float scale, hipStream_t stream) {
+  if (n_work <= 0) return PTL_OK;
+  if (!f8_matrix_sizes(Hq, Hkv, D, page_size) || window < 0 || groups <= 0 || groups > 65535 || (block_rows != 64 && block_rows != 128) ||
+      !(scale > 0.f) || ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 || q_stride % 8 || (uintptr_t)out % 8 || out_stride % 4)
+    return PTL_ERR_ARG;
+  const F8Cache cache{k, v, k_scale, v_scale};
+  const F8Tables tab{q_start, ctx_len, block_table, bt_stride};
+  int shift = 0;
+  while (1 << shift < page_size) ++shift;
+  auto go = [&](auto kernel) {
+    kernel<<<dim3(Hq, groups), 256, 0, stream>>>((bf16_t*)out, out_stride, (const bf16_t*)q, q_stride, cache, tab, work_seq, work_qoff,
+                                                 n_work, Hq, Hkv, shift, window, sink, scale * 1.4426950408889634f);
+  };
+  if (block_rows == 64) {
+    if (D == 32) go(attn_prefill_f8_kernel<1, 1>);
+    else if (D == 64) go(attn_prefill_f8_kernel<2, 1>);
+    else if (D == 96) go(attn_prefill_f8_kernel<3, 1>);
+    else go(attn_prefill_f8_kernel<4, 1>);
+  } else {
+    if (D == 32) go(attn_prefill_f8_kernel<1, 2>);
+    else if (D == 64) go(attn_prefill_f8_kernel<2, 2>);
+    else if (D == 96) go(attn_prefill_f8_kernel<3, 2>);
+    else go(attn_prefill_f8_kernel<4, 2>);
+  }
   return ptl_launch_status();
 }

@@ -142,7 +142,7 @@ def attention_generic_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
 
 
 def attention_f8_fits(dtype: torch.dtype, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> bool:
-    """Whether ``attention_decode_f8`` takes this case: bfloat16, head size 32, 64, 96 or 128, a
+    """Whether ``attention_decode_f8`` and ``attention_prefill_f8`` take this case: bfloat16, head size 32, 64, 96 or 128, a
     page size from 16 on that is a power of two, pages (of all kv heads) below 2 GiB."""
     return (dtype == torch.bfloat16 and head_dim % 32 == 0 and 0 < head_dim <= 128 and page_size >= 16
             and page_size & (page_size - 1) == 0 and num_kv_heads > 0 and num_heads % num_kv_heads == 0
@@ -176,6 +176,32 @@ def attention_decode_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tenso
         _ptr(v_scale), _ptr(q_start), _ptr(ctx_len), _ptr(block_table), int(block_table.stride(0)), ctypes.c_void_p(at),
         ctypes.c_void_p(at + 4 * heads * D), _ptr(tickets), cuts, int(n_seq), Hq, Hkv, D, page_size, int(window), _ptr(sink),
         ctypes.c_float(scale), _stream()), "attention_decode_f8")
+
+
+def attention_prefill_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                         v_scale: torch.Tensor, q_start: torch.Tensor, ctx_len: torch.Tensor, block_table: torch.Tensor,
+                         work_seq: torch.Tensor, work_qoff: torch.Tensor, scale: float, window: int = 0, block_rows: int = 64,
+                         groups: int = 0, sink: Optional[torch.Tensor] = None) -> None:
+    """``attention_prefill_mfma`` over an 8-bit cache (``attention_f8_fits`` says for which sizes): the work list names query blocks
+    of ``block_rows`` (64 or 128) rows, those with the most keys first; ``groups`` workgroups a head share it (0: one for
+    every block)."""
+    T, Hq, Hkv, D, page_size = _attention("attention_prefill_f8", out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len,
+                                          block_table, window, sink, work_seq, work_qoff)
+    if not attention_f8_fits(q.dtype, Hq, Hkv, D, page_size):
+        raise KernelError("attention_prefill_f8: needs bfloat16, a head size of 32/64/96/128, a page size from 16 on that is a power "
+                          "of two")
+    if q.stride(0) % 8 or out.stride(0) % 4 or q.data_ptr() % 16 or out.data_ptr() % 8:
+        raise KernelError("attention_prefill_f8: q rows must be 16-byte aligned, out rows 8-byte")
+    if block_rows not in (64, 128):
+        raise KernelError("attention_prefill_f8: query blocks are 64 or 128 rows")
+    if not scale > 0:
+        raise KernelError("attention_prefill_f8: scale must be positive")
+    n = _work("attention_prefill_f8", work_seq, work_qoff)
+    _check(library.load("attention_f8").ptl_attention_prefill_f8(
+        _ptr(out), ctypes.c_long(out.stride(0)), _ptr(q), ctypes.c_long(q.stride(0)), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
+        _ptr(v_scale), _ptr(q_start), _ptr(ctx_len), _ptr(block_table), int(block_table.stride(0)), _ptr(work_seq), _ptr(work_qoff),
+        n, min(n, int(groups), 65535) if groups > 0 else min(n, 65535), int(block_rows), Hq, Hkv, D, page_size, int(window),
+        _ptr(sink), ctypes.c_float(scale), _stream()), "attention_prefill_f8")
 
 
 def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:

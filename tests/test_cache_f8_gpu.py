@@ -308,6 +308,30 @@ def test_decode_of_scores_that_are_no_numbers(ops):
     assert got[1, 1].all() and not got[1, 0].any() and not got[0].any() and not got[2].any()
 
 
+PREFILLS = [  # Hq, Hkv, D, page size, window
+    (8, 2, 64, 16, 0), (8, 2, 128, 16, 0), (6, 2, 96, 32, 0), (5, 1, 32, 64, 0), (4, 4, 128, 128, 0), (8, 2, 64, 16, 100),
+    (8, 2, 128, 16, 1), (6, 2, 96, 16, 33), (2, 2, 64, 1024, 130),
+]
+PREFILL_SEQS = [(1, 1), (1, 90), (1, 0), (2, 2), (5, 5), (64, 64), (65, 65), (3, 128), (70, 203), (128, 128), (17, 33), (200, 431)]
+
+
+@pytest.mark.parametrize("rows,groups", [(64, 0), (64, 3), (128, 0), (128, 2)])
+@pytest.mark.parametrize("Hq,Hkv,D,P,window", PREFILLS)
+def test_prefill(ops, Hq, Hkv, D, P, window, rows, groups):
+    s = Step(torch.bfloat16, Hq, Hkv, D, P, PREFILL_SEQS, window, seed=Hq + D, spread=1.5).device()
+    ops.attention_prefill_f8(s.out, s.qd, *s.cache, *s.tables, *s.blocks(rows), s.scale, window, rows, groups)
+    s.check(matrix_cores=True)
+
+
+@pytest.mark.parametrize("rows", [64, 128])
+def test_prefill_behind_decoding_sequences_with_a_sink(ops, rows):
+    s = Step(torch.bfloat16, 8, 4, 64, 16, [(1, 40), (1, 700), (33, 90), (150, 150)], 0, seed=7).device()
+    sink = torch.tensor([-3.0, 0.0, 2.5, 40.0, 1.0, -60.0, 5.0, 3.0], device="cuda")
+    ops.attention_prefill_f8(s.out, s.qd, *s.cache, *s.tables, *s.blocks(rows, 2), s.scale, 0, rows, 0, sink)
+    s.out[0, :] = s.out[1, :] = 77.0             # (the list's empty item names the first sequence)
+    s.check(sink, first=2, matrix_cores=True)
+
+
 # ---- copies ----------------------------------------------------------------------------------------
 POOLS = [[(3, 20, (2, 16, 64), torch.bfloat16)], [(2, 9, (3, 5, 7), torch.float32), (2, 9, (3,), torch.float32)],
          [(4, 600, (2, 16, 32), F8), (4, 600, (2, 16, 32), F8), (4, 600, (2,), torch.float32), (4, 600, (2,), torch.float32)],
