@@ -181,10 +181,13 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return
 // ptl_attention_decode_f8: the sequences of a step that bring one token each.
 //
 // The keys of a (sequence, kv head) pair are cut into parts of ``piece`` units of 128 keys, the same piece for all sequences: as
-// long as lets the parts of all of them fit the launch, which has room for ``cuts`` parts beside one a sequence
-// (sum of ceil(n_s / piece) <= sum of n_s / piece + sequences). Every workgroup finds the piece and its own part from the context
-// lengths on the device, so a recorded launch suits whatever contexts it is replayed with. A pair's parts are merged by the
-// workgroup that is done last (a ticket), in the order of the keys.
+// long as makes some ``cap`` parts of all of them, a workgroup a compute unit. (Sum of ceil(n_s / piece) <= cap + sequences, which
+// the launch has room for.) Every workgroup finds the piece and its own part from the context lengths on the device, so a
+// recorded launch suits whatever contexts it is replayed with. A pair's parts are merged by the workgroup that is done last
+// (a ticket), in the order of the keys. More and smaller parts hide more latency, fewer meet sooner and leave no
+// second round: us with one, two and three workgroups a compute unit, 8 kv heads: 1 x 8,000 keys of 64 10.6 12.7 12.6, 8 x 2,048 of 64
+// 12.7 12.1 12.5, 64 x 61 to 2,610 of 64 25.4 26.8 26.6; 4 x 3,000 of 128 13.7 15.0 16.0, 8 x 5,000 to 7,000 of 128 27.3 26.2 29.0,
+// 20 x 130 to 2,900 of 128 23.5 21.6 22.0, 2 x 120,000 of 128 95.8 95.5 98.4.
 //
 // A workgroup has four waves, which take tiles of 32 keys in turn. Both products are transposed, as in attention_decode.h:
 //   S^T[key, head] = K . Q^T        A = K: lane (ln, lg) has key ln's k-values, straight from memory
@@ -198,17 +201,20 @@ struct DecodeF8Parts {
 };
 
 constexpr int UNIT_F8 = 128;       // keys of a workgroup's turn
+constexpr int MOST_PARTS_F8 = 128; // parts of a pair
+constexpr int WHOLE_F8 = 4;        // units up to which a pair is not cut: a turn is some 0.8 us, parts that meet cost 3
 
 template <int A, int B>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, A + B <= 1 ? 4 : 3)
 attn_decode_f8_kernel(const int32_t* __restrict__ ctx_len, const int32_t* __restrict__ block_table, const uint8_t* __restrict__ k_cache,
-                      const uint8_t* __restrict__ v_cache, int n_seq, int Hkv, int cuts, int bt_stride, int page_shift,
+                      const uint8_t* __restrict__ v_cache, int n_seq, int Hkv, int cap, int bt_stride, int page_shift,
                       const bf16_t* __restrict__ q, long q_stride, const float* __restrict__ k_scale,
                       const float* __restrict__ v_scale, int Hq, bf16_t* __restrict__ out, long out_stride,
                       const int32_t* __restrict__ q_start, DecodeF8Parts parts, int window, const float* __restrict__ sink,
                       float scale_log2) {
   constexpr int D = 64 * A + 32 * B, NT = D / 16, STEPS = D / 32;
-  constexpr int REGION = 16 * D + 32;               // floats of a wave's sums
+  constexpr int REGION = D == 32 ? 608 : 16 * D + 32;         // floats of a wave's sums
+  static_assert(4 * REGION >= MOST_PARTS_F8 * 16 + 192 * 2, "the merge's weights and sums lie there too");
   __shared__ __attribute__((aligned(16))) float regions[4][REGION];
   __shared__ int last;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -225,10 +231,13 @@ attn_decode_f8_kernel(const int32_t* __restrict__ ctx_len, const int32_t* __rest
   for (int s0 = 0; s0 < n_seq; s0 += 64) total += s0 + lane < n_seq ? units_of(s0 + lane) : 0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
-  const int piece = max(1, (total + cuts - 1) / cuts);
+  // (a sequence's last part is half a piece on average, so that many fewer whole ones fit ``cap`` parts)
+  const int whole = max(cap - n_seq / 2, (3 * cap + 3) / 4);
+  const int piece = __builtin_amdgcn_readfirstlane(max(1, (total + whole - 1) / whole));
   int seq = -1, split = 0, n_parts = 0, before = 0;
   for (int s0 = 0; s0 < n_seq && seq < 0; s0 += 64) {
-    const int mine = s0 + lane < n_seq ? max(1, (units_of(s0 + lane) + piece - 1) / piece) : 0;
+    const int units = s0 + lane < n_seq ? units_of(s0 + lane) : 0;
+    const int mine = s0 + lane < n_seq ? (units <= WHOLE_F8 ? 1 : (units + piece - 1) / piece) : 0;
     int upto = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -245,11 +254,14 @@ attn_decode_f8_kernel(const int32_t* __restrict__ ctx_len, const int32_t* __rest
     before += __builtin_amdgcn_readlane(upto, 63);
   }
   if (seq < 0) return;                              // (more room than parts)
+  // (the same in all lanes, which the compiler cannot see: loops, branches and addresses below become scalar)
   seq = __builtin_amdgcn_readfirstlane(seq);
-  const int ctx = ctx_len[seq], row = q_start[seq];
+  split = __builtin_amdgcn_readfirstlane(split);
+  n_parts = __builtin_amdgcn_readfirstlane(n_parts);
+  const int ctx = __builtin_amdgcn_readfirstlane(ctx_len[seq]), row = __builtin_amdgcn_readfirstlane(q_start[seq]);
   const int k_lo = window > 0 ? max(0, ctx - window) : 0;
   const int k_first = (k_lo & ~15) + split * piece * UNIT_F8;
-  const int k_end = min(ctx, k_first + piece * UNIT_F8);
+  const int k_end = n_parts == 1 ? ctx : min(ctx, k_first + piece * UNIT_F8);
   const int head0 = kvh * G + 16 * tile;
   const int32_t* bt = block_table + (size_t)seq * bt_stride;
   const uint32_t page_bytes = (uint32_t)(Hkv * D) << page_shift;          // < 4 GiB, checked by the host
@@ -342,19 +354,22 @@ attn_decode_f8_kernel(const int32_t* __restrict__ ctx_len, const int32_t* __rest
       }
       if (B) st[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16(t.kb[h].x, t.kb[h].y, t.ks[h]), qf[2 * A].v, st[h], 0, 0, 0);
     }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) st[h] *= scale_log2;
+    if (!whole) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = kc + 16 * h + 4 * lg + i;
+          st[h][i] = key >= k_lo && key < k_end ? st[h][i] : -INFINITY;
+        }
+    }
     float top = -INFINITY;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float s = st[h][i] * scale_log2;
-        if (!whole) {
-          const int key = kc + 16 * h + 4 * lg + i;
-          s = key >= k_lo && key < k_end ? s : -INFINITY;
-        }
-        st[h][i] = s;
-        top = __builtin_elementwise_maximum(top, s);
-      }
+      for (int i = 0; i < 4; ++i) top = __builtin_elementwise_maximum(top, st[h][i]);
     top = max_with_lane_xor32(max_with_lane_xor16(top));
     // the maximum follows only when the scores pass it by 2^8: until then float32 sums and bfloat16 probabilities hold as well
     if (top > m_run + 8.0f) {
@@ -464,36 +479,70 @@ attn_decode_f8_kernel(const int32_t* __restrict__ ctx_len, const int32_t* __rest
   if (threadIdx.x == 0) last = last_part(parts.tickets + (((size_t)seq * Hkv + kvh) * tiles + tile) * TICKET, n_parts);
   __syncthreads();
   if (!last) return;
+  // ---- the last workgroup of the pair merges its parts ----
+  // A thread takes two columns of AHEAD parts at a time; where that leaves threads, two or four groups of them share the parts.
+  // What they read first is on its way while the parts' weights are made (parts that are none weigh nothing): a part
+  // lies some 2 us off.
   const size_t part_heads = (size_t)Hkv * G, first = group - (size_t)split * part_heads;
-  constexpr int AHEAD = 8;                                  // parts that are asked for at once: they lie a long way off
-  for (int i = threadIdx.x; i < GT * D; i += 256) {
-    const int h = i / D, d = i - h * D;
-    const float *acc = parts.acc + (first + h) * D + d, *ml = parts.ml + (first + h) * 2;
-    float m = -INFINITY, l = 0.f, a = 0.f;
-    for (int s0 = 0; s0 < n_parts; s0 += AHEAD) {
-      float av[AHEAD];
-      float2 e[AHEAD];
+  constexpr int AHEAD = 16, PAIRS_D = D / 2;
+  float* const weight = regions[0];                         // [part][GT]
+  float2* const sums = reinterpret_cast<float2*>(regions[0] + MOST_PARTS_F8 * 16);
+  __shared__ float totals[16], tops[16];
+  const int columns = GT * PAIRS_D, group_size = columns <= 64 ? 64 : columns <= 128 ? 128 : 256;
+  const int side = __builtin_amdgcn_readfirstlane(threadIdx.x / group_size), in_side = threadIdx.x & (group_size - 1);
+  const int sides = 256 / group_size, turns_all = (n_parts + AHEAD - 1) / AHEAD, share = (turns_all + sides - 1) / sides * AHEAD;
+  const int p_begin = side * share, p_end = min(p_begin + share, turns_all * AHEAD);       // (of a last group also none)
+  float2 av[AHEAD];
+  auto ask = [&](int i, int p0) __attribute__((always_inline)) {
+    const uint32_t column = 2 * min(i, columns - 1);
 #pragma unroll
-      for (int s = 0; s < AHEAD; ++s) {
-        const size_t at = min(s0 + s, n_parts - 1) * part_heads;
-        e[s] = get_shared2(ml + 2 * at);
-        av[s] = get_shared(acc + at * D);
-      }
-      float top = m;
+    for (int s = 0; s < AHEAD; ++s) av[s] = get_shared2(parts.acc + (first + min(p0 + s, n_parts - 1) * part_heads) * D + column);
+  };
+  if (p_begin < p_end) ask(in_side, p_begin);
+  for (int h = wave; h < GT; h += 4) {                      // a wave a head, a lane a part (and a second one)
+    const float* ml = parts.ml + (first + h) * 2;
+    float2 e[2];
+    static_assert(MOST_PARTS_F8 <= 128, "two parts a lane");
 #pragma unroll
-      for (int s = 0; s < AHEAD; ++s) top = fmaxf(top, e[s].x);
-      const float to = top == -INFINITY ? 0.f : top, keep = __builtin_amdgcn_exp2f(m - to);
-      l *= keep;
-      a *= keep;
+    for (int x = 0; x < 2; ++x) e[x] = lane + 64 * x < n_parts ? get_shared2(ml + (lane + 64 * x) * part_heads * 2) : make_float2(-INFINITY, 0.f);
+    const float m = wave_max(fmaxf(e[0].x, e[1].x)), to = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
 #pragma unroll
-      for (int s = 0; s < AHEAD; ++s) {
-        const float f = s0 + s < n_parts ? __builtin_amdgcn_exp2f(e[s].x - to) : 0.f;
-        l = fmaf(e[s].y, f, l);
-        a = fmaf(av[s], f, a);
-      }
-      m = top;
+    for (int x = 0; x < 2; ++x) {
+      const float f = __builtin_amdgcn_exp2f(e[x].x - to);
+      if (lane + 64 * x < turns_all * AHEAD) weight[(lane + 64 * x) * GT + h] = f;
+      l = fmaf(e[x].y, f, l);
     }
-    write(h, d, m, l, a);
+    l = wave_sum(l);
+    if (lane == 0) { totals[h] = l; tops[h] = m; }
+  }
+  __syncthreads();
+  for (int i = in_side; i - in_side < columns; i += group_size) {
+    const int h = min(i / PAIRS_D, GT - 1), d = 2 * (i % PAIRS_D);
+    float2 a = make_float2(0.f, 0.f);
+    for (int p0 = p_begin; p0 < p_end; p0 += AHEAD) {
+      if (i != in_side || p0 != p_begin) ask(i, p0);
+#pragma unroll
+      for (int s = 0; s < AHEAD; ++s) {
+        const float f = weight[(p0 + s) * GT + h];
+        a.x = fmaf(av[s].x, f, a.x);
+        a.y = fmaf(av[s].y, f, a.y);
+      }
+    }
+    if (sides > 1) {                                        // (then this is the only round)
+      if (side) sums[threadIdx.x - group_size] = a;
+      __syncthreads();
+      if (side) return;
+      for (int g = 0; g < sides - 1; ++g) {
+        const float2 other = sums[g * group_size + in_side];
+        a.x += other.x;
+        a.y += other.y;
+      }
+    }
+    if (i < columns) {
+      write(h, d, tops[h], totals[h], a.x);
+      write(h, d + 1, tops[h], totals[h], a.y);
+    }
   }
 }
 
@@ -502,30 +551,23 @@ static bool f8_matrix_sizes(int Hq, int Hkv, int D, int page_size) {
          (page_size & (page_size - 1)) == 0 && (long)Hkv * D * page_size < 1l << 31;
 }
 
-// Room for parts beside one a sequence: what fills the compute units a few times over.
-extern "C" int ptl_attention_decode_f8_cuts(int n_seq, int Hkv, int Hq) {
-  if (n_seq <= 0 || Hkv <= 0 || Hq < Hkv) return 0;
-  const int tiles = (Hq / Hkv + 15) / 16, want = 3 * compute_units() / (Hkv * tiles);
-  return max(1, want > n_seq ? want - n_seq : n_seq);
-}
-
 extern "C" int ptl_attention_decode_f8(void* out, long out_stride, const void* q, long q_stride, const uint8_t* k, const uint8_t* v,
                                        const float* k_scale, const float* v_scale, const int32_t* q_start, const int32_t* ctx_len,
-                                       const int32_t* block_table, int bt_stride, float* acc, float* ml, int* tickets, int cuts,
+                                       const int32_t* block_table, int bt_stride, float* acc, float* ml, int* tickets, int cap,
                                        int n_seq, int Hq, int Hkv, int D, int page_size, int window, const float* sink, float scale,
                                        hipStream_t stream) {
   if (n_seq <= 0) return PTL_OK;
-  if (!f8_matrix_sizes(Hq, Hkv, D, page_size) || cuts <= 0 || window < 0 || !acc || !ml || !tickets ||
+  if (!f8_matrix_sizes(Hq, Hkv, D, page_size) || cap <= 0 || cap > MOST_PARTS_F8 || n_seq >= 1 << 24 || window < 0 || !acc || !ml || !tickets ||
       ((uintptr_t)ml % 8) || ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 || q_stride % 8)
     return PTL_ERR_ARG;
-  const long groups = ((long)n_seq + cuts) * Hkv;
+  const long groups = (long)(n_seq + cap) * Hkv;
   if (groups >= 1l << 31) return PTL_ERR_ARG;
   const dim3 grid((unsigned)groups, (Hq / Hkv + 15) / 16);
   int shift = 0;
   while (1 << shift < page_size) ++shift;
   const DecodeF8Parts parts{acc, ml, tickets};
   auto go = [&](auto kernel) {
-    kernel<<<grid, 256, 0, stream>>>(ctx_len, block_table, k, v, n_seq, Hkv, cuts, bt_stride, shift, (const bf16_t*)q, q_stride, k_scale,
+    kernel<<<grid, 256, 0, stream>>>(ctx_len, block_table, k, v, n_seq, Hkv, cap, bt_stride, shift, (const bf16_t*)q, q_stride, k_scale,
                                      v_scale, Hq, (bf16_t*)out, out_stride, q_start, parts, window, sink, scale * 1.4426950408889634f);
   };
   if (D == 32) go(attn_decode_f8_kernel<0, 1>);

@@ -34,24 +34,142 @@ __device__ __forceinline__ uint32_t two_codes(float a, float b) {
 // zeros); one that begins further back takes the block as it is, and where the new tokens need a larger scale the other rows'
 // codes are rounded anew to it. So a block's content does not depend on how often the same run is stored.
 //
-// Workgroups [0, T * chunks): one for every token that begins a run (the others leave) and every chunk of kv heads; two waves take the
-// keys' heads in turn and two the values'. A wave holds the run's numbers of a head, up to HELD items of VEC pairs a lane, finds
-// the largest and then writes; runs with more items read (and rotate) the rest again. A block belongs to one wave: no
-// two waves write one scale. Behind them T workgroups that rotate the queries of one token each.
+// The first workgroups store: every one makes the list of the rows that begin a run (of LISTED rows at a time) and its waves take
+// the tasks (run, kv head, keys or values) in turn, so a block belongs to one wave and no two waves write one scale. (A workgroup for
+// every row, most of which find that they begin nothing and leave, took 71 us where this takes X: 2,048 rows, 8 kv heads of 128.)
+// A wave holds the run's numbers of a head, up to HELD items of VEC pairs a lane, finds the largest and then
+// writes; runs with more items read (and rotate) the rest again. Behind them T workgroups that rotate the queries of one row each.
+constexpr int LISTED = 2048;
 constexpr int HELD = 2;
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256)
+__device__ __forceinline__ void
+store_run(int t0, int h, bool values, int lane, const T* __restrict__ k, const T* __restrict__ v, long row_stride,
+          const int32_t* __restrict__ positions, const float* __restrict__ inv_freq, const int32_t* __restrict__ slots,
+          uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache, float* __restrict__ k_scale, float* __restrict__ v_scale, int T_,
+          int Hkv, int D, int page_size) {
+  struct __attribute__((aligned(sizeof(T) * VEC))) Vec { T e[VEC]; };
+  const int half = D >> 1, per_row = half / VEC;               // items of VEC pairs in a row of D
+  const int slot = slots[t0], page = slot / page_size, off = slot - page * page_size;
+  int n = 1;                                                     // rows of the run
+  for (const int most = min(page_size - off, T_ - t0); n < most; n += 64) {
+    const bool next = n + lane < most && slots[t0 + n + lane] == slot + n + lane;
+    const unsigned long long stop = ~__ballot(next);
+    if (stop) { n += __ffsll(stop) - 1; break; }
+  }
+  n = __builtin_amdgcn_readfirstlane(n);
+  const int items = n * per_row;
+  const T* from = (values ? v : k) + (size_t)t0 * row_stride + h * D;
+  float* scale = (values ? v_scale : k_scale) + (size_t)page * Hkv + h;
+  uint8_t* const rows = (values ? v_cache : k_cache) + ((size_t)page * Hkv + h) * page_size * D;
+  const bool turn = inv_freq && !values;
+  const float old = off > 0 ? *scale : 0.f;
+
+  // item i of the run: VEC pairs of row i / per_row
+  auto load = [&](int i, float (&a)[VEC], float (&b)[VEC]) __attribute__((always_inline)) {
+    const int r = i / per_row, j = (i - r * per_row) * VEC;
+    const T* at = from + (size_t)r * row_stride + j;
+    const Vec x = *reinterpret_cast<const Vec*>(at), y = *reinterpret_cast<const Vec*>(at + half);
+    const float pos = turn ? (float)positions[t0 + r] : 0.f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float x1 = to_float<T>(x.e[e]), x2 = to_float<T>(y.e[e]);
+      float s = 0.f, c = 1.f;
+      if (turn) sincosf(pos * inv_freq[j + e], &s, &c);
+      a[e] = turn ? x1 * c - x2 * s : x1;
+      b[e] = turn ? x2 * c + x1 * s : x2;
+    }
+  };
+  auto largest_of = [&](const float (&a)[VEC], float m) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float x = fabsf(a[e]);
+      m = x < INFINITY ? fmaxf(m, x) : m;
+    }
+    return m;
+  };
+  float a[HELD][VEC], b[HELD][VEC], m = 0.f;
+#pragma unroll
+  for (int it = 0; it < HELD; ++it)
+    if (lane + 64 * it < items) {
+      load(lane + 64 * it, a[it], b[it]);
+      m = largest_of(b[it], largest_of(a[it], m));
+    }
+  for (int i = lane + 64 * HELD; i < items; i += 64) {
+    float aa[VEC], bb[VEC];
+    load(i, aa, bb);
+    m = largest_of(bb, largest_of(aa, m));
+  }
+  m = wave_max(m);
+  int e_new = scale_exponent(m);
+  if (off > 0) {
+    const int e_old = max(-126, (int)(__float_as_uint(old) >> 23) - 127);
+    if (e_old >= e_new) {
+      e_new = e_old;
+    } else {
+      // the block's other rows are rounded anew to the larger scale (of numbers below 2^-126 of it nothing is left)
+      const float f = e_old - e_new < -126 ? 0.f : power_of_two(e_old - e_new);
+      auto again = [&](uint32_t x) {
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)x, false);
+        const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)x, true);
+        return two_codes(lo[0] * f, lo[1] * f) | two_codes(hi[0] * f, hi[1] * f) << 16;
+      };
+      // (the run's own rows are left to the writes below: lanes of a wave would write them in no certain order)
+      auto other = [&](int i) { const int r = i / D; return r < off || r >= off + n; };
+      if (D % 4 == 0) {
+        for (int i = 4 * lane; i < page_size * D; i += 256)
+          if (other(i)) *reinterpret_cast<uint32_t*>(rows + i) = again(*reinterpret_cast<const uint32_t*>(rows + i));
+      } else {                                    // D is even: two neighbours lie in one row
+        for (int i = 2 * lane; i < page_size * D; i += 128)
+          if (other(i)) *reinterpret_cast<uint16_t*>(rows + i) = (uint16_t)again(*reinterpret_cast<const uint16_t*>(rows + i));
+      }
+    }
+  } else {
+    for (int i = n * D + 2 * lane; i < page_size * D; i += 128) *reinterpret_cast<uint16_t*>(rows + i) = 0;
+  }
+  if (lane == 0) *scale = power_of_two(e_new);
+  const float f = power_of_two(-e_new);
+  auto put = [&](int i, const float (&x)[VEC], const float (&y)[VEC]) __attribute__((always_inline)) {
+    const int r = i / per_row, j = (i - r * per_row) * VEC;
+    uint8_t* const to = rows + (off + r) * D + j;
+    if constexpr (VEC == 8) {
+      uint2 lo, hi;
+      lo.x = two_codes(x[0] * f, x[1] * f) | two_codes(x[2] * f, x[3] * f) << 16;
+      lo.y = two_codes(x[4] * f, x[5] * f) | two_codes(x[6] * f, x[7] * f) << 16;
+      hi.x = two_codes(y[0] * f, y[1] * f) | two_codes(y[2] * f, y[3] * f) << 16;
+      hi.y = two_codes(y[4] * f, y[5] * f) | two_codes(y[6] * f, y[7] * f) << 16;
+      *reinterpret_cast<uint2*>(to) = lo;
+      *reinterpret_cast<uint2*>(to + half) = hi;
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const uint32_t z = two_codes(x[e] * f, y[e] * f);
+        to[e] = (uint8_t)z;
+        to[half + e] = (uint8_t)(z >> 8);
+      }
+    }
+  };
+#pragma unroll
+  for (int it = 0; it < HELD; ++it)
+    if (lane + 64 * it < items) put(lane + 64 * it, a[it], b[it]);
+  for (int i = lane + 64 * HELD; i < items; i += 64) {
+    float aa[VEC], bb[VEC];
+    load(i, aa, bb);
+    put(i, aa, bb);
+  }
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256, 4)
 rope_store_f8_kernel(T* __restrict__ q_out, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                      long row_stride, const int32_t* __restrict__ positions, const float* __restrict__ inv_freq,
                      const int32_t* __restrict__ slots, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
                      float* __restrict__ k_scale, float* __restrict__ v_scale, int T_, int Hq, int Hkv, int D, int page_size,
-                     int slots_in_all, int chunks) {
+                     int slots_in_all, int store_groups) {
   extern __shared__ float cs[];                 // [2][D / 2]: cosines and sines of a query row's angles
   struct __attribute__((aligned(sizeof(T) * VEC))) Vec { T e[VEC]; };
   const int half = D >> 1, per_row = half / VEC;               // items of VEC pairs in a row of D
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int store_groups = slots ? T_ * chunks : 0;
   if ((int)blockIdx.x >= store_groups) {
     // ---- queries ----
     const int t = blockIdx.x - store_groups;
@@ -82,131 +200,42 @@ rope_store_f8_kernel(T* __restrict__ q_out, const T* __restrict__ q, const T* __
     return;
   }
   // ---- keys and values ----
-  const int t0 = blockIdx.x / chunks, chunk = blockIdx.x - t0 * chunks;
-  const int slot = slots[t0];
-  if (slot < 0 || slot >= slots_in_all) return;
-  const int page = slot / page_size, off = slot - page * page_size;
-  if (off > 0 && t0 > 0 && slots[t0 - 1] == slot - 1) return;      // inside a run
-  int n = 1;                                                     // rows of the run
-  for (const int most = min(page_size - off, T_ - t0); n < most; n += 64) {
-    const bool next = n + lane < most && slots[t0 + n + lane] == slot + n + lane;
-    const unsigned long long stop = ~__ballot(next);
-    if (stop) { n += __ffsll(stop) - 1; break; }
-  }
-  const int items = n * per_row;
-  const bool values = wave >= 2;
-  const T* from = (values ? v : k) + (size_t)t0 * row_stride;
-  uint8_t* cache = values ? v_cache : k_cache;
-  float* scales = values ? v_scale : k_scale;
-  const bool turn = inv_freq && !values;
-
-  // item i of the run: VEC pairs of row i / per_row
-  auto angles = [&](int i, float (&c)[VEC], float (&s)[VEC]) {
-    const int r = i / per_row, j = (i - r * per_row) * VEC;
-    const float pos = (float)positions[t0 + r];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) sincosf(pos * inv_freq[j + e], &s[e], &c[e]);
-  };
-  auto load = [&](int h, int i, const float (&c)[VEC], const float (&s)[VEC], float (&a)[VEC], float (&b)[VEC]) {
-    const int r = i / per_row, j = (i - r * per_row) * VEC;
-    const T* at = from + (size_t)r * row_stride + h * D + j;
-    const Vec x = *reinterpret_cast<const Vec*>(at), y = *reinterpret_cast<const Vec*>(at + half);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const float x1 = to_float<T>(x.e[e]), x2 = to_float<T>(y.e[e]);
-      a[e] = turn ? x1 * c[e] - x2 * s[e] : x1;
-      b[e] = turn ? x2 * c[e] + x1 * s[e] : x2;
+  __shared__ int16_t list[LISTED];
+  __shared__ int counts[LISTED / 64];
+  const int waves = 4 * store_groups;
+  int next = blockIdx.x * 4 + wave;                 // this wave's next task, counted from the segment's first
+  for (int seg = 0; seg < T_; seg += LISTED) {
+    const int len = min(LISTED, T_ - seg), turns = (len + 255) / 256;
+    uint32_t mine = 0;                              // the rows seg + 256 j + threadIdx.x that begin a run
+    for (int j = 0; j < turns; ++j) {
+      const int t = seg + 256 * j + threadIdx.x;
+      const int slot = t < T_ ? slots[t] : -1, before = t > 0 && t < T_ ? slots[t - 1] : -2;
+      const bool begins = slot >= 0 && slot < slots_in_all && (before != slot - 1 || before < 0 || slot % page_size == 0);
+      const unsigned long long all = __ballot(begins);
+      if (begins) mine |= 1u << j;
+      if (lane == 0) counts[4 * j + wave] = __popcll(all);
     }
-  };
-  auto largest_of = [&](const float (&a)[VEC], float m) {
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const float x = fabsf(a[e]);
-      m = x < INFINITY ? fmaxf(m, x) : m;
-    }
-    return m;
-  };
-  float c[HELD][VEC], s[HELD][VEC];
-#pragma unroll
-  for (int it = 0; it < HELD; ++it)
-    if (turn && lane + 64 * it < items) angles(lane + 64 * it, c[it], s[it]);
-
-  const int per_chunk = (Hkv + chunks - 1) / chunks, h_end = min(Hkv, (chunk + 1) * per_chunk);
-  for (int h = chunk * per_chunk + (wave & 1); h < h_end; h += 2) {
-    float a[HELD][VEC], b[HELD][VEC], m = 0.f;
-#pragma unroll
-    for (int it = 0; it < HELD; ++it)
-      if (lane + 64 * it < items) {
-        load(h, lane + 64 * it, c[it], s[it], a[it], b[it]);
-        m = largest_of(b[it], largest_of(a[it], m));
+    __syncthreads();
+    int total = 0;
+    for (int j = 0; j < turns; ++j) {
+      int at = 0;
+      for (int w = 0; w < 4; ++w) {
+        if (w == wave) at = total;
+        total += counts[4 * j + w];
       }
-    for (int i = lane + 64 * HELD; i < items; i += 64) {
-      float cc[VEC], ss[VEC], aa[VEC], bb[VEC];
-      if (turn) angles(i, cc, ss);
-      load(h, i, cc, ss, aa, bb);
-      m = largest_of(bb, largest_of(aa, m));
+      const bool begins = mine >> j & 1;
+      const unsigned long long all = __ballot(begins);
+      if (begins) list[at + __popcll(all & ((1ull << lane) - 1))] = (int16_t)(256 * j + threadIdx.x);
     }
-    m = wave_max(m);
-    const size_t block = (size_t)page * Hkv + h;
-    uint8_t* const rows = cache + block * page_size * D;
-    int e_new = scale_exponent(m);
-    if (off > 0) {
-      const float old = scales[block];
-      const int e_old = max(-126, (int)(__float_as_uint(old) >> 23) - 127);
-      if (e_old >= e_new) {
-        e_new = e_old;
-      } else {
-        // the block's other rows are rounded anew to the larger scale (of numbers below 2^-126 nothing is left in float32)
-        const float f = e_old - e_new < -126 ? 0.f : power_of_two(e_old - e_new);
-        auto again = [&](uint32_t x) {
-          const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)x, false);
-          const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)x, true);
-          return two_codes(lo[0] * f, lo[1] * f) | two_codes(hi[0] * f, hi[1] * f) << 16;
-        };
-        // (the run's own rows are left to the writes below: lanes of a wave would write them in no certain order)
-        auto other = [&](int i) { const int r = i / D; return r < off || r >= off + n; };
-        if (D % 4 == 0) {
-          for (int i = 4 * lane; i < page_size * D; i += 256)
-            if (other(i)) *reinterpret_cast<uint32_t*>(rows + i) = again(*reinterpret_cast<const uint32_t*>(rows + i));
-        } else {                                  // D is even: two neighbours lie in one row
-          for (int i = 2 * lane; i < page_size * D; i += 128)
-            if (other(i)) *reinterpret_cast<uint16_t*>(rows + i) = (uint16_t)again(*reinterpret_cast<const uint16_t*>(rows + i));
-        }
-      }
-    } else {
-      for (int i = n * D + 2 * lane; i < page_size * D; i += 128) *reinterpret_cast<uint16_t*>(rows + i) = 0;
+    __syncthreads();
+    total = __builtin_amdgcn_readfirstlane(total) * 2 * Hkv;
+    for (; next < total; next += waves) {
+      const int run = next / (2 * Hkv), task = next - run * 2 * Hkv;
+      store_run<T, VEC>(seg + __builtin_amdgcn_readfirstlane((int)list[run]), task >> 1, task & 1, lane, k, v, row_stride, positions,
+                        inv_freq, slots, k_cache, v_cache, k_scale, v_scale, T_, Hkv, D, page_size);
     }
-    if (lane == 0) scales[block] = power_of_two(e_new);
-    const float f = power_of_two(-e_new);
-    auto put = [&](int i, const float (&x)[VEC], const float (&y)[VEC]) {
-      const int r = i / per_row, j = (i - r * per_row) * VEC;
-      uint8_t* const to = rows + (size_t)(off + r) * D + j;
-      if constexpr (VEC == 8) {
-        uint2 lo, hi;
-        lo.x = two_codes(x[0] * f, x[1] * f) | two_codes(x[2] * f, x[3] * f) << 16;
-        lo.y = two_codes(x[4] * f, x[5] * f) | two_codes(x[6] * f, x[7] * f) << 16;
-        hi.x = two_codes(y[0] * f, y[1] * f) | two_codes(y[2] * f, y[3] * f) << 16;
-        hi.y = two_codes(y[4] * f, y[5] * f) | two_codes(y[6] * f, y[7] * f) << 16;
-        *reinterpret_cast<uint2*>(to) = lo;
-        *reinterpret_cast<uint2*>(to + half) = hi;
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const uint32_t z = two_codes(x[e] * f, y[e] * f);
-          to[e] = (uint8_t)z;
-          to[half + e] = (uint8_t)(z >> 8);
-        }
-      }
-    };
-#pragma unroll
-    for (int it = 0; it < HELD; ++it)
-      if (lane + 64 * it < items) put(lane + 64 * it, a[it], b[it]);
-    for (int i = lane + 64 * HELD; i < items; i += 64) {
-      float cc[VEC], ss[VEC], aa[VEC], bb[VEC];
-      if (turn) angles(i, cc, ss);
-      load(h, i, cc, ss, aa, bb);
-      put(i, aa, bb);
-    }
+    next -= total;
+    __syncthreads();
   }
 }
 
@@ -219,21 +248,22 @@ extern "C" int ptl_rope_store_f8(void* q_out, const void* q, const void* k, cons
   if (slots && (!k_cache || !v_cache || !k_scale || !v_scale)) return PTL_ERR_ARG;
   if (((uintptr_t)k_cache | (uintptr_t)v_cache) % 16) return PTL_ERR_ARG;
   const int in_all = slots ? (int)min((long)pages * page_size, 0x7fffffffl) : 0;
-  const int chunks = min(Hkv, 4);
-  if ((long)T * (chunks + 1) >= 1l << 31) return PTL_ERR_ARG;
-  const int groups = T + (slots ? T * chunks : 0);
+  if (T >= 1 << 30 || Hkv >= 1 << 16) return PTL_ERR_ARG;
+  // a wave for every task there can be, up to eight a compute unit
+  const int store_groups = slots ? (int)min(((long)T * 2 * Hkv + 3) / 4, 2l * compute_units()) : 0;
+  const int groups = T + store_groups;
   const size_t lds = (size_t)D * sizeof(float);
   const bool vec = (D / 2) % 8 == 0 && row_stride % 8 == 0 && ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out) % 16 == 0;
   if (dtype == PTL_DTYPE_F32) {
     auto go = [&](auto kernel) {
       kernel<<<groups, 256, lds, stream>>>((float*)q_out, (const float*)q, (const float*)k, (const float*)v, row_stride, positions,
-                                           inv_freq, slots, k_cache, v_cache, k_scale, v_scale, T, Hq, Hkv, D, page_size, in_all, chunks);
+                                           inv_freq, slots, k_cache, v_cache, k_scale, v_scale, T, Hq, Hkv, D, page_size, in_all, store_groups);
     };
     if (vec) go(rope_store_f8_kernel<float, 8>); else go(rope_store_f8_kernel<float, 1>);
   } else if (dtype == PTL_DTYPE_BF16) {
     auto go = [&](auto kernel) {
       kernel<<<groups, 256, lds, stream>>>((bf16_t*)q_out, (const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, row_stride, positions,
-                                           inv_freq, slots, k_cache, v_cache, k_scale, v_scale, T, Hq, Hkv, D, page_size, in_all, chunks);
+                                           inv_freq, slots, k_cache, v_cache, k_scale, v_scale, T, Hq, Hkv, D, page_size, in_all, store_groups);
     };
     if (vec) go(rope_store_f8_kernel<bf16_t, 8>); else go(rope_store_f8_kernel<bf16_t, 1>);
   } else {

@@ -3,6 +3,10 @@ ops.kernels: operands are checked on the host, launches go to torch's current st
 
 The cache: codes float8_e4m3fn [pages, Hkv, page_size, D] and scales float32 [pages, Hkv], of the keys and of the values. What the
 block of a (page, kv head) holds stands for code * scale; a scale is a power of two (2^-126 and more).
+
+A decode step is a row of short kernels, and what the host needs for a call shows in it: tensors are asked for each of their
+properties once, and entries know their arguments' types, so that addresses go as plain numbers (a call of
+``attention_decode_f8`` 16.8 us before, X with it).
 """
 from __future__ import annotations
 
@@ -13,38 +17,57 @@ from typing import Optional, Sequence
 import torch
 
 from . import library
-from .kernels import TICKET, KernelError, _check, _dtype_code, _i32, _need_gpu, _ptr, _stream, _tickets
+from .kernels import TICKET, KernelError, _check, _dtype_code, _i32, _need_gpu, _tickets, compute_units
 
 CACHE_F8 = torch.float8_e4m3fn          # the codes' type
 
+_TYPES = {"p": ctypes.c_void_p, "l": ctypes.c_long, "i": ctypes.c_int, "f": ctypes.c_float}
+# entry -> library, types of its arguments (p: address, l: long, i: int, f: float)
+_ENTRIES = {"ptl_rope_store_f8": ("cache_f8", "pppplppppppp" "iiiiiii" "p"), "ptl_copy_pages": ("cache_f8", "pippip"),
+            "ptl_attention_generic_f8": ("attention_f8", "plplppppppp" "ipp" "iiiiii" "pfip"),
+            "ptl_attention_decode_f8": ("attention_f8", "plplppppppp" "ippp" "iiiiiii" "pfp"),
+            "ptl_attention_prefill_f8": ("attention_f8", "plplppppppp" "ipp" "iiiiiiii" "pfp")}
+_loaded = {}
+
+
+def _entry(name: str):
+    f = _loaded.get(name)
+    if f is None:
+        lib, types = _ENTRIES[name]
+        f = getattr(library.load(lib), name)
+        f.argtypes = [_TYPES[t] for t in types]
+        _loaded[name] = f
+    return f
+
+
+def _launch_stream(what: str, *tensors) -> int:
+    """torch's current stream; raises unless all tensors are on the current device, where the launch goes."""
+    at = -1
+    for t in tensors:
+        if t is not None:
+            d = t.get_device()
+            if d != at or d < 0:
+                _need_gpu(t)
+                at = torch._C._cuda_getDevice()
+                if d != at:
+                    raise KernelError(f"{what}: tensors must be on the current device cuda:{at}, got one on {t.device}")
+    return torch._C._cuda_getCurrentRawStream(at) if at >= 0 else 0
+
 
 def _cache(what: str, Hkv: int, D: int, k_cache, v_cache, k_scale, v_scale):
-    """(pages, page size) of an 8-bit cache; raises where its tensors do not belong together."""
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != Hkv or k_cache.shape[3] != D:
+    """(pages, page size, addresses) of an 8-bit cache; raises where its tensors do not belong together."""
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or shape[1] != Hkv or shape[3] != D:
         raise KernelError(f"{what}: caches must be [pages, {Hkv}, page_size, {D}]")
     if k_cache.dtype != CACHE_F8 or v_cache.dtype != CACHE_F8:
         raise KernelError(f"{what}: caches must be float8_e4m3fn, got {k_cache.dtype} and {v_cache.dtype}")
-    if not k_cache.is_contiguous() or not v_cache.is_contiguous() or (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+    k, v = k_cache.data_ptr(), v_cache.data_ptr()
+    if not k_cache.is_contiguous() or not v_cache.is_contiguous() or (k | v) % 16:
         raise KernelError(f"{what}: caches must be contiguous and 16-byte aligned")
-    scales = (k_cache.shape[0], Hkv)
     for t in (k_scale, v_scale):
-        if t.dtype != torch.float32 or t.shape != scales or not t.is_contiguous():
-            raise KernelError(f"{what}: scales must be contiguous float32 [{scales[0]}, {scales[1]}]")
-    return k_cache.shape[0], k_cache.shape[2]
-
-
-def _one_device(what: str, *tensors) -> None:
-    """All on the current device, where the launch goes."""
-    at = -1
-    for t in tensors:
-        if t is None:
-            continue
-        d = t.get_device()
-        if d != at or d < 0:
-            _need_gpu(t)
-            at = torch._C._cuda_getDevice()
-            if d != at:
-                raise KernelError(f"{what}: tensors must be on the current device cuda:{at}, got one on {t.device}")
+        if t.dtype != torch.float32 or t.shape != shape[:2] or not t.is_contiguous():
+            raise KernelError(f"{what}: scales must be contiguous float32 [{shape[0]}, {Hkv}]")
+    return shape[0], shape[2], (k, v, k_scale.data_ptr(), v_scale.data_ptr())
 
 
 def rope_store_f8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, inv_freq: Optional[torch.Tensor],
@@ -59,19 +82,20 @@ def rope_store_f8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     of them has the page's first slot the page begins anew: what it held is dropped, and rows behind the call's are zeros.
     Otherwise its scale grows where the new tokens need it, and the page's other numbers are rounded anew. Storing the same once
     more changes nothing. Numbers that are not finite are held as NaN."""
-    _one_device("rope_store_f8", q, k, v, positions, inv_freq, slots, k_cache, v_cache, k_scale, v_scale)
+    stream = _launch_stream("rope_store_f8", q, k, v, positions, inv_freq, slots, k_cache, v_cache, k_scale, v_scale)
     if q.dim() != 3 or k.dim() != 3:
         raise KernelError("rope_store_f8: q, k and v must be [T, heads, D]")
     T, Hq, D = q.shape
     Hkv = k.shape[1]
-    if k.shape != (T, Hkv, D) or v.shape != (T, Hkv, D):
+    if k.shape != (T, Hkv, D) or v.shape != k.shape:
         raise KernelError("rope_store_f8: k and v must be [T, Hkv, D]")
-    rs = q.stride(0)
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dtype != q.dtype or t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != D) or (T > 1 and t.stride(0) != rs):
+    dtype, rs = q.dtype, q.stride(0)
+    for name, t, heads in (("q", q, Hq), ("k", k, Hkv), ("v", v, Hkv)):
+        rows, head, one = t.stride()
+        if t.dtype != dtype or one != 1 or (heads > 1 and head != D) or (T > 1 and rows != rs):
             raise KernelError(f"rope_store_f8: {name} must be a [T, heads, D] view with dense heads and the common row stride")
-    if D % 2 or not 0 < D <= 640:
-        raise KernelError(f"rope_store_f8: head size {D} must be even, up to 640")
+    if D % 2 or not 0 < D <= 640 or Hq < 1 or Hkv < 1:
+        raise KernelError(f"rope_store_f8: head size {D} must be even, up to 640, and there is a head at least")
     _i32(positions, "positions")
     if positions.numel() != T:
         raise KernelError("rope_store_f8: one position per token")
@@ -81,47 +105,52 @@ def rope_store_f8(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
         _i32(slots, "slots")
         if slots.numel() != T:
             raise KernelError("rope_store_f8: one slot per token")
-    pages, page_size = _cache("rope_store_f8", Hkv, D, k_cache, v_cache, k_scale, v_scale)
-    out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
-    _check(library.load("cache_f8").ptl_rope_store_f8(
-        _ptr(out), _ptr(q), _ptr(k), _ptr(v), ctypes.c_long(rs), _ptr(positions), _ptr(inv_freq), _ptr(slots), _ptr(k_cache),
-        _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), T, Hq, Hkv, D, page_size, pages, _dtype_code(q), _stream()), "rope_store_f8")
+    pages, page_size, cache = _cache("rope_store_f8", Hkv, D, k_cache, v_cache, k_scale, v_scale)
+    out = torch.empty((T, Hq, D), dtype=dtype, device=q.device)
+    _check(_entry("ptl_rope_store_f8")(
+        out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), rs, positions.data_ptr(),
+        inv_freq.data_ptr() if inv_freq is not None else None, slots.data_ptr() if slots is not None else None, *cache, T, Hq, Hkv, D,
+        page_size, pages, _dtype_code(q), stream), "rope_store_f8")
     return out
 
 
-def _attention(what: str, out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, block_table, window, sink, *more):
-    _one_device(what, out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, block_table, sink, *more)
-    if q.dim() != 3 or out.shape != q.shape or out.dtype != q.dtype:
+def _attention(what: str, out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, block_table, window, sink):
+    """What the attentions have in common: (Hq, Hkv, D, page size, the entry's first arguments, address of the sink, alignment)."""
+    shape = q.shape
+    if len(shape) != 3 or out.shape != shape or out.dtype != q.dtype:
         raise KernelError(f"{what}: q and out must be [T, Hq, D] of one dtype")
-    T, Hq, D = q.shape
-    if k_cache.dim() != 4:
-        raise KernelError(f"{what}: caches must be [pages, Hkv, page_size, {D}]")
-    Hkv = k_cache.shape[1]
-    _, page_size = _cache(what, Hkv, D, k_cache, v_cache, k_scale, v_scale)
+    _, Hq, D = shape
+    Hkv = k_cache.shape[1] if k_cache.dim() == 4 else 0
+    _, page_size, cache = _cache(what, Hkv, D, k_cache, v_cache, k_scale, v_scale)
     if Hkv == 0 or Hq == 0 or Hq % Hkv:
         raise KernelError(f"{what}: {Hq} query heads are not a multiple of {Hkv} kv heads")
-    if q.stride(2) != 1 or out.stride(2) != 1 or (Hq > 1 and (q.stride(1) != D or out.stride(1) != D)):
+    (q_row, q_head, q_one), (out_row, out_head, out_one) = q.stride(), out.stride()
+    if q_one != 1 or out_one != 1 or (Hq > 1 and (q_head != D or out_head != D)):
         raise KernelError(f"{what}: q and out need dense heads")
     _i32(q_start, "q_start")
     _i32(ctx_len, "ctx_len")
-    if q_start.numel() != ctx_len.numel() + 1:
+    n = ctx_len.numel()
+    if q_start.numel() != n + 1:
         raise KernelError(f"{what}: inconsistent sequence tables")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < ctx_len.numel() \
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < n \
+            or (block_table.stride(1) != 1 and block_table.shape[1] > 1):
         raise KernelError(f"{what}: block_table must be int32 [n, max_pages]")
     if window < 0:
         raise KernelError(f"{what}: a window is not negative")
     if sink is not None and (sink.dtype != torch.float32 or sink.shape != (Hq,) or not sink.is_contiguous()):
         raise KernelError(f"{what}: sink must be a contiguous float32 tensor [{Hq}]")
-    return T, Hq, Hkv, D, page_size
+    q_at, out_at = q.data_ptr(), out.data_ptr()
+    args = (out_at, out_row, q_at, q_row, *cache, q_start.data_ptr(), ctx_len.data_ptr(), block_table.data_ptr(), block_table.stride(0))
+    return Hq, Hkv, D, page_size, args, sink.data_ptr() if sink is not None else None, (q_at % 16 or q_row % 8, out_at % 8 or out_row % 4)
 
 
 def _work(what: str, work_seq: torch.Tensor, work_qoff: torch.Tensor) -> int:
     _i32(work_seq, "work_seq")
     _i32(work_qoff, "work_qoff")
-    if work_seq.numel() != work_qoff.numel():
+    n = work_seq.numel()
+    if n != work_qoff.numel():
         raise KernelError(f"{what}: inconsistent work list")
-    return work_seq.numel()
+    return n
 
 
 def attention_generic_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -130,15 +159,15 @@ def attention_generic_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
                          sink: Optional[torch.Tensor] = None) -> None:
     """``attention_generic`` over an 8-bit cache: float32 or bfloat16 queries, head sizes up to 640, any page size; the work list names
     16-row query blocks. window, sink: as there."""
-    T, Hq, Hkv, D, page_size = _attention("attention_generic_f8", out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len,
-                                          block_table, window, sink, work_seq, work_qoff)
+    what = "attention_generic_f8"
+    stream = _launch_stream(what, out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, block_table, sink, work_seq, work_qoff)
+    Hq, Hkv, D, page_size, args, sink_at, _ = _attention(what, out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len,
+                                                         block_table, window, sink)
     if not 0 < D <= 640 or Hq > 65535:
-        raise KernelError(f"attention_generic_f8: head size {D} exceeds the kernel's limit of 640 (or {Hq} heads that of 65,535)")
-    n = _work("attention_generic_f8", work_seq, work_qoff)
-    _check(library.load("attention_f8").ptl_attention_generic_f8(
-        _ptr(out), ctypes.c_long(out.stride(0)), _ptr(q), ctypes.c_long(q.stride(0)), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
-        _ptr(v_scale), _ptr(q_start), _ptr(ctx_len), _ptr(block_table), int(block_table.stride(0)), _ptr(work_seq), _ptr(work_qoff),
-        n, Hq, Hkv, D, page_size, int(window), _ptr(sink), ctypes.c_float(scale), _dtype_code(q), _stream()), "attention_generic_f8")
+        raise KernelError(f"{what}: head size {D} exceeds the kernel's limit of 640 (or {Hq} heads that of 65,535)")
+    n = _work(what, work_seq, work_qoff)
+    _check(_entry("ptl_attention_generic_f8")(*args, work_seq.data_ptr(), work_qoff.data_ptr(), n, Hq, Hkv, D, page_size, int(window),
+                                              sink_at, scale, _dtype_code(q), stream), what)
 
 
 def attention_f8_fits(dtype: torch.dtype, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> bool:
@@ -149,6 +178,9 @@ def attention_f8_fits(dtype: torch.dtype, num_heads: int, num_kv_heads: int, hea
             and 0 < num_heads // num_kv_heads <= 1024 and num_kv_heads * page_size * head_dim < 2 ** 31)
 
 
+MOST_PARTS_F8 = 128        # parts of a (sequence, kv head) pair (csrc/attention_f8.hip)
+
+
 def attention_decode_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                         v_scale: torch.Tensor, q_start: torch.Tensor, ctx_len: torch.Tensor, block_table: torch.Tensor, n_seq: int,
                         scale: float, window: int = 0, sink: Optional[torch.Tensor] = None,
@@ -156,26 +188,25 @@ def attention_decode_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tenso
     """Attention of the first ``n_seq`` sequences of the tables, each of which brings exactly one query token, over an 8-bit cache
     (``attention_f8_fits`` says for which sizes). How the keys are cut is decided on the device from ctx_len. ``tickets``: as for
     ``attention_decode``, TICKET * n_seq * kv heads for every 16 heads of a kv head."""
-    T, Hq, Hkv, D, page_size = _attention("attention_decode_f8", out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len,
-                                          block_table, window, sink, tickets)
-    if not attention_f8_fits(q.dtype, Hq, Hkv, D, page_size) or q.stride(0) % 8 or q.data_ptr() % 16:
-        raise KernelError("attention_decode_f8: needs bfloat16, a head size of 32/64/96/128, a page size from 16 on that is a power "
-                          "of two, aligned q rows")
+    what = "attention_decode_f8"
+    stream = _launch_stream(what, out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, block_table, sink, tickets)
+    Hq, Hkv, D, page_size, args, sink_at, unaligned = _attention(what, out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len,
+                                                                 block_table, window, sink)
+    if unaligned[0] or not attention_f8_fits(q.dtype, Hq, Hkv, D, page_size):
+        raise KernelError(f"{what}: needs bfloat16, a head size of 32/64/96/128, a page size from 16 on that is a power of two, "
+                          "aligned q rows")
     if not 0 <= n_seq <= ctx_len.numel():
-        raise KernelError("attention_decode_f8: tables are shorter than n_seq")
+        raise KernelError(f"{what}: tables are shorter than n_seq")
     if n_seq == 0:
         return
-    lib = library.load("attention_f8")
-    cuts = lib.ptl_attention_decode_f8_cuts(n_seq, Hkv, Hq)
-    heads = (n_seq + cuts) * Hq
+    tiles = -(-(Hq // Hkv) // 16)
+    cap = max(1, min(MOST_PARTS_F8, compute_units(q.device) // (Hkv * tiles)))         # a workgroup a compute unit
+    heads = (n_seq + cap) * Hq                                                       # (room for parts: csrc/attention_f8.hip)
     parts = torch.empty(heads * (D + 2), dtype=torch.float32, device=q.device)
-    tickets = _tickets(tickets, TICKET * n_seq * Hkv * -(-(Hq // Hkv) // 16), q, "attention_decode_f8")
+    tickets = _tickets(tickets, TICKET * n_seq * Hkv * tiles, q, what)
     at = parts.data_ptr()
-    _check(lib.ptl_attention_decode_f8(
-        _ptr(out), ctypes.c_long(out.stride(0)), _ptr(q), ctypes.c_long(q.stride(0)), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
-        _ptr(v_scale), _ptr(q_start), _ptr(ctx_len), _ptr(block_table), int(block_table.stride(0)), ctypes.c_void_p(at),
-        ctypes.c_void_p(at + 4 * heads * D), _ptr(tickets), cuts, int(n_seq), Hq, Hkv, D, page_size, int(window), _ptr(sink),
-        ctypes.c_float(scale), _stream()), "attention_decode_f8")
+    _check(_entry("ptl_attention_decode_f8")(*args, at, at + 4 * heads * D, tickets.data_ptr(), cap, int(n_seq), Hq, Hkv, D, page_size,
+                                             int(window), sink_at, scale, stream), what)
 
 
 def attention_prefill_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -185,23 +216,22 @@ def attention_prefill_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
     """``attention_prefill_mfma`` over an 8-bit cache (``attention_f8_fits`` says for which sizes): the work list names query blocks
     of ``block_rows`` (64 or 128) rows, those with the most keys first; ``groups`` workgroups a head share it (0: one for
     every block)."""
-    T, Hq, Hkv, D, page_size = _attention("attention_prefill_f8", out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len,
-                                          block_table, window, sink, work_seq, work_qoff)
+    what = "attention_prefill_f8"
+    stream = _launch_stream(what, out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, block_table, sink, work_seq, work_qoff)
+    Hq, Hkv, D, page_size, args, sink_at, unaligned = _attention(what, out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len,
+                                                                 block_table, window, sink)
     if not attention_f8_fits(q.dtype, Hq, Hkv, D, page_size):
-        raise KernelError("attention_prefill_f8: needs bfloat16, a head size of 32/64/96/128, a page size from 16 on that is a power "
-                          "of two")
-    if q.stride(0) % 8 or out.stride(0) % 4 or q.data_ptr() % 16 or out.data_ptr() % 8:
-        raise KernelError("attention_prefill_f8: q rows must be 16-byte aligned, out rows 8-byte")
+        raise KernelError(f"{what}: needs bfloat16, a head size of 32/64/96/128, a page size from 16 on that is a power of two")
+    if unaligned[0] or unaligned[1]:
+        raise KernelError(f"{what}: q rows must be 16-byte aligned, out rows 8-byte")
     if block_rows not in (64, 128):
-        raise KernelError("attention_prefill_f8: query blocks are 64 or 128 rows")
+        raise KernelError(f"{what}: query blocks are 64 or 128 rows")
     if not scale > 0:
-        raise KernelError("attention_prefill_f8: scale must be positive")
-    n = _work("attention_prefill_f8", work_seq, work_qoff)
-    _check(library.load("attention_f8").ptl_attention_prefill_f8(
-        _ptr(out), ctypes.c_long(out.stride(0)), _ptr(q), ctypes.c_long(q.stride(0)), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
-        _ptr(v_scale), _ptr(q_start), _ptr(ctx_len), _ptr(block_table), int(block_table.stride(0)), _ptr(work_seq), _ptr(work_qoff),
-        n, min(n, int(groups), 65535) if groups > 0 else min(n, 65535), int(block_rows), Hq, Hkv, D, page_size, int(window),
-        _ptr(sink), ctypes.c_float(scale), _stream()), "attention_prefill_f8")
+        raise KernelError(f"{what}: scale must be positive")
+    n = _work(what, work_seq, work_qoff)
+    _check(_entry("ptl_attention_prefill_f8")(*args, work_seq.data_ptr(), work_qoff.data_ptr(), n,
+                                              min(n, int(groups) if groups > 0 else n, 65535), block_rows, Hq, Hkv, D, page_size,
+                                              int(window), sink_at, scale, stream), what)
 
 
 def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:
@@ -212,24 +242,24 @@ def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
     n = len(src)
     if n != len(dst):
         raise KernelError(f"copy_pages: {n} pages to read, {len(dst)} to write")
-    _one_device("copy_pages", *pools)
+    stream = _launch_stream("copy_pages", *pools)
+    if len(pools) > 16:
+        raise KernelError("copy_pages: up to 16 pools a call")
+    low, high = (min(min(src), min(dst)), max(max(src), max(dst))) if n else (0, -1)
     desc = []
     for t in pools:
-        if t.dim() < 2 or not t.is_contiguous():
+        shape = t.shape
+        if len(shape) < 2 or not t.is_contiguous():
             raise KernelError("copy_pages: a pool is a contiguous tensor [layers, pages, ...]")
-        layers, pages = t.shape[:2]
-        if n and not (0 <= min(src) and max(src) < pages and 0 <= min(dst) and max(dst) < pages):
-            raise KernelError(f"copy_pages: a page number lies outside the pool's {pages} pages")
+        if low < 0 or high >= shape[1]:
+            raise KernelError(f"copy_pages: a page number lies outside the pool's {shape[1]} pages")
         if t.numel():
-            desc += [t.data_ptr(), layers, pages, t.numel() // (layers * pages) * t.element_size()]
+            desc += (t.data_ptr(), shape[0], shape[1], t.stride(1) * t.element_size())
     written = set(dst)
     if len(written) != n or not written.isdisjoint(src):
         raise KernelError("copy_pages: a page is written twice, or read and written")
     if n == 0 or not desc:
         return
-    if len(desc) > 4 * 16:
-        raise KernelError("copy_pages: up to 16 pools a call")
-    numbers = (ctypes.c_int32 * (2 * n))(*itertools.chain(src, dst))
+    numbers, described = (ctypes.c_int32 * (2 * n))(*itertools.chain(src, dst)), (ctypes.c_long * len(desc))(*desc)
     at = ctypes.addressof(numbers)
-    _check(library.load("cache_f8").ptl_copy_pages((ctypes.c_long * len(desc))(*desc), len(desc) // 4, ctypes.c_void_p(at),
-                                                   ctypes.c_void_p(at + 4 * n), n, _stream()), "copy_pages")
+    _check(_entry("ptl_copy_pages")(ctypes.addressof(described), len(desc) // 4, at, at + 4 * n, n, stream), "copy_pages")
