@@ -162,6 +162,13 @@ extern "C" int ptl_attention_generic_f8(void* out, long out_stride, const void* 
 // two matrix instructions (which k-value stands where is free, as long as the queries' agree); the last 32 elements come as
 // 8 bytes, 64 A + 8 lg .. +7.
 
+__device__ __forceinline__ float max2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+// two floats for another workgroup, 8-byte aligned (get_shared2 reads them)
+__device__ __forceinline__ void put_shared2(float2* p, float a, float b) {
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), __builtin_bit_cast(unsigned long long, make_float2(a, b)),
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // two codes (the low or the high half of x) times a power of two, as bfloat16: exact
 __device__ __forceinline__ uint32_t two_bf16(uint32_t x, float scale, bool high) {
   const auto r = high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x, scale, true)
@@ -584,11 +591,26 @@ extern "C" int ptl_attention_decode_f8(void* out, long out_stride, const void* q
 // converted into the other buffer and tile t + 2 sets out. Products, softmax and the layout of LDS are those of
 // attention_prefill.h: S^T = K Q^T, O^T += V^T P^T, sums of the rounded probabilities by one more product with ones.
 // Of a tile every wave brings 16 rows, which lie in one page: page and scales are the wave's, in scalar registers.
-template <int ND, int RT>
+//
+// CUT (blocks of 64 rows): few of them. Their tiles are dealt out evenly: a block is cut into parts of about (all tiles) / cap
+// tiles, a workgroup a part, as the decode kernel cuts its sequences, and the workgroup of a block that is done last merges its
+// parts: sums lie in the workspace as the lanes hold them. Otherwise workgroups take whole blocks in turn. us, not cut and cut, 32 heads:
+// 200 rows behind 3,000 keys of 128 66.5 36.1, 512 behind 8,000 of 128 189.5 127.4, 512 behind 1,024 of 64 23.2 23.1; with more blocks
+// 700 rows of 128 19.6 21.1, 1,500 behind 500 of 64 34.2 38.0, 1,531 behind 6,145 of 128 315 330.
+//
+// What bounds it: 1,531 rows behind 6,145 keys, 32 heads of 128: X
+struct PrefillF8Parts {
+  float2 *acc, *ml;                // [part][head][RT][2 ND][2][thread], [part][head][RT][thread]
+  int* tickets;                    // [block][head][TICKET]
+  int cap;
+};
+constexpr int WHOLE_TILES = 6;     // tiles up to which a block is not cut
+
+template <int ND, int RT, bool CUT>
 __global__ void __launch_bounds__(256, ND <= 2 ? 3 : 2)
 attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* __restrict__ q, long q_stride, F8Cache cache, F8Tables tab,
                        const int32_t* __restrict__ work_seq, const int32_t* __restrict__ work_qoff, int n_work, int Hq, int Hkv,
-                       int page_shift, int window, const float* __restrict__ sink, float scale_log2) {
+                       int page_shift, int window, const float* __restrict__ sink, float scale_log2, PrefillF8Parts parts) {
   constexpr int D = 32 * ND, BN = 64, ROWS = 64 * RT;
   constexpr int PIECES = D / 8;                     // 8-element pieces of a row: 8 codes, 16 bytes of bfloat16
   __shared__ __attribute__((aligned(16))) bf16_t Ks[2][BN * D], Vs[2][BN * D];
@@ -607,26 +629,61 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
   for (int j = 0; j < 8; ++j) ones.v[j] = (__bf16)1.0f;
   const float lazy = 8.0f / scale_log2;             // (raw scores: the maximum follows only where they pass it by 2^8)
   // Wave w brings rows 16 w .. +15 of a tile: 16 D bytes side by side in one page, lane l the 8 codes from 512 i + 8 l on of them
-  int plds[ND];
+  // (addresses that differ from another one by a constant are that one and the constant: registers are short at D = 128)
+  constexpr int STORES = D == 128 ? 2 : D == 64 ? 1 : ND;     // of D = 128 and 64: every 8 rows the same piece lies in the same place
+  int plds[STORES];
 #pragma unroll
-  for (int i = 0; i < ND; ++i) {
+  for (int i = 0; i < STORES; ++i) {
     const int r = (64 * i + lane) / PIECES, c = 64 * i + lane - r * PIECES;
     plds[i] = (16 * wave + r) * D + (c ^ swz(r)) * 8;
   }
+  auto store_at = [&](int i) { return plds[i % STORES] + i / STORES * 8 * D; };
   // where this lane reads: the first product takes row 16 kt + ln, piece 4 kk + lg; the second points at row
   // 32 half + 16 j + 4 lg + ln / 4, elements 16 dt + 4 (ln % 4) .. +3
-  int k_at[ND], v_at[2 * ND];
+  constexpr int SWAPPED = PIECES % 8 == 0 ? 8 : 4;            // pieces change places within so many
+  int k_at[SWAPPED / 4], v_at[SWAPPED / 2];
 #pragma unroll
-  for (int kk = 0; kk < ND; ++kk) k_at[kk] = ln * D + 8 * ((4 * kk + lg) ^ swz(ln));
+  for (int kk = 0; kk < SWAPPED / 4; ++kk) k_at[kk] = ln * D + 8 * ((4 * kk + lg) ^ swz(ln));
   {
     const int r = 4 * lg + (ln >> 2);
 #pragma unroll
-    for (int dt = 0; dt < 2 * ND; ++dt) v_at[dt] = r * D + 8 * ((2 * dt + ((ln & 3) >> 1)) ^ swz(r)) + 4 * (ln & 1);
+    for (int dt = 0; dt < SWAPPED / 2; ++dt) v_at[dt] = r * D + 8 * ((2 * dt + ((ln & 3) >> 1)) ^ swz(r)) + 4 * (ln & 1);
   }
+  auto key_at = [&](int kk) { return k_at[kk % (SWAPPED / 4)] + kk / (SWAPPED / 4) * 8 * SWAPPED; };
+  auto value_at = [&](int dt) { return v_at[dt % (SWAPPED / 2)] + dt / (SWAPPED / 2) * 8 * SWAPPED; };
+  const int seen_back = window > 0 ? window : 1 << 30;
 
-  // the list is sorted, most keys first; the workgroups of a head walk it forwards and backwards in turn
+  int my_item = -1, part = 0, n_parts = 1;
+  if constexpr (CUT) {
+    // lane i has block i
+    int tiles = -1;                                 // (of a block without rows)
+    if (lane < n_work) {
+      const int seq = work_seq[lane], qoff = work_qoff[lane];
+      const int qlen = tab.q_start[seq + 1] - tab.q_start[seq], ctx = tab.ctx_len[seq], rows = min(ROWS, qlen - qoff);
+      const int first_q = ctx - qlen + qoff, k_lo = window > 0 ? max(0, first_q - window + 1) : 0;
+      if (rows > 0) tiles = max(0, (min(ctx, first_q + rows) - k_lo / BN * BN + BN - 1) / BN);
+    }
+    int total = max(tiles, 0);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+    const int whole = max(parts.cap - n_work / 2, (3 * parts.cap + 3) / 4), piece = max(1, (total + whole - 1) / whole);
+    const int mine = tiles < 0 ? 0 : tiles <= WHOLE_TILES ? 1 : (tiles + piece - 1) / piece;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(upto, o, 64);
+      upto += lane >= o ? x : 0;
+    }
+    const unsigned long long here = __ballot(upto > (int)blockIdx.y);
+    if (!here) return;                              // (more room than parts)
+    my_item = __ffsll(here) - 1;
+    n_parts = __builtin_amdgcn_readlane(mine, my_item);
+    part = blockIdx.y - (__builtin_amdgcn_readlane(upto, my_item) - n_parts);
+  }
+  // not cut: the list is sorted, most keys first; the workgroups of a head walk it forwards and backwards in turn
   for (int round = 0;; ++round) {
-    const int item = round * gridDim.y + ((round & 1) ? gridDim.y - 1 - blockIdx.y : blockIdx.y);
+    const int item = CUT ? (round ? n_work : my_item)
+                         : round * gridDim.y + ((round & 1) ? gridDim.y - 1 - blockIdx.y : blockIdx.y);
     if (item >= n_work) break;
     const int seq = work_seq[item], qoff = work_qoff[item];
     const int first = tab.q_start[seq], qlen = tab.q_start[seq + 1] - first, ctx = tab.ctx_len[seq];
@@ -634,16 +691,13 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
     if (rows <= 0) continue;
     const int32_t* bt = tab.block_table + (size_t)seq * tab.bt_stride;
     const int first_q = ctx - qlen + qoff;          // position of the block's first row
-    int qpos[RT], lo[RT];
-    bool row_ok[RT];
+    int qpos[RT];
     Frag8 qf[RT][ND];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int mine = 16 * (RT * wave + r) + ln;
-      row_ok[r] = mine < rows;
-      const int qrow = row_ok[r] ? mine : 0;        // (rows behind the end repeat the first; they are not stored)
+      const int qrow = mine < rows ? mine : 0;      // (rows behind the end repeat the first; they are not stored)
       qpos[r] = first_q + qrow;
-      lo[r] = window > 0 ? max(0, qpos[r] - window + 1) : 0;
       const bf16_t* x = q + (size_t)(first + qoff + qrow) * q_stride + (size_t)head * D + 8 * lg;
 #pragma unroll
       for (int kk = 0; kk < ND; ++kk) qf[r][kk].u = load16(x + 32 * kk);
@@ -661,7 +715,8 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
       for (int t = 0; t <= 2 * ND; ++t) o[r][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
     const int k_lo = window > 0 ? max(0, first_q - window + 1) : 0, k_end = min(ctx, first_q + rows);
-    const int k_begin = k_lo / BN * BN, n_tiles = (k_end - k_begin + BN - 1) / BN;
+    const int k_begin = k_lo / BN * BN, n_all = max(0, (k_end - k_begin + BN - 1) / BN);
+    const int per = (n_all + n_parts - 1) / n_parts, t_first = part * per, n_tiles = min(n_all, t_first + per);      // this part's tiles
 
     uint2 kc[ND], vc[ND];
     float ks, vs;
@@ -693,8 +748,8 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
       }
 #pragma unroll
       for (int i = 0; i < ND; ++i) {
-        *reinterpret_cast<bf16x8_t*>(Kb + plds[i]) = eight_bf16(kc[i].x, kc[i].y, ks);
-        *reinterpret_cast<bf16x8_t*>(Vb + plds[i]) = eight_bf16(vc[i].x, vc[i].y, vs);
+        *reinterpret_cast<bf16x8_t*>(Kb + store_at(i)) = eight_bf16(kc[i].x, kc[i].y, ks);
+        *reinterpret_cast<bf16x8_t*>(Vb + store_at(i)) = eight_bf16(vc[i].x, vc[i].y, vs);
       }
     };
     auto tile = [&](int k0, const bf16_t* Kb, const bf16_t* Vb, auto masked_tag) __attribute__((always_inline)) {
@@ -707,12 +762,11 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
 #pragma unroll
         for (int kk = 0; kk < ND; ++kk) {
           Frag8 a;
-          a.u = *reinterpret_cast<const uint4*>(Kb + 16 * kt * D + k_at[kk]);
+          a.u = *reinterpret_cast<const uint4*>(Kb + 16 * kt * D + key_at(kk));
 #pragma unroll
           for (int r = 0; r < RT; ++r) st[r][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, qf[r][kk].v, st[r][kt], 0, 0, 0);
         }
       }
-      __builtin_amdgcn_sched_barrier(0);
       Frag8 p[RT][2];
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
@@ -722,7 +776,7 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int k = k0 + 16 * kt + 4 * lg + i;
-              st[r][kt][i] = k <= qpos[r] && k < k_end && k >= lo[r] ? st[r][kt][i] : -INFINITY;
+              st[r][kt][i] = k <= qpos[r] && k < k_end && k > qpos[r] - seen_back ? st[r][kt][i] : -INFINITY;
             }
         }
         float top = -INFINITY;
@@ -746,7 +800,8 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
             for (int i = 0; i < 4; ++i)
               p[r][half].v[4 * t + i] = (__bf16)__builtin_amdgcn_exp2f(fmaf(st[r][2 * half + t][i], scale_log2, mc));
       }
-      __builtin_amdgcn_sched_barrier(0);
+      // (two row tiles leave no registers for values that are read early)
+      if constexpr (RT == 2) __builtin_amdgcn_sched_barrier(0);
       auto transposed = [&](const bf16_t* x) {
         return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)x);
       };
@@ -755,8 +810,8 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
 #pragma unroll
         for (int dt = 0; dt < 2 * ND; ++dt) {
           Frag8 a;
-          a.s[0] = transposed(Vb + 32 * half * D + v_at[dt]);
-          a.s[1] = transposed(Vb + (32 * half + 16) * D + v_at[dt]);
+          a.s[0] = transposed(Vb + 32 * half * D + value_at(dt));
+          a.s[1] = transposed(Vb + (32 * half + 16) * D + value_at(dt));
 #pragma unroll
           for (int r = 0; r < RT; ++r) o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, p[r][half].v, o[r][dt], 0, 0, 0);
         }
@@ -770,7 +825,6 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
         convert(t + 1, Ks[1 - buffer], Vs[1 - buffer]);
         if (t + 2 < n_tiles) { load(t + 2); load_page(t + 3); }
       }
-      __builtin_amdgcn_sched_barrier(0);
       if (wave_has_rows && k0 <= max_q && k0 + BN > wave_lo) {
         const bool need_mask = k0 + BN - 1 > min_q || k0 + BN > k_end || k0 < wave_lo_last;
         if (need_mask) tile(k0, Ks[buffer], Vs[buffer], std::true_type{});
@@ -778,23 +832,73 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
       }
       __syncthreads();
     };
-    if (n_tiles > 0) {
-      load_page(0);
-      load(0);
-      load_page(1);
-      convert(0, Ks[0], Vs[0]);
-      if (n_tiles > 1) { load(1); load_page(2); }
+    if (t_first < n_tiles) {
+      load_page(t_first);
+      load(t_first);
+      load_page(t_first + 1);
+      convert(t_first, Ks[0], Vs[0]);
+      if (t_first + 1 < n_tiles) { load(t_first + 1); load_page(t_first + 2); }
     }
     __syncthreads();
-    for (int t = 0; t < n_tiles; t += 2) {
+    for (int t = t_first; t < n_tiles; t += 2) {
       turn(t, 0);
       if (t + 1 < n_tiles) turn(t + 1, 1);
     }
+    float l_sum[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) l_sum[r] = o[r][2 * ND][0];
+    if constexpr (CUT) {
+      if (n_parts > 1) {
+        __shared__ int last;
+        constexpr int WORDS = RT * 2 * ND * 2 * 256, ENDS = RT * 256;
+        const size_t first_part = (size_t)(blockIdx.y - part) * Hq + head, mine = (size_t)blockIdx.y * Hq + head;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+#pragma unroll
+          for (int dt = 0; dt < 2 * ND; ++dt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              put_shared2(parts.acc + mine * WORDS + ((r * 2 * ND + dt) * 2 + x) * 256 + threadIdx.x, o[r][dt][2 * x], o[r][dt][2 * x + 1]);
+          put_shared2(parts.ml + mine * ENDS + r * 256 + threadIdx.x, m_run[r], l_sum[r]);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // this wave's share of the part has reached memory
+        __syncthreads();
+        if (threadIdx.x == 0) last = last_part(parts.tickets + ((size_t)item * Hq + head) * TICKET, n_parts);
+        __syncthreads();
+        if (!last) return;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          float top = -INFINITY;
+          for (int p = 0; p < n_parts; ++p)
+            top = max2(top, get_shared2((const float*)(parts.ml + (first_part + (size_t)p * Hq) * ENDS + r * 256 + threadIdx.x)).x);
+          float l = 0.f;
+#pragma unroll
+          for (int dt = 0; dt < 2 * ND; ++dt) o[r][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+          for (int p = 0; p < n_parts; ++p) {                     // (in the order of the keys)
+            const size_t at = first_part + (size_t)p * Hq;
+            const float2 e = get_shared2((const float*)(parts.ml + at * ENDS + r * 256 + threadIdx.x));
+            // (a part that has seen no key has zero sums; its maximum, and where no part has seen one the largest too, is -inf)
+            const float f = e.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((e.x - top) * scale_log2);
+            l = fmaf(e.y, f, l);
+#pragma unroll
+            for (int dt = 0; dt < 2 * ND; ++dt)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const float2 a = get_shared2((const float*)(parts.acc + at * WORDS + ((r * 2 * ND + dt) * 2 + x) * 256 + threadIdx.x));
+                o[r][dt][2 * x] = fmaf(a.x, f, o[r][dt][2 * x]);
+                o[r][dt][2 * x + 1] = fmaf(a.y, f, o[r][dt][2 * x + 1]);
+              }
+          }
+          m_run[r] = top;
+          l_sum[r] = l;
+        }
+      }
+    }
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      float l = o[r][2 * ND][0];
+      float l = l_sum[r];
       if (sink) l += __builtin_amdgcn_exp2f(sink[head] * 1.4426950408889634f - m_run[r] * scale_log2);
-      if (!row_ok[r]) continue;
+      if (16 * (RT * wave + r) + ln >= rows) continue;
       const float inv = l == 0.f ? 0.f : 1.0f / l;
       bf16_t* to = out + (size_t)(first + qoff + 16 * (RT * wave + r) + ln) * out_stride + (size_t)head * D + 4 * lg;
 #pragma unroll
@@ -808,33 +912,39 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
   }
 }
 
+// cap > 0: blocks are cut into some ``cap`` parts a head in all (n_work up to 64; work: (n_work + cap) * Hq * block_rows *
+// (D + 8) floats, tickets: n_work * Hq * TICKET zeros, zeros again afterwards). Else ``groups`` workgroups a head take whole blocks.
 extern "C" int ptl_attention_prefill_f8(void* out, long out_stride, const void* q, long q_stride, const uint8_t* k, const uint8_t* v,
                                         const float* k_scale, const float* v_scale, const int32_t* q_start, const int32_t* ctx_len,
                                         const int32_t* block_table, int bt_stride, const int32_t* work_seq, const int32_t* work_qoff,
-                                        int n_work, int groups, int block_rows, int Hq, int Hkv, int D, int page_size, int window,
-                                        const float* sink, float scale, hipStream_t stream) {
+                                        int n_work, int groups, int cap, float* work, int* tickets, int block_rows, int Hq, int Hkv,
+                                        int D, int page_size, int window, const float* sink, float scale, hipStream_t stream) {
   if (n_work <= 0) return PTL_OK;
   if (!f8_matrix_sizes(Hq, Hkv, D, page_size) || window < 0 || groups <= 0 || groups > 65535 || (block_rows != 64 && block_rows != 128) ||
       !(scale > 0.f) || ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 || q_stride % 8 || (uintptr_t)out % 8 || out_stride % 4)
     return PTL_ERR_ARG;
+  if (cap < 0 || (cap && (block_rows != 64 || n_work > 64 || cap > 4096 || !work || (uintptr_t)work % 8 || !tickets))) return PTL_ERR_ARG;
   const F8Cache cache{k, v, k_scale, v_scale};
   const F8Tables tab{q_start, ctx_len, block_table, bt_stride};
+  const PrefillF8Parts parts{(float2*)work, (float2*)(work + (size_t)(n_work + cap) * Hq * block_rows * D), tickets, cap};
   int shift = 0;
   while (1 << shift < page_size) ++shift;
-  auto go = [&](auto kernel) {
-    kernel<<<dim3(Hq, groups), 256, 0, stream>>>((bf16_t*)out, out_stride, (const bf16_t*)q, q_stride, cache, tab, work_seq, work_qoff,
-                                                 n_work, Hq, Hkv, shift, window, sink, scale * 1.4426950408889634f);
+  auto go = [&](auto kernel, int y) {
+    kernel<<<dim3(Hq, y), 256, 0, stream>>>((bf16_t*)out, out_stride, (const bf16_t*)q, q_stride, cache, tab, work_seq, work_qoff, n_work,
+                                            Hq, Hkv, shift, window, sink, scale * 1.4426950408889634f, parts);
   };
-  if (block_rows == 64) {
-    if (D == 32) go(attn_prefill_f8_kernel<1, 1>);
-    else if (D == 64) go(attn_prefill_f8_kernel<2, 1>);
-    else if (D == 96) go(attn_prefill_f8_kernel<3, 1>);
-    else go(attn_prefill_f8_kernel<4, 1>);
-  } else {
-    if (D == 32) go(attn_prefill_f8_kernel<1, 2>);
-    else if (D == 64) go(attn_prefill_f8_kernel<2, 2>);
-    else if (D == 96) go(attn_prefill_f8_kernel<3, 2>);
-    else go(attn_prefill_f8_kernel<4, 2>);
-  }
+  auto size = [&](auto nd) {
+    constexpr int ND = decltype(nd)::value;
+    if (block_rows == 64) {
+      if (cap) go(attn_prefill_f8_kernel<ND, 1, true>, n_work + cap);
+      else go(attn_prefill_f8_kernel<ND, 1, false>, groups);
+    } else {
+      go(attn_prefill_f8_kernel<ND, 2, false>, groups);
+    }
+  };
+  if (D == 32) size(std::integral_constant<int, 1>{});
+  else if (D == 64) size(std::integral_constant<int, 2>{});
+  else if (D == 96) size(std::integral_constant<int, 3>{});
+  else size(std::integral_constant<int, 4>{});
   return ptl_launch_status();
 }

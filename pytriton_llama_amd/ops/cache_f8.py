@@ -26,7 +26,7 @@ _TYPES = {"p": ctypes.c_void_p, "l": ctypes.c_long, "i": ctypes.c_int, "f": ctyp
 _ENTRIES = {"ptl_rope_store_f8": ("cache_f8", "pppplppppppp" "iiiiiii" "p"), "ptl_copy_pages": ("cache_f8", "pippip"),
             "ptl_attention_generic_f8": ("attention_f8", "plplppppppp" "ipp" "iiiiii" "pfip"),
             "ptl_attention_decode_f8": ("attention_f8", "plplppppppp" "ippp" "iiiiiii" "pfp"),
-            "ptl_attention_prefill_f8": ("attention_f8", "plplppppppp" "ipp" "iiiiiiii" "pfp")}
+            "ptl_attention_prefill_f8": ("attention_f8", "plplppppppp" "ipp" "iiippiiiiii" "pfp")}
 _loaded = {}
 
 
@@ -209,15 +209,21 @@ def attention_decode_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tenso
                                              int(window), sink_at, scale, stream), what)
 
 
+WHOLE_TILES = 6            # tiles of 64 keys up to which a block of query rows is not cut (csrc/attention_f8.hip)
+
+
 def attention_prefill_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                          v_scale: torch.Tensor, q_start: torch.Tensor, ctx_len: torch.Tensor, block_table: torch.Tensor,
                          work_seq: torch.Tensor, work_qoff: torch.Tensor, scale: float, window: int = 0, block_rows: int = 64,
-                         groups: int = 0, sink: Optional[torch.Tensor] = None) -> None:
+                         groups: int = 0, sink: Optional[torch.Tensor] = None, tickets: Optional[torch.Tensor] = None) -> None:
     """``attention_prefill_mfma`` over an 8-bit cache (``attention_f8_fits`` says for which sizes): the work list names query blocks
     of ``block_rows`` (64 or 128) rows, those with the most keys first; ``groups`` workgroups a head share it (0: one for
-    every block)."""
+    every block). Where blocks of 64 rows have a workgroup each and fill less than half of the GPU, their keys are dealt out to as
+    many as fill it;
+    ``tickets``: zeros that such launches on one stream may share, TICKET * blocks * query heads (else they are made)."""
     what = "attention_prefill_f8"
-    stream = _launch_stream(what, out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, block_table, sink, work_seq, work_qoff)
+    stream = _launch_stream(what, out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, block_table, sink, work_seq, work_qoff,
+                            tickets)
     Hq, Hkv, D, page_size, args, sink_at, unaligned = _attention(what, out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len,
                                                                  block_table, window, sink)
     if not attention_f8_fits(q.dtype, Hq, Hkv, D, page_size):
@@ -229,9 +235,19 @@ def attention_prefill_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
     if not scale > 0:
         raise KernelError(f"{what}: scale must be positive")
     n = _work(what, work_seq, work_qoff)
-    _check(_entry("ptl_attention_prefill_f8")(*args, work_seq.data_ptr(), work_qoff.data_ptr(), n,
-                                              min(n, int(groups) if groups > 0 else n, 65535), block_rows, Hq, Hkv, D, page_size,
-                                              int(window), sink_at, scale, stream), what)
+    if n == 0:
+        return
+    groups = min(n, groups, 65535) if groups > 0 else min(n, 65535)
+    cap, work, work_at, tickets_at = 0, None, None, None
+    if groups == n <= 64 and block_table.shape[1] * page_size > 64 * WHOLE_TILES:
+        resident = compute_units(q.device) * (3 if D <= 64 else 2) // Hq        # workgroups of a head that run at once
+        if 2 * n <= resident and block_rows == 64:
+            cap = resident
+            work = torch.empty((n + cap) * Hq * block_rows * (D + 8), dtype=torch.float32, device=q.device)
+            tickets = _tickets(tickets, TICKET * n * Hq, q, what)
+            work_at, tickets_at = work.data_ptr(), tickets.data_ptr()
+    _check(_entry("ptl_attention_prefill_f8")(*args, work_seq.data_ptr(), work_qoff.data_ptr(), n, groups, cap, work_at, tickets_at,
+                                              block_rows, Hq, Hkv, D, page_size, int(window), sink_at, scale, stream), what)
 
 
 def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:
