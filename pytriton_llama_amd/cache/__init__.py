@@ -1,2 +1,2 @@
-from .manager import RELEASED, CacheManager, OutOfPages, OutOfSlots, PagedGroup, PagePool, StateGroup
+from .manager import RELEASED, CacheManager, CannotShare, OutOfPages, OutOfSlots, PagedGroup, PagePool, StateGroup
 from .storage import CacheStorage, PagedLayerView, StateLayerView

@@ -7,7 +7,7 @@ gives them back when the whole batch is done
 Here the unit is a page of ``page_size`` tokens, pages are taken when a request's
 tokens need them and go back on the free list when the request ends or, for a
 group whose queries read a window or a chunk of the positions, when every later query has moved
-past them. All of it is
+past them. Requests that branch from one another share the full pages they have in common (``fork``). All of it is
 host-side bookkeeping: no device call, no synchronisation.
 
 Cache layers with the same needs form a group; a group has a page pool and, for
@@ -37,15 +37,19 @@ class OutOfSlots(RuntimeError):
     """More live requests than state slots."""
 
 
+class CannotShare(RuntimeError):
+    """What a request has in the cache cannot be given to another one as it is."""
+
+
 class PagePool:
-    """Free list (LIFO) of page ids 0..num_pages-1 with a held/free flag per page."""
+    """Free list (LIFO) of page ids 0..num_pages-1 with, for every page, how many tables hold it."""
 
     def __init__(self, num_pages: int):
         if num_pages <= 0:
             raise ValueError("a page pool needs at least one page")
         self.num_pages = int(num_pages)
         self._free: List[int] = list(range(self.num_pages - 1, -1, -1))
-        self._held = [False] * self.num_pages
+        self._held = [0] * self.num_pages
 
     @property
     def num_free(self) -> int:
@@ -56,17 +60,29 @@ class PagePool:
             raise OutOfPages(f"{n} pages wanted, {len(self._free)} free")
         out = [self._free.pop() for _ in range(n)]
         for p in out:
-            self._held[p] = True
+            self._held[p] = 1
         return out
+
+    def share(self, pages: Sequence[int]) -> None:
+        """One more table holds these pages: each is given back once more before it is free."""
+        for p in pages:
+            if not (0 <= p < self.num_pages) or not self._held[p]:
+                raise RuntimeError(f"page {p} shared but not held")
+        for p in pages:
+            self._held[p] += 1
 
     def give_back(self, pages: Sequence[int]) -> None:
         for p in pages:
             if not (0 <= p < self.num_pages) or not self._held[p]:
                 raise RuntimeError(f"page {p} given back but not held")
-            self._held[p] = False
-            self._free.append(p)
+            self._held[p] -= 1
+            if not self._held[p]:
+                self._free.append(p)
 
     def is_held(self, p: int) -> bool:
+        return self._held[p] > 0
+
+    def holders(self, p: int) -> int:
         return self._held[p]
 
 
@@ -190,6 +206,48 @@ class CacheManager:
         self.num_tokens[req] = start + n_new
         return start
 
+    def fork(self, req, new, num_tokens: Optional[int] = None) -> List[Tuple[int, int, int]]:
+        """Make ``new`` a live request that has what ``req`` has in the cache, its first ``num_tokens``
+        tokens (None: all). Full pages are shared: nobody writes them again, and each is free once
+        both have given it back. A last page that is not full is the new request's own: returns the
+        copies to be made, (group, page to read, page to write). A state slot is taken; where the
+        model has state, the caller copies it (all tokens only). Changes nothing where it raises:
+        CannotShare if pages the new request will read are gone, or state is asked for that was, OutOfPages,
+        OutOfSlots."""
+        if req not in self.slot_of:
+            raise RuntimeError(f"request {req!r} is not live")
+        if new in self.slot_of:
+            raise RuntimeError(f"request {new!r} is already live")
+        have = self.num_tokens[req]
+        n = have if num_tokens is None else int(num_tokens)
+        if not 0 < n <= have:
+            raise ValueError(f"request {req!r} has {have} tokens in the cache, {n} wanted")
+        if self.states and n != have:
+            raise CannotShare(f"the state of request {req!r} is that of {have} tokens, not of {n}")
+        if not self._free_slots:
+            raise OutOfSlots(f"all {self.max_num_seqs} state slots are taken")
+        full, rest = divmod(n, self.page_size)
+        for g in self.paged:
+            table = g.tables[req]
+            first = g.first_needed_page(n)
+            needed = list(range(min(g.kept_pages(), first, full))) + list(range(min(first, full), full + (rest > 0)))
+            if any(table[i] < 0 for i in needed):
+                raise CannotShare(f"request {req!r} has given back pages that {n} tokens need")
+            if rest and not g.pool.num_free:
+                raise OutOfPages(f"request {new!r} needs a page of {g.spec} for what it does not share")
+        self.slot_of[new] = self._free_slots.pop()
+        self.num_tokens[new] = n
+        copies = []
+        for gi, g in enumerate(self.paged):
+            table = g.tables[req]
+            g.pool.share([p for p in table[:full] if p >= 0])
+            g.tables[new] = table[:full]
+            if rest:
+                (page,) = g.pool.take(1)
+                g.tables[new].append(page)
+                copies.append((gi, table[full], page))
+        return copies
+
     def slot_array(self, req, group: int, start: int, n: int) -> np.ndarray:
         """Flat cache slots page*page_size+offset of positions start..start+n-1 (int32)."""
         table = self.paged[group].tables[req]
@@ -244,16 +302,22 @@ class CacheManager:
     def check(self) -> None:
         """No page lost, held twice or free while in a table; slots likewise."""
         for gi, g in enumerate(self.paged):
-            seen = {}
+            seen: Dict[int, list] = {}
             for req, table in g.tables.items():
-                for p in table:
+                for i, p in enumerate(table):
                     if p < 0:
                         continue
-                    if p in seen:
-                        raise AssertionError(f"group {gi}: page {p} held by {seen[p]!r} and {req!r}")
                     if not g.pool.is_held(p):
                         raise AssertionError(f"group {gi}: page {p} of {req!r} is on the free list")
-                    seen[p] = req
+                    seen.setdefault(p, []).append((req, i))
+            for p, places in seen.items():
+                if len(places) != g.pool.holders(p):
+                    raise AssertionError(f"group {gi}: page {p} held by {[r for r, _ in places]!r}, "
+                                         f"{g.pool.holders(p)} times by its count")
+                # a shared page is full for all who hold it, and the same piece of each
+                if len(places) > 1 and (len({i for _, i in places}) > 1 or len({r for r, _ in places}) < len(places)
+                                        or any((i + 1) * g.page_size > self.num_tokens[r] for r, i in places)):
+                    raise AssertionError(f"group {gi}: page {p} held by {[r for r, _ in places]!r} is not theirs to share")
             if len(seen) + g.pool.num_free != g.pool.num_pages:
                 raise AssertionError(f"group {gi}: {len(seen)} held + {g.pool.num_free} free "
                                      f"!= {g.pool.num_pages} pages")

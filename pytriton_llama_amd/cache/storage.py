@@ -2,10 +2,11 @@
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Sequence
 
 import torch
 
+from .. import ops
 from .manager import CacheManager
 
 
@@ -77,6 +78,16 @@ class CacheStorage:
                                   self.manager.page_size, writable)
         return StateLayerView(self.state_pools[g][i], g, writable)
 
+    def copy_pages(self, group: int, src: Sequence[int], dst: Sequence[int]) -> None:
+        """Page src[i] -> page dst[i] of a paged group, all its layers and tensors."""
+        if src:
+            ops.copy_pages(list(self.paged_pools[group].values()), src, dst)
+
+    def copy_slot(self, src: int, dst: int) -> None:
+        """The fixed-size state of one state slot into another."""
+        for pool in self.state_pools:
+            pool[:, dst].copy_(pool[:, src])
+
     def clear_slot(self, slot: int) -> None:
         """A new request starts from zero state."""
         for pool in self.state_pools:
@@ -101,8 +112,8 @@ class CacheStorage:
         total = 0
         for g in manager.paged:
             for t in g.spec.tensors:
-                n = g.page_size
-                for d in t.shape:
+                n = 1
+                for d in t.page_shape(g.page_size):
                     n *= int(d)
                 total += len(g.layers) * n * _element_size(t.dtype or dtype)
         return total

@@ -45,6 +45,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--prompt_ids", action="append", default=None,
                     help="prompt as token ids, e.g. '1,5,17' (repeatable)")
     ap.add_argument("--stream", type=_bool, default=True)
+    ap.add_argument("--cache_dtype", default=None, help="float8_e4m3fn: keys and values in 8 bits (default: as --dtype)")
+    ap.add_argument("--samples", type=int, default=1, help="completions of every prompt, which is computed once")
     return ap
 
 
@@ -72,10 +74,19 @@ def main(argv: Optional[List[str]] = None) -> int:
         max_gpu_num_blocks=args.max_gpu_num_blocks, load_model=args.load_model,
         triton_weight=args.triton_weight, compiled_model=args.compiled_model, dtype=args.dtype,
         seed=args.seed, page_size=args.page_size, max_batch_size=args.max_batch_size,
-        max_num_batched_tokens=args.max_num_batched_tokens, prefill_chunk=args.prefill_chunk)
+        max_num_batched_tokens=args.max_num_batched_tokens, prefill_chunk=args.prefill_chunk,
+        cache_dtype=args.cache_dtype)
 
     def run(prompts_text, prompts_ids):
-        if prompts_ids is not None:
+        if args.samples > 1 and prompts_ids is not None:
+            for group in gen.generate_samples(prompts_ids, args.samples, args.max_gen_len, args.temperature, args.top_p)[0]:
+                for ids in group:
+                    print(" ".join(map(str, ids)))
+        elif args.samples > 1:
+            for group in gen.text_samples(prompts_text, args.samples, args.temperature, args.top_p, args.max_gen_len):
+                for c in group:
+                    print(c["generation"])
+        elif prompts_ids is not None:
             stream = gen.generate_stream(prompts_ids, args.max_gen_len, args.temperature, args.top_p)
             done = [[] for _ in prompts_ids]
             for batch in stream:

@@ -29,6 +29,19 @@ def parse_dtype(name) -> torch.dtype:
         raise ValueError(f"engine dtype must be one of {sorted(_DTYPES)}, got {name!r}") from None
 
 
+_CACHE_DTYPES = {"float8_e4m3fn": torch.float8_e4m3fn, "float8_e4m3": torch.float8_e4m3fn, "fp8": torch.float8_e4m3fn}
+
+
+def parse_cache_dtype(name) -> Optional[torch.dtype]:
+    """The type keys and values are held in: None is the engine's."""
+    if name is None or name == torch.float8_e4m3fn:
+        return name
+    try:
+        return _CACHE_DTYPES[str(name).lower()]
+    except KeyError:
+        raise ValueError(f"cache dtype must be one of {sorted(_CACHE_DTYPES)} (or None, the engine's), got {name!r}") from None
+
+
 @dataclass
 class EngineConfig:
     dtype: torch.dtype = torch.bfloat16
@@ -52,11 +65,17 @@ class EngineConfig:
                                              # result). Which one wins can differ between processes,
                                              # and with it the last bit of bfloat16 results; False:
                                              # always the library's first, the same bits every time
+    cache_dtype: Optional[torch.dtype] = None    # "float8_e4m3fn": keys and values in 8 bits with a scale
+                                             # a page and kv head, half the memory of bfloat16 and half
+                                             # of what decode attention reads; results are those of
+                                             # keys and values rounded to four significant bits. For
+                                             # models whose mixers know it (paged_attention)
     async_decode: bool = True                # launch a decode step before the tokens of the one
                                              # before it have reached the host
 
     def __post_init__(self):
         self.dtype = parse_dtype(self.dtype)
+        self.cache_dtype = parse_cache_dtype(self.cache_dtype)
         if self.page_size <= 0:
             raise ValueError("page_size must be positive")
         if self.max_num_seqs <= 0 or self.max_num_batched_tokens <= 0:

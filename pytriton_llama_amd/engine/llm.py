@@ -1,6 +1,7 @@
 """The engine: a loaded model, its runner, a scheduler and a sampler."""
 from __future__ import annotations
 
+import dataclasses
 import itertools
 import os
 from typing import Dict, Hashable, Iterator, List, Optional, Sequence, Union
@@ -8,12 +9,12 @@ from typing import Dict, Hashable, Iterator, List, Optional, Sequence, Union
 import numpy as np
 import torch
 
-from ..cache import CacheManager, CacheStorage
+from ..cache import CacheManager, CacheStorage, CannotShare, OutOfPages, OutOfSlots
 from ..config import EngineConfig, build_model, read_config_json
 from ..sampling import Sampler
 from ..weights import load_random_weights, load_weights
 from .batch import StepEntry
-from .request import Request, SamplingParams, StepOutput
+from .request import FINISHED, Request, SamplingParams, StepOutput
 from .runner import ModelRunner
 from .scheduler import Scheduler
 
@@ -52,7 +53,7 @@ def pages_from_memory(model, engine: EngineConfig) -> int:
     are loaded (the reference: (total*0.9 - peak - non_torch) // bytes per block,
     lite_llama/executor/mem_manager.py:44-60,98-110), less what the state pools and the
     recorded steps' memory pool take."""
-    probe = CacheManager(model.cache_layers, engine.page_size, 1, engine.max_num_seqs)
+    probe = CacheManager(model.cache_layers_in(engine.cache_dtype), engine.page_size, 1, engine.max_num_seqs)
     per_page = CacheStorage.bytes_per_page(probe, engine.dtype)
     fixed = CacheStorage.state_bytes(probe, engine.dtype) + graph_pool_bytes(model, engine)
     free, total = torch.cuda.mem_get_info(torch.device(engine.device))
@@ -90,7 +91,7 @@ def make_decode_copies_if_room(model, device, keep_free_bytes: int) -> bool:
 def cache_floor_bytes(model, engine: EngineConfig) -> int:
     """The least the cache must get: the pages the engine was told to have, or those of one
     request of max_model_len tokens, plus the state pools and the recorded steps' pool."""
-    probe = CacheManager(model.cache_layers, engine.page_size, 1, engine.max_num_seqs)
+    probe = CacheManager(model.cache_layers_in(engine.cache_dtype), engine.page_size, 1, engine.max_num_seqs)
     pages = engine.num_pages if engine.num_pages is not None else -(-engine.max_model_len // engine.page_size)
     return (pages * CacheStorage.bytes_per_page(probe, engine.dtype)
             + CacheStorage.state_bytes(probe, engine.dtype) + graph_pool_bytes(model, engine))
@@ -143,7 +144,7 @@ class Engine:
             make_decode_copies_if_room(self.model, ec.device, cache_floor_bytes(self.model, ec))
         num_pages = ec.num_pages if ec.num_pages is not None else pages_from_memory(self.model, ec)
         self.runner = ModelRunner(self.model, ec.page_size, num_pages, ec.max_num_seqs,
-                                  ec.max_model_len, ec.use_graphs, ec.timed_library_products)
+                                  ec.max_model_len, ec.use_graphs, ec.timed_library_products, ec.cache_dtype)
         eos = getattr(self.model.config, "eos_token_ids", ())
         self.scheduler = Scheduler(self.runner.manager, ec.max_num_seqs, ec.max_num_batched_tokens,
                                    ec.prefill_chunk, ec.max_model_len, eos)
@@ -161,7 +162,7 @@ class Engine:
     # ---- requests ------------------------------------------------------------
     def add_request(self, prompt: Sequence[int], params: Optional[SamplingParams] = None,
                     request_id: Optional[Hashable] = None) -> Hashable:
-        rid = request_id if request_id is not None else next(self._ids)
+        rid = request_id if request_id is not None else self._new_id()
         if rid in self.requests:
             raise ValueError(f"request id {rid!r} is in use")
         V = self.model.vocab_size
@@ -174,6 +175,61 @@ class Engine:
         req = Request(rid, ids.astype(np.int32), params or SamplingParams())
         self.scheduler.add(req)
         self.requests[rid] = req
+        return rid
+
+    def fork(self, request_id: Hashable, params: Union[SamplingParams, Sequence[SamplingParams], None] = None,
+             count: int = 1, num_output: Optional[int] = None) -> List[Hashable]:
+        """Branch a request that is not finished: ``count`` new requests that continue its prompt and
+        the first ``num_output`` tokens of its output (None: all it has), each by itself. ``params``: theirs
+        (one, or one each; None: the request's own); max_new_tokens counts the output they start
+        with. A branch draws numbers of its own unless its params name a seed: one that shares the seed
+        repeats the request. What the request has in the cache is shared where that is possible
+        (CacheManager.fork) and there is room to run; otherwise the branch waits and is computed from its tokens,
+        like a preempted request. Returns the new requests' ids."""
+        req = self.requests.get(request_id)
+        if req is None or req.status == FINISHED:
+            raise ValueError(f"request {request_id!r} is not one that can branch")
+        if count < 1:
+            raise ValueError("a request branches into one more at least")
+        n = len(req.output) if num_output is None else int(num_output)
+        if not 0 <= n <= len(req.output):
+            raise ValueError(f"request {request_id!r} has {len(req.output)} tokens of output, {n} wanted")
+        params = req.params if params is None else params
+        params = [params] * count if isinstance(params, SamplingParams) else list(params)
+        if len(params) != count:
+            raise ValueError("one SamplingParams for every branch, or one for all")
+        if any(p.max_new_tokens <= n for p in params):
+            raise ValueError(f"a branch that starts with {n} tokens of output needs max_new_tokens beyond that")
+        branches = []
+        for p in params:
+            b = Request(self._new_id(), req.prompt_array, p, req.output[:n], req.output_logprobs[:n])
+            self.scheduler.check(b)
+            branches.append(b)
+        # every branch computes one token at least, the one whose logits it samples from
+        share = min(req.num_computed, len(req.prompt) + n - 1)
+        shared = False
+        if share > 0 and self.runner.manager.is_live(request_id) \
+                and len(self.scheduler.running) + count <= self.scheduler.max_num_seqs:
+            try:
+                self.runner.fork(request_id, [b.id for b in branches], share)
+                shared = True
+            except (CannotShare, OutOfPages, OutOfSlots):
+                pass
+        if shared:
+            for b in branches:
+                b.num_computed = share
+            self.scheduler.adopt(branches)
+        else:
+            for b in branches:
+                self.scheduler.add(b)
+        for b in branches:
+            self.requests[b.id] = b
+        return [b.id for b in branches]
+
+    def _new_id(self) -> Hashable:
+        rid = next(self._ids)
+        while rid in self.requests:
+            rid = next(self._ids)
         return rid
 
     def step(self) -> List[StepOutput]:
@@ -294,6 +350,34 @@ class Engine:
         while self.has_work:
             self.step()
         return [self.requests.pop(i) for i in ids]
+
+    def generate_samples(self, prompts: Sequence[Sequence[int]], count: int,
+                         params: Union[SamplingParams, Sequence[SamplingParams], None] = None) -> List[List[Request]]:
+        """``count`` finished requests for every prompt, each with tokens drawn by itself. A prompt is
+        computed once: when its first request has its first token the others branch off behind the
+        prompt. With a seed in a prompt's params its requests draw by seed, seed + 1, ..."""
+        if count < 1:
+            raise ValueError("one sample at least")
+        ids = self._add_all(prompts, params)
+        groups = {rid: [rid] for rid in ids}
+        waiting = set(ids) if count > 1 else set()
+        ended: Dict[Hashable, List[SamplingParams]] = {}
+        while self.has_work or ended:
+            for rid, each in ended.items():           # (its only token ended it: the prompt is computed again)
+                groups[rid] += [self.add_request(self.requests[rid].prompt_array, p) for p in each]
+            ended.clear()
+            for o in self.step():
+                if o.request not in waiting:
+                    continue
+                waiting.discard(o.request)
+                req = self.requests[o.request]
+                seed = req.params.seed
+                each = [dataclasses.replace(req.params, seed=None if seed is None else seed + i) for i in range(1, count)]
+                if req.status == FINISHED:
+                    ended[o.request] = each
+                else:
+                    groups[o.request] += self.fork(o.request, each, count - 1, num_output=0)
+        return [[self.requests.pop(r) for r in groups[rid]] for rid in ids]
 
     def generate_stream(self, prompts, params=None) -> Iterator[List[StepOutput]]:
         """Yields, step by step, the new token of every request that got one;

@@ -22,14 +22,14 @@ class ModelRunner:
 
     def __init__(self, model, page_size: int, num_pages, max_num_seqs: int,
                  max_model_len: Optional[int] = None, use_graphs: bool = False,
-                 timed_library_products: bool = True):
+                 timed_library_products: bool = True, cache_dtype: Optional[torch.dtype] = None):
         if model.dtype is None:
             raise RuntimeError("load the model's weights before making a runner")
         self.model = model
         self.device = model.device
         if self.device.type == "cuda":
-            ops.library.require(model.kernel_libraries())
-        self.manager = CacheManager(model.cache_layers, page_size, num_pages, max_num_seqs)
+            ops.library.require(model.kernel_libraries() + (("cache_f8", "attention_f8") if cache_dtype is not None else ()))
+        self.manager = CacheManager(model.cache_layers_in(cache_dtype), page_size, num_pages, max_num_seqs)
         self.storage = CacheStorage(self.manager, model.dtype, self.device)
         # decode-only steps replay a HIP graph when the longest request is known
         self.graphs = None
@@ -75,6 +75,26 @@ class ModelRunner:
         for e in entries:
             self.manager.release_behind_window(e.request)
         return logits
+
+    @torch.inference_mode()
+    def fork(self, request: Hashable, new: Sequence[Hashable], num_tokens: Optional[int] = None) -> None:
+        """Admit the requests ``new`` with what ``request`` has in the cache, its first ``num_tokens``
+        tokens (None: all): full pages are shared, the last one and the state copied, on the device and
+        behind the steps launched so far. All of them or, where this raises (as CacheManager.fork), none."""
+        copies: List[tuple] = []
+        made: List[Hashable] = []
+        try:
+            for n in new:
+                copies += self.manager.fork(request, n, num_tokens)
+                made.append(n)
+        except Exception:
+            for n in made:
+                self.manager.free(n)
+            raise
+        for g in range(len(self.manager.paged)):
+            self.storage.copy_pages(g, [s for h, s, _ in copies if h == g], [d for h, _, d in copies if h == g])
+        for n in made:
+            self.storage.copy_slot(self.manager.slot_of[request], self.manager.slot_of[n])
 
     def end(self, request: Hashable) -> None:
         """The request is finished: what it holds is given back."""

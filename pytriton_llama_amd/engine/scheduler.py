@@ -62,7 +62,8 @@ class Scheduler:
         self.num_preemptions = 0
 
     # ---- submitting -----------------------------------------------------------
-    def add(self, req: Request) -> None:
+    def check(self, req: Request) -> None:
+        """Raise where a request could never run."""
         if not req.prompt:
             raise ValueError(f"request {req.id!r} has an empty prompt")
         total = len(req.prompt) + req.params.max_new_tokens
@@ -74,8 +75,24 @@ class Scheduler:
             if -(-total // P) > g.pool.num_pages and not g.spec.gives_back:
                 raise ValueError(f"request {req.id!r} needs {-(-total // P)} pages, the pool has "
                                  f"{g.pool.num_pages}: it can never fit")
+
+    def add(self, req: Request) -> None:
+        self.check(req)
         req.status = WAITING
         self.waiting.append(req)
+
+    def adopt(self, reqs: Sequence[Request]) -> None:
+        """Take over requests that are live already, branches of a running one: they run from the next
+        step on, like ones that were admitted last."""
+        for req in reqs:
+            self.check(req)
+            if not self.manager.is_live(req.id) or not 0 < req.num_computed < req.num_tokens:
+                raise ValueError(f"request {req.id!r} is not a branch of a running one")
+        if len(self.running) + len(reqs) > self.max_num_seqs:
+            raise ValueError(f"{len(self.running)} requests are running, {len(reqs)} more are too many")
+        for req in reqs:
+            req.status = RUNNING
+            self.running.append(req)
 
     @property
     def has_work(self) -> bool:

@@ -42,20 +42,22 @@ class GenerateText:
     it the launch of a decode step ahead of the tokens of the step before; it is
     on by default (the reference's flag defaults to off, lite_llama/generate.py:59,
     and its captured graphs are never replayed, model_executor.py:314-320; here
-    the replayed step is the fast path and the one that is measured)."""
+    the replayed step is the fast path and the one that is measured).
+    cache_dtype "float8_e4m3fn" holds keys and values in 8 bits (None: in dtype)."""
 
     def __init__(self, checkpoints_dir: str, tokenizer_path: Optional[str] = None,
                  max_seq_len: int = 1024, max_gpu_num_blocks: Optional[int] = None,
                  load_model: bool = True, triton_weight: bool = True, compiled_model: bool = True,
                  device: str = "cuda", dtype: str = "bfloat16", seed: int = 0,
                  page_size: int = 16, max_batch_size: int = 64,
-                 max_num_batched_tokens: int = 2048, prefill_chunk: Optional[int] = None):
+                 max_num_batched_tokens: int = 2048, prefill_chunk: Optional[int] = None,
+                 cache_dtype: Optional[str] = None):
         dev = "cuda:0" if device == "cuda" else device
         self.engine_config = EngineConfig(
             dtype=dtype, device=dev, page_size=page_size, num_pages=max_gpu_num_blocks,
             max_num_seqs=max_batch_size, max_num_batched_tokens=max_num_batched_tokens,
             prefill_chunk=prefill_chunk, max_model_len=max_seq_len, seed=seed,
-            use_graphs=compiled_model)
+            use_graphs=compiled_model, cache_dtype=cache_dtype)
         self.engine = Engine(checkpoints_dir, self.engine_config,
                              random_seed=None if load_model else seed)
         self.model_config = self.engine.model.config
@@ -83,6 +85,28 @@ class GenerateText:
         if echo:
             outs = [list(p) + o for p, o in zip(prompt_tokens, outs)]
         return outs, ([r.output_logprobs for r in reqs] if logprobs else None)
+
+    def generate_samples(self, prompt_tokens: List[List[int]], count: int, max_gen_len: int, temperature: float = 0.6,
+                         top_p: float = 0.9, logprobs: bool = False
+                         ) -> Tuple[List[List[List[int]]], Optional[List[List[List[float]]]]]:
+        """As ``generate``, ``count`` times for every prompt, which is computed once: the tokens (and with
+        ``logprobs`` their log-probabilities) of every sample of every prompt."""
+        params = [self._params(max_gen_len, temperature, top_p, len(p), logprobs) for p in prompt_tokens]
+        groups = self.engine.generate_samples(prompt_tokens, count, params)
+        outs = [[r.output for r in g] for g in groups]
+        return outs, ([[r.output_logprobs for r in g] for g in groups] if logprobs else None)
+
+    def text_samples(self, prompts: List[str], count: int, temperature: float = 0.6, top_p: float = 0.9,
+                     max_gen_len: Optional[int] = None) -> List[List[dict]]:
+        """As ``text_completion``, ``count`` times for every prompt."""
+        if max_gen_len is None:
+            max_gen_len = self.engine_config.max_model_len - 1
+        groups, _ = self.generate_samples(self._encode(prompts), count, max_gen_len, temperature, top_p)
+        return [[self._text(ts) for ts in group] for group in groups]
+
+    def _text(self, tokens: List[int]) -> dict:
+        eos = set(self.model_config.eos_token_ids)
+        return {"generation": self.tokenizer.decode([t for t in tokens if t not in eos], skip_special_tokens=True)}
 
     def _need_tokenizer(self):
         if self.tokenizer is None:

@@ -80,6 +80,22 @@ class CausalLM:
     def is_ignorable(self, name: str) -> bool:
         return any(fnmatch.fnmatchcase(name, pat) for pat in self.ignorable)
 
+    def cache_layers_in(self, dtype: Optional[torch.dtype]) -> List[object]:
+        """The cache layers as their mixers hold them in ``dtype`` (None: the engine's). Every layer
+        has to be of a mixer that knows how (``cache_spec_in``, parts/base.py)."""
+        layers = list(self.cache_layers)
+        if dtype is None:
+            return layers
+        for call in self.schedule:
+            c = call.cache_layer
+            if c is None:
+                continue
+            mixer = getattr(self.blocks[call.block], "mixer", None)
+            if isinstance(c, (tuple, list)) or not says(mixer, "cache_spec_in") or self.cache_layers[c] != mixer.cache_spec():
+                raise ValueError(f"{type(mixer).__name__} holds its cache in the engine's type only, not in {dtype}")
+            layers[c] = mixer.cache_spec_in(dtype)
+        return layers
+
     def kernel_libraries(self) -> Tuple[str, ...]:
         libs: Tuple[str, ...] = ()
         for part in [self.embedding, *self.blocks, self.final_norm, self.head]:

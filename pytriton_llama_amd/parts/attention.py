@@ -74,6 +74,14 @@ class PagedAttention(Part):
     def cache_spec(self):
         return paged_kv_spec(self.num_kv_heads, self.head_dim, self.window)
 
+    def cache_spec_in(self, dtype: torch.dtype):
+        """The keys and values held in ``dtype``; ``forward`` takes the cache as it finds it."""
+        if dtype != ops.CACHE_F8:
+            raise ValueError(f"attention holds its cache in the engine's type or in {ops.CACHE_F8}, not in {dtype}")
+        if self.head_dim % 2:
+            raise ValueError(f"a cache in 8 bits takes even head sizes, got {self.head_dim}")
+        return paged_kv_spec(self.num_kv_heads, self.head_dim, self.window, dtype)
+
     @property
     def graph_capturable(self) -> bool:
         return self.position is None or getattr(self.position, "graph_capturable", True)
@@ -111,6 +119,8 @@ class PagedAttention(Part):
         T = x.shape[0]
         Hq, Hkv, D = self.num_heads, self.num_kv_heads, self.head_dim
         group = ctx.groups[cache.group]
+        if cache.k.dtype == ops.CACHE_F8:
+            return self._forward_f8(as_tensor(x), ctx, cache, group, defer_output)
         rotary = self.position.rotary_inv_freq() if self.position is not None else None
         fused = self.position is None or rotary is not None
         scale = None
@@ -145,6 +155,20 @@ class PagedAttention(Part):
         ops.rope_store(q, k, v, ctx.positions, inv_freq,
                        group.slots if cache.writable else None, cache.k, cache.v,
                        cache.page_size)
+        return self._attended(q, ctx, cache, group, defer_output)
+
+    def _forward_f8(self, x, ctx, cache, group, defer_output: bool):
+        """The same over a cache in 8 bits: the projection, then one kernel that rotates and stores."""
+        T, Hq, Hkv, D = x.shape[0], self.num_heads, self.num_kv_heads, self.head_dim
+        qkv = linear(x, self.qkv, blocked=self.qkv_blocked)
+        q = qkv[:, :self.q_size].view(T, Hq, D)
+        k = qkv[:, self.q_size:self.q_size + self.kv_size].view(T, Hkv, D)
+        v = qkv[:, self.q_size + self.kv_size:].view(T, Hkv, D)
+        inv_freq = self.position.rotary_inv_freq() if self.position is not None else None
+        if self.position is not None and inv_freq is None:
+            self.position.apply(q, k, ctx.positions)
+        q = ops.rope_store_f8(q, k, v, ctx.positions, inv_freq, group.slots if cache.writable else None, cache.k, cache.v,
+                              cache.k_scale, cache.v_scale)
         return self._attended(q, ctx, cache, group, defer_output)
 
     def _attended(self, q, ctx, cache, group, defer_output: bool):
@@ -208,6 +232,9 @@ class PagedAttention(Part):
         """``k`` / ``v``: the pools of keys and of values, [pages, Hkv, page_size, D] each, when
         they are not the cache layer's "k" and "v" (a mixer that keeps one tensor a token and
         reads it as both)."""
+        if k is None and cache.k.dtype == ops.CACHE_F8:
+            self._attend_f8(out, q, cache, ctx, group)
+            return
         k = cache.k if k is None else k
         v = cache.v if v is None else v
         D, window = self.head_dim, self.window or 0
@@ -244,3 +271,21 @@ class PagedAttention(Part):
             ops.attention_generic(out, q, k, v, ctx.q_start, ctx.ctx_len,
                                   group.block_table, ws, wo, self.scale, window, sink=self.sink)
 
+    def _attend_f8(self, out, q, cache, ctx, group) -> None:
+        D, window, n_dec = self.head_dim, self.window or 0, ctx.num_decode_seqs
+        held = (cache.k, cache.v, cache.k_scale, cache.v_scale)
+        tables = (ctx.q_start, ctx.ctx_len, group.block_table)
+        if not ops.attention_f8_fits(q.dtype, self.num_heads, self.num_kv_heads, D, cache.page_size):
+            ops.attention_generic_f8(out, q, *held, *tables, *ctx.work[ALL_16], self.scale, window, sink=self.sink)
+            return
+        if n_dec:
+            ops.attention_decode_f8(out, q, *held, *tables, n_dec, self.scale, window, sink=self.sink,
+                                    tickets=getattr(ctx, "tickets", None))
+        if n_dec == ctx.num_seqs:
+            return
+        keys = max(ctx.ctx_lens[n_dec:])
+        rows, groups = ops.attention_prefill_mfma_plan(
+            q.device, self.num_heads, D, ctx.work[PORTIONS_64][0].numel(), ctx.work[PORTIONS_128][0].numel(),
+            min(keys, window) if window else keys)
+        ops.attention_prefill_f8(out, q, *held, *tables, *ctx.work[PORTIONS_128 if rows == 128 else PORTIONS_64], self.scale, window,
+                                 rows, groups, sink=self.sink)

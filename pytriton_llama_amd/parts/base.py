@@ -16,6 +16,8 @@ every part:
     load(tensors, dtype, device)   take them (keyed by the same names); may fuse
 norm:            forward(x, residual) -> (y, new_residual)    residual may be None
 mixer:           cache_spec() -> PagedSpec | StateSpec | None
+                 cache_spec_in(dtype) -> PagedSpec   (optional) the same held in another type than
+                 the engine's (torch.float8_e4m3fn: 8 bits); its forward then finds that in the view
                  forward(x, ctx, cache) -> y      x, y: [T, hidden]
                  work_lists() -> WorkList, ...   (optional) how its kernels cut the query rows
 feed-forward:    forward(x) -> y
@@ -88,13 +90,17 @@ class PagedTensor:
     token; a page of the tensor has the shape shape[:token_axis] + (page_size,) +
     shape[token_axis:], so that a kernel can have the tokens of a page where it reads them
     best (keys and values: (kv heads, head size) with token_axis 1 gives pages of
-    [kv heads, page_size, head size])."""
+    [kv heads, page_size, head size]). ``per_page``: a page holds ``shape`` once, not for every
+    token (the scales of its numbers)."""
     name: str
     shape: Tuple[int, ...]
     token_axis: int = 0
     dtype: Optional[torch.dtype] = None     # None: the engine dtype
+    per_page: bool = False
 
     def page_shape(self, page_size: int) -> Tuple[int, ...]:
+        if self.per_page:
+            return tuple(self.shape)
         if not 0 <= self.token_axis <= len(self.shape):
             raise ValueError(f"paged tensor {self.name!r}: token_axis {self.token_axis} outside "
                              f"its {len(self.shape)} dimensions")
@@ -138,10 +144,16 @@ class PagedSpec:
         return 0
 
 
-def paged_kv_spec(num_kv_heads: int, head_dim: int, window: Optional[int] = None) -> PagedSpec:
-    """Keys and values of every token: tensors "k" and "v", pages of [kv heads, page_size, head size]."""
+def paged_kv_spec(num_kv_heads: int, head_dim: int, window: Optional[int] = None,
+                  dtype: Optional[torch.dtype] = None) -> PagedSpec:
+    """Keys and values of every token: tensors "k" and "v", pages of [kv heads, page_size, head size].
+    ``dtype`` torch.float8_e4m3fn: held in 8 bits, with "k_scale" and "v_scale", a float32 number a
+    page and kv head (ops/cache_f8.py)."""
     shape = (int(num_kv_heads), int(head_dim))
-    return PagedSpec((PagedTensor("k", shape, 1), PagedTensor("v", shape, 1)), window)
+    tensors = (PagedTensor("k", shape, 1, dtype), PagedTensor("v", shape, 1, dtype))
+    if dtype == torch.float8_e4m3fn:
+        tensors += tuple(PagedTensor(n, shape[:1], 0, torch.float32, per_page=True) for n in ("k_scale", "v_scale"))
+    return PagedSpec(tensors, window)
 
 
 @dataclass(frozen=True)

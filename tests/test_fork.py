@@ -1,0 +1,205 @@
+"""Requests that branch: who holds which page, on the CPU. And which models hold their cache in 8 bits."""
+import random
+
+import pytest
+import torch
+
+from pytriton_llama_amd.cache import RELEASED, CacheManager, CannotShare, OutOfPages, OutOfSlots
+from pytriton_llama_amd.cache.storage import CacheStorage
+from pytriton_llama_amd.config import EngineConfig, build_model
+from pytriton_llama_amd.engine.request import Request, SamplingParams
+from pytriton_llama_amd.engine.scheduler import Scheduler
+from pytriton_llama_amd.parts import StateSpec, paged_kv_spec
+from tiny_configs import tiny
+
+FULL = paged_kv_spec(2, 16)
+WIN = paged_kv_spec(2, 16, window=10)
+F8 = torch.float8_e4m3fn
+
+
+def live(m, name, n):
+    m.admit(name)
+    m.append(name, n)
+
+
+@pytest.mark.parametrize("n,shared,copied", [(1, 0, 1), (3, 0, 1), (4, 1, 0), (5, 1, 1), (8, 2, 0), (9, 2, 1), (None, 2, 1)])
+def test_full_pages_are_shared_and_the_last_one_is_copied(n, shared, copied):
+    m = CacheManager([FULL, FULL], page_size=4, num_pages=9, max_num_seqs=3)
+    live(m, "a", 9)
+    copies = m.fork("a", "b", n)
+    a, b = m.block_table("a", 0), m.block_table("b", 0)
+    assert b[:shared] == a[:shared] and len(b) == shared + copied
+    assert copies == ([(0, a[shared], b[shared])] if copied else [])
+    assert m.num_tokens["b"] == (9 if n is None else n) and m.slot_of["b"] != m.slot_of["a"]
+    assert m.paged[0].pool.num_free == 9 - 3 - copied
+    m.check()
+    m.append("b", 6)                                   # into pages of its own
+    assert set(m.block_table("b", 0)[shared:]).isdisjoint(a)
+    m.check()
+    m.free("a")
+    assert all(m.paged[0].pool.is_held(p) for p in m.block_table("b", 0))
+    m.check()
+    m.free("b")
+    assert m.paged[0].pool.num_free == 9
+    m.check()
+
+
+def test_a_fork_that_cannot_be_changes_nothing():
+    m = CacheManager([FULL], page_size=4, num_pages=3, max_num_seqs=2)
+    live(m, "a", 9)
+    for n in (0, 10, -1):
+        with pytest.raises(ValueError):
+            m.fork("a", "b", n)
+    with pytest.raises(OutOfPages):
+        m.fork("a", "b")
+    with pytest.raises(RuntimeError):
+        m.fork("x", "b")
+    with pytest.raises(RuntimeError):
+        m.fork("a", "a", 4)
+    m.check()
+    assert not m.is_live("b") and m.num_free_slots == 1
+    m.fork("a", "b", 8)
+    with pytest.raises(OutOfSlots):
+        m.fork("a", "c", 4)
+    m.check()
+
+
+def test_pages_that_a_window_has_left_behind():
+    m = CacheManager([WIN], page_size=4, num_pages=12, max_num_seqs=4)
+    live(m, "a", 30)
+    m.release_behind_window("a")
+    assert m.block_table("a", 0)[:5] == [RELEASED] * 5
+    m.fork("a", "b")
+    m.fork("a", "c", 29)                                # a query at 29 sees 20 .. 29: page 5 and on
+    with pytest.raises(CannotShare):
+        m.fork("a", "d", 28)                            # ... at 28 sees 19, on page 4
+    m.check()
+    for name in "abc":
+        m.append(name, 9)
+        m.release_behind_window(name)
+        m.check()
+    for name in "abc":
+        m.free(name)
+    assert m.paged[0].pool.num_free == 12
+
+
+def test_state_is_that_of_all_tokens():
+    m = CacheManager([FULL, StateSpec((3,))], page_size=4, num_pages=8, max_num_seqs=3)
+    live(m, "a", 9)
+    with pytest.raises(CannotShare):
+        m.fork("a", "b", 8)
+    m.fork("a", "b", 9)
+    m.check()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_random_orders(seed):
+    rng = random.Random(seed)
+    m = CacheManager([FULL, WIN], page_size=3, num_pages=[40, 25], max_num_seqs=7)
+    names = iter(range(10 ** 6))
+    for _ in range(400):
+        alive = list(m.slot_of)
+        what = rng.random()
+        try:
+            if what < 0.2 or not alive:
+                n = next(names)
+                m.admit(n)
+                if m.can_append(n, 5):
+                    m.append(n, rng.randint(1, 5))
+                else:
+                    m.free(n)
+            elif what < 0.4 and m.num_tokens[alive[0]]:
+                r = rng.choice([a for a in alive if m.num_tokens[a]])
+                m.fork(r, next(names), rng.choice([None, rng.randint(1, m.num_tokens[r])]))
+            elif what < 0.8:
+                r, k = rng.choice(alive), rng.randint(1, 7)
+                if m.can_append(r, k):
+                    m.append(r, k)
+                    m.release_behind_window(r)
+            else:
+                m.free(rng.choice(alive))
+        except (OutOfSlots, OutOfPages, CannotShare):
+            pass
+        m.check()
+    for r in list(m.slot_of):
+        m.free(r)
+    assert [g.pool.num_free for g in m.paged] == [40, 25]
+
+
+def test_check_finds_a_page_held_without_being_shared():
+    m = CacheManager([FULL], page_size=4, num_pages=8, max_num_seqs=3)
+    live(m, "a", 8)
+    live(m, "b", 4)
+    m.paged[0].tables["b"][0] = m.paged[0].tables["a"][0]
+    with pytest.raises(AssertionError):
+        m.check()
+
+
+def test_the_scheduler_runs_branches_and_preempts_them():
+    m = CacheManager([FULL], page_size=4, num_pages=6, max_num_seqs=3)
+    s = Scheduler(m, 3, 64, eos_token_ids=())
+    a = Request("a", list(range(7)), SamplingParams(max_new_tokens=8))
+    s.add(a)
+
+    def step():
+        plan = s.schedule()
+        for e in plan.entries:
+            if not m.is_live(e.request.id):
+                m.admit(e.request.id)
+            m.append(e.request.id, e.num_tokens)
+        s.update(plan, {e.request.id: 1 for e in plan.entries if e.samples})
+        m.check()
+        return [(e.request.id, e.num_tokens) for e in plan.entries]
+    assert step() == [("a", 7)]
+    branches = [Request(n, a.prompt, a.params) for n in "bc"]
+    for b in branches:
+        m.fork("a", b.id, 6)
+        b.num_computed = 6
+    with pytest.raises(ValueError):
+        s.adopt([Request("x", [1, 2], SamplingParams())])        # lives nowhere
+    s.adopt(branches)
+    assert m.paged[0].pool.num_free == 6 - 2 - 2
+    assert step() == [("a", 1), ("b", 1), ("c", 1)]
+    seen = set()
+    while s.has_work:
+        seen |= {r for r, _ in step()}
+    assert seen == {"a", "b", "c"} and s.num_preemptions > 0
+    assert all(len(r.output) == 8 for r in [a] + branches) and m.paged[0].pool.num_free == 6
+
+
+# ---- which models hold their cache in 8 bits -----------------------------------------------------
+def test_the_llama_cache_in_8_bits():
+    cfg = EngineConfig(cache_dtype="fp8", max_num_seqs=4)
+    assert cfg.cache_dtype == F8 and EngineConfig().cache_dtype is None and EngineConfig(cache_dtype=F8).cache_dtype == F8
+    with pytest.raises(ValueError):
+        EngineConfig(cache_dtype="int8")
+    model = build_model(tiny("B")[0])
+    assert model.cache_layers_in(None) == model.cache_layers
+    layers = model.cache_layers_in(F8)
+    assert [t.name for t in layers[0].tensors] == ["k", "v", "k_scale", "v_scale"] and len(set(layers)) == 1
+    m = CacheManager(layers, 16, 5, 2)
+    storage = CacheStorage(m, torch.bfloat16, "cpu")
+    view = storage.view(1)
+    assert view.k.shape == (5, 1, 16, 32) and view.k.dtype == F8 and view.k_scale.shape == (5, 1)
+    assert view.v_scale.dtype == torch.float32
+    assert CacheStorage.bytes_per_page(m, torch.bfloat16) == 3 * 2 * (16 * 32 + 4)
+    plain = CacheManager(model.cache_layers, 16, 5, 2)
+    assert CacheStorage.bytes_per_page(plain, torch.bfloat16) == 3 * 2 * 16 * 32 * 2
+
+
+def other_models():
+    import bimopel_configs
+    import fogapel_configs
+    import matusun_configs
+    import rubasun_configs
+    import senavik_configs
+    import virusun_configs
+    return [bimopel_configs, fogapel_configs, matusun_configs, rubasun_configs, senavik_configs, virusun_configs]
+
+
+@pytest.mark.parametrize("module", other_models(), ids=lambda m: m.__name__)
+def test_other_models_refuse(module):
+    table = getattr(module, module.__name__.split("_")[0].upper())            # name -> (configuration, ...)
+    model = build_model(next(iter(table.values()))[0])
+    with pytest.raises(ValueError, match="engine's type only"):
+        model.cache_layers_in(F8)
