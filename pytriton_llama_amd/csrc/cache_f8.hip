@@ -34,51 +34,95 @@ __device__ __forceinline__ uint32_t two_codes(float a, float b) {
 // zeros); one that begins further back takes the block as it is, and where the new tokens need a larger scale the other rows'
 // codes are rounded anew to it. So a block's content does not depend on how often the same run is stored.
 //
-// The first workgroups store: every one makes the list of the rows that begin a run (of LISTED rows at a time) and its waves take
-// the tasks (run, kv head, keys or values) in turn, so a block belongs to one wave and no two waves write one scale. (A workgroup for
-// every row, most of which find that they begin nothing and leave, took 71 us where this takes X: 2,048 rows, 8 kv heads of 128.)
-// A wave holds the run's numbers of a head, up to HELD items of VEC pairs a lane, finds the largest and then
-// writes; runs with more items read (and rotate) the rest again. Behind them T workgroups that rotate the queries of one row each.
+// The first workgroups store, a wave a task (row that begins a run, kv head, keys or values): a block belongs to one wave and no two
+// waves write one scale. Up to DIRECT rows every row has its tasks, and the waves of rows that begin nothing leave. Beyond, a
+// workgroup makes the list of the rows that begin a run (of LISTED rows at a time) and its waves take their share of the
+// tasks; with a workgroup for every row 2,048 rows, 8 kv heads of 128, took 71 us where they take X.
+// A wave takes the rows of its run a chunk at a time, holds their numbers of a head and finds the largest; a run of one chunk (16 rows
+// of 128) is then written from the registers, a longer one read and rotated again. Behind them the workgroups that rotate the queries, a
+// row a wave.
+constexpr int DIRECT = 128;
 constexpr int LISTED = 2048;
-constexpr int HELD = 2;
+constexpr int ANGLES = 1024;         // cosines and sines that a wave keeps in LDS, and pairs that it holds: the rows of a chunk
 
-template <typename T, int VEC>
+// The run that begins at row t0, if one does: its keys or values of head h. A wave's work, or (TEAM) that of the workgroup's four.
+template <typename T, int VEC, bool TEAM>
 __device__ __forceinline__ void
-store_run(int t0, int h, bool values, int lane, const T* __restrict__ k, const T* __restrict__ v, long row_stride,
-          const int32_t* __restrict__ positions, const float* __restrict__ inv_freq, const int32_t* __restrict__ slots,
-          uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache, float* __restrict__ k_scale, float* __restrict__ v_scale, int T_,
-          int Hkv, int D, int page_size) {
+store_run(int t0, int h, bool values, int lane, int wave, float2* __restrict__ table, float* __restrict__ largest_of_wave, const T* __restrict__ k, const T* __restrict__ v,
+          long row_stride, const int32_t* __restrict__ positions, const float* __restrict__ inv_freq,
+          const int32_t* __restrict__ slots, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
+          float* __restrict__ k_scale, float* __restrict__ v_scale, int T_, int Hkv, int D, int page_size, int slots_in_all) {
   struct __attribute__((aligned(sizeof(T) * VEC))) Vec { T e[VEC]; };
-  const int half = D >> 1, per_row = half / VEC;               // items of VEC pairs in a row of D
-  const int slot = slots[t0], page = slot / page_size, off = slot - page * page_size;
-  int n = 1;                                                     // rows of the run
-  for (const int most = min(page_size - off, T_ - t0); n < most; n += 64) {
-    const bool next = n + lane < most && slots[t0 + n + lane] == slot + n + lane;
-    const unsigned long long stop = ~__ballot(next);
-    if (stop) { n += __ffsll(stop) - 1; break; }
-  }
-  n = __builtin_amdgcn_readfirstlane(n);
-  const int items = n * per_row;
+  constexpr int HELD = ANGLES / 64 / VEC;                        // items of VEC pairs a lane has of a chunk
+  constexpr int WAVES = TEAM ? 4 : 1;
+  const int w = TEAM ? wave : 0;
+  const int half = D >> 1, per_row = half / VEC, chunk = ANGLES / half;       // items in a row of D, rows of a chunk
   const T* from = (values ? v : k) + (size_t)t0 * row_stride + h * D;
+  const bool turn = inv_freq && !values;
+  // the slots from the row before on, a lane each
+  const int near = t0 - 1 + lane;
+  const int seen = near >= 0 && near < T_ ? slots[near] : -2;
+  const int slot = __builtin_amdgcn_readlane(seen, 1), before = __builtin_amdgcn_readlane(seen, 0);
+  const int page = slot / page_size, off = slot - page * page_size;
+  if (slot < 0 || slot >= slots_in_all || (before >= 0 && before == slot - 1 && off > 0)) return;     // no run begins here
+  const int most = min(page_size - off, T_ - t0);
+  int n;                                                         // rows of the run
+  {
+    const unsigned long long stop = ~(__ballot(lane <= most && seen == slot + lane - 1) | 1ull);      // (the first row without a next slot)
+    n = stop ? __ffsll(stop) - 2 : 63;
+    for (; n >= 63 && n < most; n += 64) {
+      const bool next = n + lane < most && slots[t0 + n + lane] == slot + n + lane;
+      const unsigned long long end = ~__ballot(next);
+      if (end) { n += __ffsll(end) - 1; break; }
+    }
+    n = __builtin_amdgcn_readfirstlane(min(n, most));
+  }
   float* scale = (values ? v_scale : k_scale) + (size_t)page * Hkv + h;
   uint8_t* const rows = (values ? v_cache : k_cache) + ((size_t)page * Hkv + h) * page_size * D;
-  const bool turn = inv_freq && !values;
   const float old = off > 0 ? *scale : 0.f;
 
-  // item i of the run: VEC pairs of row i / per_row
-  auto load = [&](int i, float (&a)[VEC], float (&b)[VEC]) __attribute__((always_inline)) {
-    const int r = i / per_row, j = (i - r * per_row) * VEC;
-    const T* at = from + (size_t)r * row_stride + j;
-    const Vec x = *reinterpret_cast<const Vec*>(at), y = *reinterpret_cast<const Vec*>(at + half);
-    const float pos = turn ? (float)positions[t0 + r] : 0.f;
+  // rows r0 .. of the run, as many as a chunk has: a and b hold item lane + 64 it of them, VEC pairs of one row
+  auto load = [&](int r0, float (&a)[HELD][VEC], float (&b)[HELD][VEC]) __attribute__((always_inline)) {
+    const int count = min(chunk, n - r0), items = count * per_row;
+    Vec x[HELD], y[HELD];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const float x1 = to_float<T>(x.e[e]), x2 = to_float<T>(y.e[e]);
-      float s = 0.f, c = 1.f;
-      if (turn) sincosf(pos * inv_freq[j + e], &s, &c);
-      a[e] = turn ? x1 * c - x2 * s : x1;
-      b[e] = turn ? x2 * c + x1 * s : x2;
+    for (int it = 0; it < HELD; ++it) {
+      const int i = min(lane + 64 * it, items - 1), r = i / per_row;
+      const T* at = from + (size_t)(r0 + r) * row_stride + (i - r * per_row) * VEC;
+      x[it] = *reinterpret_cast<const Vec*>(at);
+      y[it] = *reinterpret_cast<const Vec*>(at + half);
     }
+    if (turn) {
+      // the angles' cosines and sines once for the chunk, an angle a lane (sincosf is some hundred instructions: in the loop below
+      // they would be 16 times as many, and a launch that has one row a wave is the time of fetching them)
+      for (int i = lane; i < count * half; i += 64) {
+        const int r = i / half;
+        float s, c;
+        sincosf((float)positions[t0 + r0 + r] * inv_freq[i - r * half], &s, &c);
+        table[i] = make_float2(c, s);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");      // (the wave's own LDS: written above, read below)
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+#pragma unroll
+    for (int it = 0; it < HELD; ++it) {
+      const int i = min(lane + 64 * it, items - 1);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float x1 = to_float<T>(x[it].e[e]), x2 = to_float<T>(y[it].e[e]);
+        float2 cs = make_float2(1.f, 0.f);
+        if (turn) cs = table[i * VEC + e];                        // (row r's pairs begin at r * half)
+        a[it][e] = turn ? x1 * cs.x - x2 * cs.y : x1;
+        b[it][e] = turn ? x2 * cs.x + x1 * cs.y : x2;
+      }
+    }
+    if (turn) {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    return items;
   };
   auto largest_of = [&](const float (&a)[VEC], float m) {
 #pragma unroll
@@ -89,18 +133,18 @@ store_run(int t0, int h, bool values, int lane, const T* __restrict__ k, const T
     return m;
   };
   float a[HELD][VEC], b[HELD][VEC], m = 0.f;
+  int items = 0;
+  for (int r0 = w * chunk; r0 < n; r0 += WAVES * chunk) {
+    items = load(r0, a, b);                                       // (lanes behind the last item hold it once more)
 #pragma unroll
-  for (int it = 0; it < HELD; ++it)
-    if (lane + 64 * it < items) {
-      load(lane + 64 * it, a[it], b[it]);
-      m = largest_of(b[it], largest_of(a[it], m));
-    }
-  for (int i = lane + 64 * HELD; i < items; i += 64) {
-    float aa[VEC], bb[VEC];
-    load(i, aa, bb);
-    m = largest_of(bb, largest_of(aa, m));
+    for (int it = 0; it < HELD; ++it) m = largest_of(b[it], largest_of(a[it], m));
   }
   m = wave_max(m);
+  if constexpr (TEAM) {
+    if (lane == 0) largest_of_wave[wave] = m;
+    __syncthreads();                                              // (and every wave has read the scale there was)
+    m = fmaxf(fmaxf(largest_of_wave[0], largest_of_wave[1]), fmaxf(largest_of_wave[2], largest_of_wave[3]));
+  }
   int e_new = scale_exponent(m);
   if (off > 0) {
     const int e_old = max(-126, (int)(__float_as_uint(old) >> 23) - 127);
@@ -117,20 +161,19 @@ store_run(int t0, int h, bool values, int lane, const T* __restrict__ k, const T
       // (the run's own rows are left to the writes below: lanes of a wave would write them in no certain order)
       auto other = [&](int i) { const int r = i / D; return r < off || r >= off + n; };
       if (D % 4 == 0) {
-        for (int i = 4 * lane; i < page_size * D; i += 256)
+        for (int i = 4 * (64 * w + lane); i < page_size * D; i += 256 * WAVES)
           if (other(i)) *reinterpret_cast<uint32_t*>(rows + i) = again(*reinterpret_cast<const uint32_t*>(rows + i));
       } else {                                    // D is even: two neighbours lie in one row
-        for (int i = 2 * lane; i < page_size * D; i += 128)
+        for (int i = 2 * (64 * w + lane); i < page_size * D; i += 128 * WAVES)
           if (other(i)) *reinterpret_cast<uint16_t*>(rows + i) = (uint16_t)again(*reinterpret_cast<const uint16_t*>(rows + i));
       }
     }
   } else {
-    for (int i = n * D + 2 * lane; i < page_size * D; i += 128) *reinterpret_cast<uint16_t*>(rows + i) = 0;
+    for (int i = n * D + 2 * (64 * w + lane); i < page_size * D; i += 128 * WAVES) *reinterpret_cast<uint16_t*>(rows + i) = 0;
   }
-  if (lane == 0) *scale = power_of_two(e_new);
+  if (w == 0 && lane == 0) *scale = power_of_two(e_new);
   const float f = power_of_two(-e_new);
-  auto put = [&](int i, const float (&x)[VEC], const float (&y)[VEC]) __attribute__((always_inline)) {
-    const int r = i / per_row, j = (i - r * per_row) * VEC;
+  auto put = [&](int r, int j, const float (&x)[VEC], const float (&y)[VEC]) __attribute__((always_inline)) {
     uint8_t* const to = rows + (off + r) * D + j;
     if constexpr (VEC == 8) {
       uint2 lo, hi;
@@ -149,13 +192,13 @@ store_run(int t0, int h, bool values, int lane, const T* __restrict__ k, const T
       }
     }
   };
+  for (int r0 = w * chunk; r0 < n; r0 += WAVES * chunk) {
+    if (n > WAVES * chunk) items = load(r0, a, b);
 #pragma unroll
-  for (int it = 0; it < HELD; ++it)
-    if (lane + 64 * it < items) put(lane + 64 * it, a[it], b[it]);
-  for (int i = lane + 64 * HELD; i < items; i += 64) {
-    float aa[VEC], bb[VEC];
-    load(i, aa, bb);
-    put(i, aa, bb);
+    for (int it = 0; it < HELD; ++it) {
+      const int i = lane + 64 * it, r = i / per_row;
+      if (i < items) put(r0 + r, (i - r * per_row) * VEC, a[it], b[it]);
+    }
   }
 }
 
@@ -166,73 +209,115 @@ rope_store_f8_kernel(T* __restrict__ q_out, const T* __restrict__ q, const T* __
                      const int32_t* __restrict__ slots, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
                      float* __restrict__ k_scale, float* __restrict__ v_scale, int T_, int Hq, int Hkv, int D, int page_size,
                      int slots_in_all, int store_groups) {
-  extern __shared__ float cs[];                 // [2][D / 2]: cosines and sines of a query row's angles
+  __shared__ __attribute__((aligned(16))) float2 tables[4][ANGLES];
+  __shared__ float largest_of_wave[4];
   struct __attribute__((aligned(sizeof(T) * VEC))) Vec { T e[VEC]; };
   const int half = D >> 1, per_row = half / VEC;               // items of VEC pairs in a row of D
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if ((int)blockIdx.x >= store_groups) {
-    // ---- queries ----
-    const int t = blockIdx.x - store_groups;
-    const float pos = (float)positions[t];
-    for (int j = threadIdx.x; j < half; j += 256) {
-      float s = 0.f, c = 1.f;
-      if (inv_freq) sincosf(pos * inv_freq[j], &s, &c);
-      cs[j] = c;
-      cs[half + j] = s;
-    }
-    __syncthreads();
+    // ---- queries: a wave a row, of few rows a workgroup ----
+    const int share = T_ <= DIRECT ? 4 : 1, block = blockIdx.x - store_groups;
+    const int t = share == 4 ? block : 4 * block + wave;
+    if (t >= T_) return;
     const T* row = q + (size_t)t * row_stride;
     T* to = q_out + (size_t)t * Hq * D;
-    for (int i = threadIdx.x; i < Hq * per_row; i += 256) {
-      const int h = i / per_row, j = (i - h * per_row) * VEC;
-      Vec a = *reinterpret_cast<const Vec*>(row + h * D + j), b = *reinterpret_cast<const Vec*>(row + h * D + j + half);
-      if (inv_freq) {
+    const int total = Hq * per_row;
+    constexpr int AHEAD = VEC == 8 ? 4 : 8;
+    float2* const table = tables[wave];
+    for (int i0 = share == 4 ? 64 * wave : 0, at = i0; i0 < total; i0 += 64 * AHEAD * share) {
+      Vec x[AHEAD], y[AHEAD];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float x1 = to_float<T>(a.e[e]), x2 = to_float<T>(b.e[e]), c = cs[j + e], s = cs[half + j + e];
-          a.e[e] = from_float<T>(x1 * c - x2 * s);
-          b.e[e] = from_float<T>(x2 * c + x1 * s);
-        }
+      for (int n = 0; n < AHEAD; ++n) {
+        const int i = min(i0 + 64 * share * n + lane, total - 1), h = i / per_row, j = (i - h * per_row) * VEC;
+        x[n] = *reinterpret_cast<const Vec*>(row + h * D + j);
+        y[n] = *reinterpret_cast<const Vec*>(row + h * D + j + half);
       }
-      *reinterpret_cast<Vec*>(to + h * D + j) = a;
-      *reinterpret_cast<Vec*>(to + h * D + j + half) = b;
+      if (inv_freq && i0 == at) {                   // (the first time)
+        const float pos = (float)positions[t];
+        for (int j = lane; j < half; j += 64) {
+          float s, c;
+          sincosf(pos * inv_freq[j], &s, &c);
+          table[j] = make_float2(c, s);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      }
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n) {
+        const int i = i0 + 64 * share * n + lane;
+        if (i >= total) continue;
+        const int h = i / per_row, j = (i - h * per_row) * VEC;
+        if (inv_freq) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const float x1 = to_float<T>(x[n].e[e]), x2 = to_float<T>(y[n].e[e]);
+            const float2 cs = table[j + e];
+            x[n].e[e] = from_float<T>(x1 * cs.x - x2 * cs.y);
+            y[n].e[e] = from_float<T>(x2 * cs.x + x1 * cs.y);
+          }
+        }
+        *reinterpret_cast<Vec*>(to + h * D + j) = x[n];
+        *reinterpret_cast<Vec*>(to + h * D + j + half) = y[n];
+      }
     }
     return;
   }
   // ---- keys and values ----
+  if (T_ <= DIRECT) {
+    const int task = blockIdx.x * 4 + wave, t = task / (2 * Hkv), rest = task - t * 2 * Hkv;
+    if (t < T_)
+      store_run<T, VEC, false>(t, rest >> 1, rest & 1, lane, wave, tables[wave], nullptr, k, v, row_stride, positions, inv_freq, slots,
+                               k_cache, v_cache, k_scale, v_scale, T_, Hkv, D, page_size, slots_in_all);
+    return;
+  }
   __shared__ int16_t list[LISTED];
   __shared__ int counts[LISTED / 64];
-  const int waves = 4 * store_groups;
-  int next = blockIdx.x * 4 + wave;                 // this wave's next task, counted from the segment's first
+  // pages of more rows than a chunk has: a workgroup a task (us, pages of 64 rows of 128, 2,048 rows: a wave a task 49.5, so X)
+  const bool team = page_size * half > ANGLES;
+  const int step = team ? store_groups : 4 * store_groups;
+  int next = team ? blockIdx.x : blockIdx.x * 4 + wave;         // the next task, counted from the segment's first
   for (int seg = 0; seg < T_; seg += LISTED) {
-    const int len = min(LISTED, T_ - seg), turns = (len + 255) / 256;
-    uint32_t mine = 0;                              // the rows seg + 256 j + threadIdx.x that begin a run
-    for (int j = 0; j < turns; ++j) {
+    constexpr int TURNS = LISTED / 256;             // row seg + 256 j + threadIdx.x in turn j: all are asked for at once
+    int at[TURNS], before[TURNS];
+#pragma unroll
+    for (int j = 0; j < TURNS; ++j) {
       const int t = seg + 256 * j + threadIdx.x;
-      const int slot = t < T_ ? slots[t] : -1, before = t > 0 && t < T_ ? slots[t - 1] : -2;
-      const bool begins = slot >= 0 && slot < slots_in_all && (before != slot - 1 || before < 0 || slot % page_size == 0);
-      const unsigned long long all = __ballot(begins);
-      if (begins) mine |= 1u << j;
-      if (lane == 0) counts[4 * j + wave] = __popcll(all);
+      at[j] = t < T_ ? slots[t] : -1;
+      before[j] = t > 0 && t < T_ ? slots[t - 1] : -2;
+    }
+    unsigned long long all[TURNS];                  // the wave's rows that begin a run
+#pragma unroll
+    for (int j = 0; j < TURNS; ++j) {
+      all[j] = 0;
+      if (seg + 256 * j < T_)
+        all[j] = __ballot(at[j] >= 0 && at[j] < slots_in_all && (before[j] != at[j] - 1 || before[j] < 0 || at[j] % page_size == 0));
+      if (lane == 0) counts[4 * j + wave] = __popcll(all[j]);
     }
     __syncthreads();
     int total = 0;
-    for (int j = 0; j < turns; ++j) {
-      int at = 0;
+#pragma unroll
+    for (int j = 0; j < TURNS; ++j) {
+      int first = total;
+#pragma unroll
       for (int w = 0; w < 4; ++w) {
-        if (w == wave) at = total;
+        first += w < wave ? counts[4 * j + w] : 0;
         total += counts[4 * j + w];
       }
-      const bool begins = mine >> j & 1;
-      const unsigned long long all = __ballot(begins);
-      if (begins) list[at + __popcll(all & ((1ull << lane) - 1))] = (int16_t)(256 * j + threadIdx.x);
+      if (all[j] >> lane & 1) list[first + __popcll(all[j] & ((1ull << lane) - 1))] = (int16_t)(256 * j + threadIdx.x);
     }
     __syncthreads();
     total = __builtin_amdgcn_readfirstlane(total) * 2 * Hkv;
-    for (; next < total; next += waves) {
-      const int run = next / (2 * Hkv), task = next - run * 2 * Hkv;
-      store_run<T, VEC>(seg + __builtin_amdgcn_readfirstlane((int)list[run]), task >> 1, task & 1, lane, k, v, row_stride, positions,
-                        inv_freq, slots, k_cache, v_cache, k_scale, v_scale, T_, Hkv, D, page_size);
+    for (; next < total; next += step) {
+      const int run = next / (2 * Hkv), task = next - run * 2 * Hkv, t0 = seg + __builtin_amdgcn_readfirstlane((int)list[run]);
+      if (team) {
+        store_run<T, VEC, true>(t0, task >> 1, task & 1, lane, wave, tables[wave], largest_of_wave, k, v, row_stride, positions, inv_freq,
+                                slots, k_cache, v_cache, k_scale, v_scale, T_, Hkv, D, page_size, slots_in_all);
+        __syncthreads();                            // (the waves' largest numbers have been read)
+      } else {
+        store_run<T, VEC, false>(t0, task >> 1, task & 1, lane, wave, tables[wave], nullptr, k, v, row_stride, positions, inv_freq, slots,
+                                 k_cache, v_cache, k_scale, v_scale, T_, Hkv, D, page_size, slots_in_all);
+      }
     }
     next -= total;
     __syncthreads();
@@ -250,19 +335,19 @@ extern "C" int ptl_rope_store_f8(void* q_out, const void* q, const void* k, cons
   const int in_all = slots ? (int)min((long)pages * page_size, 0x7fffffffl) : 0;
   if (T >= 1 << 30 || Hkv >= 1 << 16) return PTL_ERR_ARG;
   // a wave for every task there can be, up to eight a compute unit
-  const int store_groups = slots ? (int)min(((long)T * 2 * Hkv + 3) / 4, 2l * compute_units()) : 0;
-  const int groups = T + store_groups;
-  const size_t lds = (size_t)D * sizeof(float);
+  const long tasks = ((long)T * 2 * Hkv + 3) / 4;
+  const int store_groups = !slots ? 0 : T <= DIRECT ? (int)tasks : (int)min(tasks, 2l * compute_units());
+  const int groups = (T <= DIRECT ? T : (T + 3) / 4) + store_groups;
   const bool vec = (D / 2) % 8 == 0 && row_stride % 8 == 0 && ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out) % 16 == 0;
   if (dtype == PTL_DTYPE_F32) {
     auto go = [&](auto kernel) {
-      kernel<<<groups, 256, lds, stream>>>((float*)q_out, (const float*)q, (const float*)k, (const float*)v, row_stride, positions,
+      kernel<<<groups, 256, 0, stream>>>((float*)q_out, (const float*)q, (const float*)k, (const float*)v, row_stride, positions,
                                            inv_freq, slots, k_cache, v_cache, k_scale, v_scale, T, Hq, Hkv, D, page_size, in_all, store_groups);
     };
     if (vec) go(rope_store_f8_kernel<float, 8>); else go(rope_store_f8_kernel<float, 1>);
   } else if (dtype == PTL_DTYPE_BF16) {
     auto go = [&](auto kernel) {
-      kernel<<<groups, 256, lds, stream>>>((bf16_t*)q_out, (const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, row_stride, positions,
+      kernel<<<groups, 256, 0, stream>>>((bf16_t*)q_out, (const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, row_stride, positions,
                                            inv_freq, slots, k_cache, v_cache, k_scale, v_scale, T, Hq, Hkv, D, page_size, in_all, store_groups);
     };
     if (vec) go(rope_store_f8_kernel<bf16_t, 8>); else go(rope_store_f8_kernel<bf16_t, 1>);
