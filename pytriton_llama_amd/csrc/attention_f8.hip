@@ -454,7 +454,8 @@ attn_decode_f8_kernel(const int32_t* __restrict__ ctx_len, const int32_t* __rest
   auto write = [&](int h, int d, float m, float l, float a) {
     const int head = head0 + h;
     if (sink) {
-      const float s = sink[head] * 1.4426950408889634f, to = fmaxf(m, s), f = __builtin_amdgcn_exp2f(m - to);
+      const float s = sink[head] * 1.4426950408889634f, top = fmaxf(m, s), to = top == -INFINITY ? 0.f : top;
+      const float f = __builtin_amdgcn_exp2f(m - to);
       l = l * f + __builtin_amdgcn_exp2f(s - to);
       a *= f;
     }
@@ -586,9 +587,11 @@ extern "C" int ptl_attention_decode_f8(void* out, long out_stride, const void* q
 
 // ===========================================================================
 // ptl_attention_prefill_f8: portions of prompts. A workgroup of four waves takes 64 RT query rows of one head, 16 RT a wave, and walks the
-// keys that they see in tiles of 64. A tile's codes come into registers, are turned into bfloat16 (with their scales) and
-// lie in LDS in two buffers: in the turn in which tile t is used, tile t + 1, which arrived during the turn before, is
-// converted into the other buffer and tile t + 2 sets out. Products, softmax and the layout of LDS are those of
+// keys that they see in tiles of 64. A tile's codes are turned into bfloat16 (with their scales) and lie in LDS in two buffers: in the
+// turn in which tile t is used, tile t + 1 is converted into the other buffer, and tile t + 2 sets out. With registers
+// between memory and the conversion it sets out at the turn's end: its codes then take no registers beside the products (us
+// before and behind the products, 32 heads: 2,048 rows of 64 36.9 35.2, 2,048 behind 2,048 of 128 in 128-row blocks 158 145; the conversion
+// between the two products instead of before them spills there, 353). Products, softmax and the layout of LDS are those of
 // attention_prefill.h: S^T = K Q^T, O^T += V^T P^T, sums of the rounded probabilities by one more product with ones.
 // Of a tile every wave brings 16 rows, which lie in one page: page and scales are the wave's, in scalar registers.
 //
@@ -598,7 +601,9 @@ extern "C" int ptl_attention_decode_f8(void* out, long out_stride, const void* q
 // 200 rows behind 3,000 keys of 128 66.5 36.1, 512 behind 8,000 of 128 189.5 127.4, 512 behind 1,024 of 64 23.2 23.1; with more blocks
 // 700 rows of 128 19.6 21.1, 1,500 behind 500 of 64 34.2 38.0, 1,531 behind 6,145 of 128 315 330.
 //
-// What bounds it: 1,531 rows behind 6,145 keys, 32 heads of 128: X
+// What bounds it: 1,531 rows behind 6,145 keys, 32 heads of 128, take 274 us in blocks of 128 rows (312 in blocks of 64): 173 GFLOP, 633
+// TFLOP/s, 41 % of what a large product of matrices reaches; the conversion of a tile, done once for each of the blocks that read it,
+// and the softmax share the vector units (the same attention over a bfloat16 cache, without the conversion: 250).
 struct PrefillF8Parts {
   float2 *acc, *ml;                // [part][head][RT][2 ND][2][thread], [part][head][RT][thread]
   int* tickets;                    // [block][head][TICKET]
@@ -613,7 +618,12 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
                        int page_shift, int window, const float* __restrict__ sink, float scale_log2, PrefillF8Parts parts) {
   constexpr int D = 32 * ND, BN = 64, ROWS = 64 * RT;
   constexpr int PIECES = D / 8;                     // 8-element pieces of a row: 8 codes, 16 bytes of bfloat16
+  // two row tiles: registers are short, so codes go to LDS without one in between, to a place of the wave's own (its 16 rows are whole
+  // kilobytes, 64 lanes of 16 bytes). us with and without, 32 heads of 128: 1,531 rows behind 6,145 keys 274 284, 2,048 behind 2,048
+  // 139 145; with one row tile 332 312, 185 171.
+  constexpr bool STAGED = RT == 2 && D % 64 == 0;
   __shared__ __attribute__((aligned(16))) bf16_t Ks[2][BN * D], Vs[2][BN * D];
+  __shared__ __attribute__((aligned(16))) uint8_t staged[STAGED ? 4 : 1][2][STAGED ? 16 * D : 16];
   // piece c of row r lies at c ^ swz(r), so that neither product's reads meet in a bank
   auto swz = [](int r) { return PIECES % 8 == 0 ? (r & 7) : ((r >> 1) & 3); };
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -728,10 +738,22 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
     auto load = [&](int t) __attribute__((always_inline)) {
       const uint64_t at = (uint64_t)(uint32_t)page * page_bytes + (uint32_t)(((k_begin + t * BN + 16 * wave) & page_mask) * D);
       const uint8_t *kr = k_head + at, *vr = v_head + at;
+      if constexpr (STAGED) {
+        auto to_lds = [&](const uint8_t* from, uint8_t* to) {
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + (uint32_t)(16 * lane)),
+                                           (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+        };
 #pragma unroll
-      for (int i = 0; i < ND; ++i) {
-        kc[i] = *reinterpret_cast<const uint2*>(kr + (uint32_t)(512 * i + 8 * lane));
-        vc[i] = *reinterpret_cast<const uint2*>(vr + (uint32_t)(512 * i + 8 * lane));
+        for (int i = 0; i < ND / 2; ++i) {
+          to_lds(kr + 1024 * i, &staged[wave][0][1024 * i]);
+          to_lds(vr + 1024 * i, &staged[wave][1][1024 * i]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+          kc[i] = *reinterpret_cast<const uint2*>(kr + (uint32_t)(512 * i + 8 * lane));
+          vc[i] = *reinterpret_cast<const uint2*>(vr + (uint32_t)(512 * i + 8 * lane));
+        }
       }
       const size_t block = (size_t)page * Hkv + kvh;
       ks = *(const __attribute__((address_space(4))) float*)(uintptr_t)(cache.k_scale + block);
@@ -739,6 +761,14 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
     };
     auto convert = [&](int t, bf16_t* Kb, bf16_t* Vb) __attribute__((always_inline)) {
       const int k0 = k_begin + t * BN + 16 * wave;
+      if constexpr (STAGED) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // the wave's codes have landed
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+          kc[i] = *reinterpret_cast<const uint2*>(&staged[wave][0][512 * i + 8 * lane]);
+          vc[i] = *reinterpret_cast<const uint2*>(&staged[wave][1][512 * i + 8 * lane]);
+        }
+      }
       if (k0 < k_lo || k0 + 16 > k_end) {           // rows that are no keys read as zeros (what lies there may be a NaN)
 #pragma unroll
         for (int i = 0; i < ND; ++i) {
@@ -751,6 +781,8 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
         *reinterpret_cast<bf16x8_t*>(Kb + store_at(i)) = eight_bf16(kc[i].x, kc[i].y, ks);
         *reinterpret_cast<bf16x8_t*>(Vb + store_at(i)) = eight_bf16(vc[i].x, vc[i].y, vs);
       }
+      // what was read is in registers: the next tile's codes may come to its place (free here: the products read none of it)
+      if constexpr (STAGED) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
     auto tile = [&](int k0, const bf16_t* Kb, const bf16_t* Vb, auto masked_tag) __attribute__((always_inline)) {
       constexpr bool MASKED = decltype(masked_tag)::value;
@@ -823,13 +855,16 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
       const int k0 = k_begin + t * BN;
       if (t + 1 < n_tiles) {
         convert(t + 1, Ks[1 - buffer], Vs[1 - buffer]);
-        if (t + 2 < n_tiles) { load(t + 2); load_page(t + 3); }
+        if constexpr (STAGED) {
+          if (t + 2 < n_tiles) { load(t + 2); load_page(t + 3); }
+        }
       }
       if (wave_has_rows && k0 <= max_q && k0 + BN > wave_lo) {
         const bool need_mask = k0 + BN - 1 > min_q || k0 + BN > k_end || k0 < wave_lo_last;
         if (need_mask) tile(k0, Ks[buffer], Vs[buffer], std::true_type{});
         else tile(k0, Ks[buffer], Vs[buffer], std::false_type{});
       }
+      if (!STAGED && t + 2 < n_tiles) { load(t + 2); load_page(t + 3); }
       __syncthreads();
     };
     if (t_first < n_tiles) {
@@ -897,7 +932,7 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       float l = l_sum[r];
-      if (sink) l += __builtin_amdgcn_exp2f(sink[head] * 1.4426950408889634f - m_run[r] * scale_log2);
+      if (sink && sink[head] > -INFINITY) l += __builtin_amdgcn_exp2f(sink[head] * 1.4426950408889634f - m_run[r] * scale_log2);
       if (16 * (RT * wave + r) + ln >= rows) continue;
       const float inv = l == 0.f ? 0.f : 1.0f / l;
       bf16_t* to = out + (size_t)(first + qoff + 16 * (RT * wave + r) + ln) * out_stride + (size_t)head * D + 4 * lg;

@@ -37,7 +37,7 @@ __device__ __forceinline__ uint32_t two_codes(float a, float b) {
 // The first workgroups store, a wave a task (row that begins a run, kv head, keys or values): a block belongs to one wave and no two
 // waves write one scale. Up to DIRECT rows every row has its tasks, and the waves of rows that begin nothing leave. Beyond, a
 // workgroup makes the list of the rows that begin a run (of LISTED rows at a time) and its waves take their share of the
-// tasks; with a workgroup for every row 2,048 rows, 8 kv heads of 128, took 71 us where they take X.
+// tasks; with a workgroup for every row 2,048 rows, 8 kv heads of 128, took 71 us, from lists they take 17.6.
 // A wave takes the rows of its run a chunk at a time, holds their numbers of a head and finds the largest; a run of one chunk (16 rows
 // of 128) is then written from the registers, a longer one read and rotated again. Behind them the workgroups that rotate the queries, a
 // row a wave.
@@ -45,13 +45,29 @@ constexpr int DIRECT = 128;
 constexpr int LISTED = 2048;
 constexpr int ANGLES = 1024;         // cosines and sines that a wave keeps in LDS, and pairs that it holds: the rows of a chunk
 
+// The factor that row m of q, k and v still lacks (ops.RowScale): rsqrt(sum_j partials[m][j] / size + eps); partials == null: none. For the
+// few rows of a decode step, whose norm is finished by who reads its product.
+constexpr int SCALED_ROWS = 16;      // no more than DIRECT
+struct RowFactor {
+  const float* partials;           // [T, count]
+  int count;
+  float inv_size, eps;
+  // by a whole wave
+  __device__ __forceinline__ float of(int m, int lane) const {
+    float sum = 0.f;
+    for (int j = lane; j < count; j += 64) sum += partials[(size_t)m * count + j];
+    return rsqrtf(wave_sum(sum) * inv_size + eps);
+  }
+};
+
 // The run that begins at row t0, if one does: its keys or values of head h. A wave's work, or (TEAM) that of the workgroup's four.
-template <typename T, int VEC, bool TEAM>
+template <typename T, int VEC, bool TEAM, bool SCALED>
 __device__ __forceinline__ void
 store_run(int t0, int h, bool values, int lane, int wave, float2* __restrict__ table, float* __restrict__ largest_of_wave, const T* __restrict__ k, const T* __restrict__ v,
           long row_stride, const int32_t* __restrict__ positions, const float* __restrict__ inv_freq,
           const int32_t* __restrict__ slots, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
-          float* __restrict__ k_scale, float* __restrict__ v_scale, int T_, int Hkv, int D, int page_size, int slots_in_all) {
+          float* __restrict__ k_scale, float* __restrict__ v_scale, int T_, int Hkv, int D, int page_size, int slots_in_all,
+          const RowFactor& factor, float* __restrict__ row_factor) {
   struct __attribute__((aligned(sizeof(T) * VEC))) Vec { T e[VEC]; };
   constexpr int HELD = ANGLES / 64 / VEC;                        // items of VEC pairs a lane has of a chunk
   constexpr int WAVES = TEAM ? 4 : 1;
@@ -92,6 +108,12 @@ store_run(int t0, int h, bool values, int lane, int wave, float2* __restrict__ t
       x[it] = *reinterpret_cast<const Vec*>(at);
       y[it] = *reinterpret_cast<const Vec*>(at + half);
     }
+    if constexpr (SCALED) {
+      for (int r = 0; r < count; ++r) {
+        const float f = factor.of(t0 + r0 + r, lane);
+        if (lane == 0) row_factor[r] = f;
+      }
+    }
     if (turn) {
       // the angles' cosines and sines once for the chunk, an angle a lane (sincosf is some hundred instructions: in the loop below
       // they would be 16 times as many, and a launch that has one row a wave is the time of fetching them)
@@ -101,27 +123,28 @@ store_run(int t0, int h, bool values, int lane, int wave, float2* __restrict__ t
         sincosf((float)positions[t0 + r0 + r] * inv_freq[i - r * half], &s, &c);
         table[i] = make_float2(c, s);
       }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");      // (the wave's own LDS: written above, read below)
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");        // (the wave's own LDS: written above, read below)
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
     for (int it = 0; it < HELD; ++it) {
       const int i = min(lane + 64 * it, items - 1);
+      float f = 1.f;
+      if constexpr (SCALED) f = row_factor[i / per_row];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        const float x1 = to_float<T>(x[it].e[e]), x2 = to_float<T>(y[it].e[e]);
+        float x1 = to_float<T>(x[it].e[e]), x2 = to_float<T>(y[it].e[e]);
+        if constexpr (SCALED) { x1 *= f; x2 *= f; }
         float2 cs = make_float2(1.f, 0.f);
         if (turn) cs = table[i * VEC + e];                        // (row r's pairs begin at r * half)
         a[it][e] = turn ? x1 * cs.x - x2 * cs.y : x1;
         b[it][e] = turn ? x2 * cs.x + x1 * cs.y : x2;
       }
     }
-    if (turn) {
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     return items;
   };
   auto largest_of = [&](const float (&a)[VEC], float m) {
@@ -202,15 +225,15 @@ store_run(int t0, int h, bool values, int lane, int wave, float2* __restrict__ t
   }
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256, 4)
+template <typename T, int VEC, bool SCALED>
+__global__ void __launch_bounds__(256, VEC == 8 ? 4 : 2)
 rope_store_f8_kernel(T* __restrict__ q_out, const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                      long row_stride, const int32_t* __restrict__ positions, const float* __restrict__ inv_freq,
                      const int32_t* __restrict__ slots, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
                      float* __restrict__ k_scale, float* __restrict__ v_scale, int T_, int Hq, int Hkv, int D, int page_size,
-                     int slots_in_all, int store_groups) {
+                     int slots_in_all, int store_groups, RowFactor factor) {
   __shared__ __attribute__((aligned(16))) float2 tables[4][ANGLES];
-  __shared__ float largest_of_wave[4];
+  __shared__ float largest_of_wave[4], row_factors[4][SCALED_ROWS];
   struct __attribute__((aligned(sizeof(T) * VEC))) Vec { T e[VEC]; };
   const int half = D >> 1, per_row = half / VEC;               // items of VEC pairs in a row of D
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -224,6 +247,7 @@ rope_store_f8_kernel(T* __restrict__ q_out, const T* __restrict__ q, const T* __
     const int total = Hq * per_row;
     constexpr int AHEAD = VEC == 8 ? 4 : 8;
     float2* const table = tables[wave];
+    float f = 1.f;
     for (int i0 = share == 4 ? 64 * wave : 0, at = i0; i0 < total; i0 += 64 * AHEAD * share) {
       Vec x[AHEAD], y[AHEAD];
 #pragma unroll
@@ -232,6 +256,7 @@ rope_store_f8_kernel(T* __restrict__ q_out, const T* __restrict__ q, const T* __
         x[n] = *reinterpret_cast<const Vec*>(row + h * D + j);
         y[n] = *reinterpret_cast<const Vec*>(row + h * D + j + half);
       }
+      if (SCALED && i0 == at) f = factor.of(t, lane);
       if (inv_freq && i0 == at) {                   // (the first time)
         const float pos = (float)positions[t];
         for (int j = lane; j < half; j += 64) {
@@ -248,11 +273,12 @@ rope_store_f8_kernel(T* __restrict__ q_out, const T* __restrict__ q, const T* __
         const int i = i0 + 64 * share * n + lane;
         if (i >= total) continue;
         const int h = i / per_row, j = (i - h * per_row) * VEC;
-        if (inv_freq) {
+        if (inv_freq || SCALED) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            const float x1 = to_float<T>(x[n].e[e]), x2 = to_float<T>(y[n].e[e]);
-            const float2 cs = table[j + e];
+            float x1 = to_float<T>(x[n].e[e]), x2 = to_float<T>(y[n].e[e]);
+            if constexpr (SCALED) { x1 *= f; x2 *= f; }
+            const float2 cs = inv_freq ? table[j + e] : make_float2(1.f, 0.f);
             x[n].e[e] = from_float<T>(x1 * cs.x - x2 * cs.y);
             y[n].e[e] = from_float<T>(x2 * cs.x + x1 * cs.y);
           }
@@ -267,71 +293,76 @@ rope_store_f8_kernel(T* __restrict__ q_out, const T* __restrict__ q, const T* __
   if (T_ <= DIRECT) {
     const int task = blockIdx.x * 4 + wave, t = task / (2 * Hkv), rest = task - t * 2 * Hkv;
     if (t < T_)
-      store_run<T, VEC, false>(t, rest >> 1, rest & 1, lane, wave, tables[wave], nullptr, k, v, row_stride, positions, inv_freq, slots,
-                               k_cache, v_cache, k_scale, v_scale, T_, Hkv, D, page_size, slots_in_all);
+      store_run<T, VEC, false, SCALED>(t, rest >> 1, rest & 1, lane, wave, tables[wave], nullptr, k, v, row_stride, positions, inv_freq, slots,
+                               k_cache, v_cache, k_scale, v_scale, T_, Hkv, D, page_size, slots_in_all, factor, row_factors[wave]);
     return;
   }
-  __shared__ int16_t list[LISTED];
-  __shared__ int counts[LISTED / 64];
-  // pages of more rows than a chunk has: a workgroup a task (us, pages of 64 rows of 128, 2,048 rows: a wave a task 49.5, so X)
-  const bool team = page_size * half > ANGLES;
-  const int step = team ? store_groups : 4 * store_groups;
-  int next = team ? blockIdx.x : blockIdx.x * 4 + wave;         // the next task, counted from the segment's first
-  for (int seg = 0; seg < T_; seg += LISTED) {
-    constexpr int TURNS = LISTED / 256;             // row seg + 256 j + threadIdx.x in turn j: all are asked for at once
-    int at[TURNS], before[TURNS];
+  if constexpr (!SCALED) {                         // (few rows: never here)
+    __shared__ int16_t list[LISTED];
+    __shared__ int counts[LISTED / 64];
+    // pages of more rows than a chunk has: a workgroup a task (us, pages of 64 rows of 128, 2,048 rows: a wave a task 49.5,
+    // so 16.9)
+    const bool team = page_size * half > ANGLES;
+    const int step = team ? store_groups : 4 * store_groups;
+    int next = team ? blockIdx.x : blockIdx.x * 4 + wave;         // the next task, counted from the segment's first
+    for (int seg = 0; seg < T_; seg += LISTED) {
+      constexpr int TURNS = LISTED / 256;             // row seg + 256 j + threadIdx.x in turn j: all are asked for at once
+      int at[TURNS], before[TURNS];
 #pragma unroll
-    for (int j = 0; j < TURNS; ++j) {
-      const int t = seg + 256 * j + threadIdx.x;
-      at[j] = t < T_ ? slots[t] : -1;
-      before[j] = t > 0 && t < T_ ? slots[t - 1] : -2;
-    }
-    unsigned long long all[TURNS];                  // the wave's rows that begin a run
-#pragma unroll
-    for (int j = 0; j < TURNS; ++j) {
-      all[j] = 0;
-      if (seg + 256 * j < T_)
-        all[j] = __ballot(at[j] >= 0 && at[j] < slots_in_all && (before[j] != at[j] - 1 || before[j] < 0 || at[j] % page_size == 0));
-      if (lane == 0) counts[4 * j + wave] = __popcll(all[j]);
-    }
-    __syncthreads();
-    int total = 0;
-#pragma unroll
-    for (int j = 0; j < TURNS; ++j) {
-      int first = total;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        first += w < wave ? counts[4 * j + w] : 0;
-        total += counts[4 * j + w];
+      for (int j = 0; j < TURNS; ++j) {
+        const int t = seg + 256 * j + threadIdx.x;
+        at[j] = t < T_ ? slots[t] : -1;
+        before[j] = t > 0 && t < T_ ? slots[t - 1] : -2;
       }
-      if (all[j] >> lane & 1) list[first + __popcll(all[j] & ((1ull << lane) - 1))] = (int16_t)(256 * j + threadIdx.x);
-    }
-    __syncthreads();
-    total = __builtin_amdgcn_readfirstlane(total) * 2 * Hkv;
-    for (; next < total; next += step) {
-      const int run = next / (2 * Hkv), task = next - run * 2 * Hkv, t0 = seg + __builtin_amdgcn_readfirstlane((int)list[run]);
-      if (team) {
-        store_run<T, VEC, true>(t0, task >> 1, task & 1, lane, wave, tables[wave], largest_of_wave, k, v, row_stride, positions, inv_freq,
-                                slots, k_cache, v_cache, k_scale, v_scale, T_, Hkv, D, page_size, slots_in_all);
-        __syncthreads();                            // (the waves' largest numbers have been read)
-      } else {
-        store_run<T, VEC, false>(t0, task >> 1, task & 1, lane, wave, tables[wave], nullptr, k, v, row_stride, positions, inv_freq, slots,
-                                 k_cache, v_cache, k_scale, v_scale, T_, Hkv, D, page_size, slots_in_all);
+      unsigned long long all[TURNS];                  // the wave's rows that begin a run
+#pragma unroll
+      for (int j = 0; j < TURNS; ++j) {
+        all[j] = 0;
+        if (seg + 256 * j < T_)
+          all[j] = __ballot(at[j] >= 0 && at[j] < slots_in_all && (before[j] != at[j] - 1 || before[j] < 0 || at[j] % page_size == 0));
+        if (lane == 0) counts[4 * j + wave] = __popcll(all[j]);
       }
+      __syncthreads();
+      int total = 0;
+#pragma unroll
+      for (int j = 0; j < TURNS; ++j) {
+        int first = total;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          first += w < wave ? counts[4 * j + w] : 0;
+          total += counts[4 * j + w];
+        }
+        if (all[j] >> lane & 1) list[first + __popcll(all[j] & ((1ull << lane) - 1))] = (int16_t)(256 * j + threadIdx.x);
+      }
+      __syncthreads();
+      total = __builtin_amdgcn_readfirstlane(total) * 2 * Hkv;
+      for (; next < total; next += step) {
+        const int run = next / (2 * Hkv), task = next - run * 2 * Hkv, t0 = seg + __builtin_amdgcn_readfirstlane((int)list[run]);
+        if (team) {
+          store_run<T, VEC, true, SCALED>(t0, task >> 1, task & 1, lane, wave, tables[wave], largest_of_wave, k, v, row_stride, positions, inv_freq,
+                                  slots, k_cache, v_cache, k_scale, v_scale, T_, Hkv, D, page_size, slots_in_all, factor, row_factors[wave]);
+          __syncthreads();                            // (the waves' largest numbers have been read)
+        } else {
+          store_run<T, VEC, false, SCALED>(t0, task >> 1, task & 1, lane, wave, tables[wave], nullptr, k, v, row_stride, positions, inv_freq, slots,
+                                   k_cache, v_cache, k_scale, v_scale, T_, Hkv, D, page_size, slots_in_all, factor, row_factors[wave]);
+        }
+      }
+      next -= total;
+      __syncthreads();
     }
-    next -= total;
-    __syncthreads();
   }
 }
 
 extern "C" int ptl_rope_store_f8(void* q_out, const void* q, const void* k, const void* v, long row_stride,
                                  const int32_t* positions, const float* inv_freq, const int32_t* slots, uint8_t* k_cache,
                                  uint8_t* v_cache, float* k_scale, float* v_scale, int T, int Hq, int Hkv, int D, int page_size,
-                                 int pages, int dtype, hipStream_t stream) {
+                                 int pages, const float* partials, int count, int size, float eps, int dtype, hipStream_t stream) {
   if (T <= 0) return PTL_OK;
   if (Hq <= 0 || Hkv <= 0 || D <= 0 || (D & 1) || D > 640 || page_size <= 0 || (long)page_size * D >= 1l << 30) return PTL_ERR_ARG;
   if (slots && (!k_cache || !v_cache || !k_scale || !v_scale)) return PTL_ERR_ARG;
   if (((uintptr_t)k_cache | (uintptr_t)v_cache) % 16) return PTL_ERR_ARG;
+  if (partials && (T > SCALED_ROWS || count <= 0 || size <= 0)) return PTL_ERR_ARG;
+  const RowFactor factor{partials, count, partials ? 1.0f / (float)size : 0.f, eps};
   const int in_all = slots ? (int)min((long)pages * page_size, 0x7fffffffl) : 0;
   if (T >= 1 << 30 || Hkv >= 1 << 16) return PTL_ERR_ARG;
   // a wave for every task there can be, up to eight a compute unit
@@ -342,15 +373,17 @@ extern "C" int ptl_rope_store_f8(void* q_out, const void* q, const void* k, cons
   if (dtype == PTL_DTYPE_F32) {
     auto go = [&](auto kernel) {
       kernel<<<groups, 256, 0, stream>>>((float*)q_out, (const float*)q, (const float*)k, (const float*)v, row_stride, positions,
-                                           inv_freq, slots, k_cache, v_cache, k_scale, v_scale, T, Hq, Hkv, D, page_size, in_all, store_groups);
+                                           inv_freq, slots, k_cache, v_cache, k_scale, v_scale, T, Hq, Hkv, D, page_size, in_all, store_groups, factor);
     };
-    if (vec) go(rope_store_f8_kernel<float, 8>); else go(rope_store_f8_kernel<float, 1>);
+    if (partials) { if (vec) go(rope_store_f8_kernel<float, 8, true>); else go(rope_store_f8_kernel<float, 1, true>); }
+    else if (vec) go(rope_store_f8_kernel<float, 8, false>); else go(rope_store_f8_kernel<float, 1, false>);
   } else if (dtype == PTL_DTYPE_BF16) {
     auto go = [&](auto kernel) {
       kernel<<<groups, 256, 0, stream>>>((bf16_t*)q_out, (const bf16_t*)q, (const bf16_t*)k, (const bf16_t*)v, row_stride, positions,
-                                           inv_freq, slots, k_cache, v_cache, k_scale, v_scale, T, Hq, Hkv, D, page_size, in_all, store_groups);
+                                           inv_freq, slots, k_cache, v_cache, k_scale, v_scale, T, Hq, Hkv, D, page_size, in_all, store_groups, factor);
     };
-    if (vec) go(rope_store_f8_kernel<bf16_t, 8>); else go(rope_store_f8_kernel<bf16_t, 1>);
+    if (partials) { if (vec) go(rope_store_f8_kernel<bf16_t, 8, true>); else go(rope_store_f8_kernel<bf16_t, 1, true>); }
+    else if (vec) go(rope_store_f8_kernel<bf16_t, 8, false>); else go(rope_store_f8_kernel<bf16_t, 1, false>);
   } else {
     return PTL_ERR_ARG;
   }

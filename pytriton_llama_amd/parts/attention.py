@@ -120,7 +120,7 @@ class PagedAttention(Part):
         Hq, Hkv, D = self.num_heads, self.num_kv_heads, self.head_dim
         group = ctx.groups[cache.group]
         if cache.k.dtype == ops.CACHE_F8:
-            return self._forward_f8(as_tensor(x), ctx, cache, group, defer_output)
+            return self._forward_f8(x, ctx, cache, group, defer_output)
         rotary = self.position.rotary_inv_freq() if self.position is not None else None
         fused = self.position is None or rotary is not None
         scale = None
@@ -160,15 +160,18 @@ class PagedAttention(Part):
     def _forward_f8(self, x, ctx, cache, group, defer_output: bool):
         """The same over a cache in 8 bits: the projection, then one kernel that rotates and stores."""
         T, Hq, Hkv, D = x.shape[0], self.num_heads, self.num_kv_heads, self.head_dim
-        qkv = linear(x, self.qkv, blocked=self.qkv_blocked)
+        inv_freq = self.position.rotary_inv_freq() if self.position is not None else None
+        scale = None
+        if isinstance(x, PendingScale) and (self.position is None or inv_freq is not None) and T <= ops.SCALED_ROWS:
+            x, scale = x.values, x.scale               # (of the product's rows as well as of its operand's)
+        qkv = linear(as_tensor(x), self.qkv, blocked=self.qkv_blocked)
         q = qkv[:, :self.q_size].view(T, Hq, D)
         k = qkv[:, self.q_size:self.q_size + self.kv_size].view(T, Hkv, D)
         v = qkv[:, self.q_size + self.kv_size:].view(T, Hkv, D)
-        inv_freq = self.position.rotary_inv_freq() if self.position is not None else None
         if self.position is not None and inv_freq is None:
             self.position.apply(q, k, ctx.positions)
         q = ops.rope_store_f8(q, k, v, ctx.positions, inv_freq, group.slots if cache.writable else None, cache.k, cache.v,
-                              cache.k_scale, cache.v_scale)
+                              cache.k_scale, cache.v_scale, scale)
         return self._attended(q, ctx, cache, group, defer_output)
 
     def _attended(self, q, ctx, cache, group, defer_output: bool):

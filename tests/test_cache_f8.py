@@ -1,8 +1,22 @@
 """What the faces of the 8-bit cache's kernels refuse before anything is launched (no GPU needed: a refusal comes first)."""
+import os
+import re
+
 import pytest
 import torch
 
 from pytriton_llama_amd import ops
+from pytriton_llama_amd.ops import cache_f8, library
+
+
+@pytest.mark.parametrize("name", sorted(cache_f8._ENTRIES))
+def test_entries_take_the_arguments_of_the_source(name):
+    """ctypes passes what is too many as an int: the types that the faces state are those of the source."""
+    lib, types = cache_f8._ENTRIES[name]
+    with open(os.path.join(library.CSRC_DIR, lib + ".hip"), encoding="utf-8") as f:
+        found = re.search(r'extern "C" int ' + name + r"\((.*?)\) \{", f.read(), re.S).group(1).split(",")
+    kinds = ["p" if "*" in a or "hipStream_t" in a else {"long": "l", "float": "f", "int": "i"}[a.split()[0]] for a in found]
+    assert "".join(kinds) == types
 
 
 def test_tensors_on_the_host_are_refused():

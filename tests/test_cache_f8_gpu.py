@@ -153,6 +153,41 @@ def test_store_at_the_edges_of_numbers(ops, dtype):
     assert torch.equal(kc.view(torch.uint8), vc.view(torch.uint8))
 
 
+@pytest.mark.parametrize("T,rotated", [(1, True), (5, True), (16, True), (16, False)])
+@pytest.mark.parametrize("D", [64, 34])
+def test_store_of_rows_that_lack_their_norms_factor(ops, T, rotated, D):
+    """The factor of a row is rsqrt(mean square + eps), off by at most 2^-20 here (a float32 sum of 80 numbers and the root); it
+    comes in before the rotation, so the numbers stored are those of rows that have it, but for that and a tie."""
+    Hq, Hkv, P = 6, 3, 16
+    g = torch.Generator().manual_seed(T + D)
+    x = torch.randn(T, (Hq + 2 * Hkv) * D, generator=g).bfloat16()
+    partials = torch.rand(T, 80, generator=g) * 50
+    f = torch.rsqrt(partials.double().sum(-1) / 512 + 1e-5)
+    pos = torch.arange(7, 7 + T, dtype=torch.int32)
+    inv = 10000.0 ** (-torch.arange(0, D, 2).float() / D) if rotated else None
+    slots = torch.arange(7, 7 + T, dtype=torch.int32)
+    cut = lambda y: [y[:, a * D:b * D].view(T, b - a, D) for a, b in ((0, Hq), (Hq, Hq + Hkv), (Hq + Hkv, Hq + 2 * Hkv))]   # noqa: E731
+    codes, scales = torch.zeros(2, 3, Hkv, P, D).to(F8).cuda(), torch.full((2, 3, Hkv), 2.0 ** -126, device="cuda")
+    got = ops.rope_store_f8(*cut(x.cuda()), pos.cuda(), None if inv is None else inv.cuda(), slots.cuda(), codes[0], codes[1], scales[0],
+                            scales[1], ops.RowScale(partials.cuda(), 512, 1e-5))
+    q, k, v = cut(x.double() * f[:, None])
+    want = plain_f8.rotate(q, pos, inv)
+    size = torch.cat([q.abs()[..., :D // 2] + q.abs()[..., D // 2:]] * 2, -1)
+    assert ((got.cpu().double() - want).abs() <= 2.0 ** -19 * size + 2.0 ** -8 * want.abs() * (1 + 2.0 ** -10)).all()
+    for i, new in enumerate((plain_f8.rotate(k, pos, inv), v)):
+        plain = plain_f8.Blocks(torch.zeros(3, Hkv, P, D).to(F8), torch.full((3, Hkv), 2.0 ** -126))
+        plain.store(new, slots.tolist())
+        held = codes[i].cpu().float().double() * scales[i].cpu().double()[:, :, None, None]
+        s = plain.scale[:, :, None, None]
+        assert ((held - plain.held).abs() <= 2 * 2.0 ** -4 * plain.held.abs() + 2.0 ** -9 * s).all()
+        assert ((held - plain.held).abs() > 2.0 ** -9 * s).double().mean() <= 2e-3
+    with pytest.raises(ops.KernelError):
+        y = torch.zeros(17, (Hq + 2 * Hkv) * D, dtype=torch.bfloat16, device="cuda")
+        c = [y[:, a * D:b * D].view(17, b - a, D) for a, b in ((0, Hq), (Hq, Hq + Hkv), (Hq + Hkv, Hq + 2 * Hkv))]
+        ops.rope_store_f8(*c, torch.zeros(17, dtype=torch.int32, device="cuda"), None, None, codes[0], codes[1], scales[0], scales[1],
+                          ops.RowScale(torch.ones(17, 4, device="cuda"), 4, 0.0))
+
+
 def test_store_of_nothing(ops):
     (kc, vc), (ks, vs) = empty_cache(3, 2, 16, 64)
     before = kc.view(torch.uint8).clone(), ks.clone()
