@@ -595,21 +595,25 @@ extern "C" int ptl_attention_decode_f8(void* out, long out_stride, const void* q
 // attention_prefill.h: S^T = K Q^T, O^T += V^T P^T, sums of the rounded probabilities by one more product with ones.
 // Of a tile every wave brings 16 rows, which lie in one page: page and scales are the wave's, in scalar registers.
 //
-// CUT (blocks of 64 rows): few of them. Their tiles are dealt out evenly: a block is cut into parts of about (all tiles) / cap
-// tiles, a workgroup a part, as the decode kernel cuts its sequences, and the workgroup of a block that is done last merges its
-// parts: sums lie in the workspace as the lanes hold them. Otherwise workgroups take whole blocks in turn. us, not cut and cut, 32 heads:
-// 200 rows behind 3,000 keys of 128 66.5 36.1, 512 behind 8,000 of 128 189.5 127.4, 512 behind 1,024 of 64 23.2 23.1; with more blocks
-// 700 rows of 128 19.6 21.1, 1,500 behind 500 of 64 34.2 38.0, 1,531 behind 6,145 of 128 315 330.
+// CUT: few blocks. Their tiles, one block's behind the other's, are dealt out evenly to the workgroups that the GPU runs at once: a
+// workgroup has a part of a block, blocks as a whole, and a part of one. It writes the sums of parts to the workspace as its lanes
+// hold them and, its tiles done, counts them; who is last of a block's merges them. (A part costs some 8 us, ten tiles: the writes' way
+// to memory, the count, and each part's way back, which is hidden behind the addition of the one before.) us, not cut and
+// cut, 32 heads, rows behind keys: blocks of 64 rows 200 behind 3,000 of 128 67.7 38.4, 512 behind 8,000 of 128 178 128, 512 behind 1,024
+// of 64 23.4 22.4, but 700 of 128 (11 blocks, 16 workgroups) 19.7 21.4, 1,500 behind 500 of 64 (24, 24) 34.2 42.5; of 128 rows 512 behind
+// 8,000 of 128 250 109, 1,100 behind 6,000 (9, 16) 253 180, 1,531 behind 6,145 (12, 16) 279 243, 1,600 behind 6,000 (13) 272 255, 1,700 (14)
+// 278 277, 2,048 behind 2,048 (16) 141 163; 1,000 behind 8,000 of 64 (8, 24) 183 114.
 //
-// What bounds it: 1,531 rows behind 6,145 keys, 32 heads of 128, take 274 us in blocks of 128 rows (312 in blocks of 64): 173 GFLOP, 633
-// TFLOP/s, 41 % of what a large product of matrices reaches; the conversion of a tile, done once for each of the blocks that read it,
-// and the softmax share the vector units (the same attention over a bfloat16 cache, without the conversion: 250).
+// What bounds it: 1,531 rows behind 6,145 keys, 32 heads of 128, take 243 us in blocks of 128 rows that are cut: 173 GFLOP, 713 TFLOP/s,
+// 46 % of what a large product of matrices reaches. The conversion of a tile, done once for each of the blocks that read it, and the
+// softmax share the vector units (the same attention over a bfloat16 cache, without the conversion and not cut: 250).
 struct PrefillF8Parts {
   float2 *acc, *ml;                // [part][head][RT][2 ND][2][thread], [part][head][RT][thread]
   int* tickets;                    // [block][head][TICKET]
   int cap;
 };
-constexpr int WHOLE_TILES = 6;     // tiles up to which a block is not cut
+constexpr int NEAR_TILES = 3;      // so far from a block's beginning and end it is not cut
+constexpr int WORTH_TILES = 12;    // blocks are cut where the longest becomes so many tiles shorter
 
 template <int ND, int RT, bool CUT>
 __global__ void __launch_bounds__(256, ND <= 2 ? 3 : 2)
@@ -663,38 +667,76 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
   auto value_at = [&](int dt) { return v_at[dt % (SWAPPED / 2)] + dt / (SWAPPED / 2) * 8 * SWAPPED; };
   const int seen_back = window > 0 ? window : 1 << 30;
 
-  int my_item = -1, part = 0, n_parts = 1;
+  // CUT: lane i has block i, tiles first_tile .. upto - 1 of the list's; bit i of todo: this workgroup has some of them
+  int first_tile = 0, upto = 0, piece = 1, my_lo = 0, my_hi = 0;
+  unsigned long long todo = 0;
   if constexpr (CUT) {
-    // lane i has block i
-    int tiles = -1;                                 // (of a block without rows)
+    int tiles = 0;                                  // (a block without keys has one, of none; one without rows none)
     if (lane < n_work) {
       const int seq = work_seq[lane], qoff = work_qoff[lane];
       const int qlen = tab.q_start[seq + 1] - tab.q_start[seq], ctx = tab.ctx_len[seq], rows = min(ROWS, qlen - qoff);
       const int first_q = ctx - qlen + qoff, k_lo = window > 0 ? max(0, first_q - window + 1) : 0;
-      if (rows > 0) tiles = max(0, (min(ctx, first_q + rows) - k_lo / BN * BN + BN - 1) / BN);
+      if (rows > 0) tiles = max(1, (min(ctx, first_q + rows) - k_lo / BN * BN + BN - 1) / BN);
     }
-    int total = max(tiles, 0);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
-    const int whole = max(parts.cap - n_work / 2, (3 * parts.cap + 3) / 4), piece = max(1, (total + whole - 1) / whole);
-    const int mine = tiles < 0 ? 0 : tiles <= WHOLE_TILES ? 1 : (tiles + piece - 1) / piece;
-    int upto = mine;
+    upto = tiles;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int x = __shfl_up(upto, o, 64);
       upto += lane >= o ? x : 0;
     }
-    const unsigned long long here = __ballot(upto > (int)blockIdx.y);
-    if (!here) return;                              // (more room than parts)
-    my_item = __ffsll(here) - 1;
-    n_parts = __builtin_amdgcn_readlane(mine, my_item);
-    part = blockIdx.y - (__builtin_amdgcn_readlane(upto, my_item) - n_parts);
+    first_tile = upto - tiles;
+    const int total = __builtin_amdgcn_readlane(upto, 63), groups = gridDim.y;
+    int longest = tiles;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o, 64));
+    longest = __builtin_amdgcn_readfirstlane(longest);
+    piece = max(NEAR_TILES + 1, (total + groups - 1) / groups);
+    if (longest - piece < WORTH_TILES && n_work <= groups) {
+      // a workgroup a block
+      piece = my_hi = 1 << 30;
+      todo = __ballot(tiles > 0 && lane == (int)blockIdx.y);
+    } else {
+      // where workgroup w begins: at tile w piece, or at a block's beginning or end that is near
+      auto begin = [&](int w) {
+        const int x = min(w * piece, total);
+        const unsigned long long near = __ballot(tiles > 0 && x < total && abs(x - first_tile) <= NEAR_TILES);
+        if (near) return __builtin_amdgcn_readlane(first_tile, __ffsll(near) - 1);
+        return total - x <= NEAR_TILES ? total : x;
+      };
+      my_lo = begin(blockIdx.y);
+      my_hi = begin(blockIdx.y + 1);
+      todo = __ballot(tiles > 0 && first_tile < my_hi && upto > my_lo);
+    }
   }
+  constexpr int WORDS = RT * 2 * ND * 2 * 256, ENDS = RT * 256;                  // of a part
+  unsigned long long cut_items = 0;                 // the blocks of which this workgroup has a part
+  // how many parts a block has, and the workgroup of the first: workgroups begin inside of it unless near its ends
+  auto parts_of = [&](int item, int& n_parts, int& first_group) {
+    const int inside = (__builtin_amdgcn_readlane(first_tile, item) + NEAR_TILES + piece) / piece;
+    n_parts = max(0, (__builtin_amdgcn_readlane(upto, item) - NEAR_TILES - 1) / piece - inside + 1) + 1;
+    first_group = inside - 1;
+  };
+  // what a lane has of row tile r of a block whose rows begin at row0
+  auto write = [&](int row0, int rows, int r, const f32x4_t* o, float m, float l) __attribute__((always_inline)) {
+    if (sink && sink[head] > -INFINITY) l += __builtin_amdgcn_exp2f(sink[head] * 1.4426950408889634f - m * scale_log2);
+    const int mine = 16 * (RT * wave + r) + ln;
+    if (mine >= rows) return;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    bf16_t* to = out + (size_t)(row0 + mine) * out_stride + (size_t)head * D + 4 * lg;
+#pragma unroll
+    for (int dt = 0; dt < 2 * ND; ++dt) {
+      union { uint2 u; bf16_t e[4]; } x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.e[i] = float_to_bf16(o[dt][i] * inv);
+      *reinterpret_cast<uint2*>(to + 16 * dt) = x.u;
+    }
+  };
   // not cut: the list is sorted, most keys first; the workgroups of a head walk it forwards and backwards in turn
   for (int round = 0;; ++round) {
-    const int item = CUT ? (round ? n_work : my_item)
+    const int item = CUT ? (todo ? __ffsll(todo) - 1 : n_work)
                          : round * gridDim.y + ((round & 1) ? gridDim.y - 1 - blockIdx.y : blockIdx.y);
     if (item >= n_work) break;
+    todo &= todo - 1;
     const int seq = work_seq[item], qoff = work_qoff[item];
     const int first = tab.q_start[seq], qlen = tab.q_start[seq + 1] - first, ctx = tab.ctx_len[seq];
     const int rows = min(ROWS, qlen - qoff);
@@ -726,7 +768,14 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
     }
     const int k_lo = window > 0 ? max(0, first_q - window + 1) : 0, k_end = min(ctx, first_q + rows);
     const int k_begin = k_lo / BN * BN, n_all = max(0, (k_end - k_begin + BN - 1) / BN);
-    const int per = (n_all + n_parts - 1) / n_parts, t_first = part * per, n_tiles = min(n_all, t_first + per);      // this part's tiles
+    int t_first = 0, n_tiles = n_all, n_parts = 1;   // this workgroup's tiles of the block
+    if constexpr (CUT) {
+      int first_group;
+      parts_of(item, n_parts, first_group);
+      const int begin = __builtin_amdgcn_readlane(first_tile, item);
+      t_first = max(my_lo - begin, 0);
+      n_tiles = min(n_all, my_hi - begin);
+    }
 
     uint2 kc[ND], vc[ND];
     float ks, vs;
@@ -879,14 +928,10 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
       turn(t, 0);
       if (t + 1 < n_tiles) turn(t + 1, 1);
     }
-    float l_sum[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) l_sum[r] = o[r][2 * ND][0];
     if constexpr (CUT) {
       if (n_parts > 1) {
-        __shared__ int last;
-        constexpr int WORDS = RT * 2 * ND * 2 * 256, ENDS = RT * 256;
-        const size_t first_part = (size_t)(blockIdx.y - part) * Hq + head, mine = (size_t)blockIdx.y * Hq + head;
+        cut_items |= 1ull << item;
+        const size_t mine = (size_t)(blockIdx.y + item) * Hq + head;         // (workgroup + block: goes up from part to part)
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
 #pragma unroll
@@ -894,54 +939,77 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
 #pragma unroll
             for (int x = 0; x < 2; ++x)
               put_shared2(parts.acc + mine * WORDS + ((r * 2 * ND + dt) * 2 + x) * 256 + threadIdx.x, o[r][dt][2 * x], o[r][dt][2 * x + 1]);
-          put_shared2(parts.ml + mine * ENDS + r * 256 + threadIdx.x, m_run[r], l_sum[r]);
+          put_shared2(parts.ml + mine * ENDS + r * 256 + threadIdx.x, m_run[r], o[r][2 * ND][0]);
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // this wave's share of the part has reached memory
-        __syncthreads();
-        if (threadIdx.x == 0) last = last_part(parts.tickets + ((size_t)item * Hq + head) * TICKET, n_parts);
-        __syncthreads();
-        if (!last) return;
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          float top = -INFINITY;
-          for (int p = 0; p < n_parts; ++p)
-            top = max2(top, get_shared2((const float*)(parts.ml + (first_part + (size_t)p * Hq) * ENDS + r * 256 + threadIdx.x)).x);
-          float l = 0.f;
-#pragma unroll
-          for (int dt = 0; dt < 2 * ND; ++dt) o[r][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-          for (int p = 0; p < n_parts; ++p) {                     // (in the order of the keys)
-            const size_t at = first_part + (size_t)p * Hq;
-            const float2 e = get_shared2((const float*)(parts.ml + at * ENDS + r * 256 + threadIdx.x));
-            // (a part that has seen no key has zero sums; its maximum, and where no part has seen one the largest too, is -inf)
-            const float f = e.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((e.x - top) * scale_log2);
-            l = fmaf(e.y, f, l);
-#pragma unroll
-            for (int dt = 0; dt < 2 * ND; ++dt)
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const float2 a = get_shared2((const float*)(parts.acc + at * WORDS + ((r * 2 * ND + dt) * 2 + x) * 256 + threadIdx.x));
-                o[r][dt][2 * x] = fmaf(a.x, f, o[r][dt][2 * x]);
-                o[r][dt][2 * x + 1] = fmaf(a.y, f, o[r][dt][2 * x + 1]);
-              }
-          }
-          m_run[r] = top;
-          l_sum[r] = l;
-        }
+        continue;
       }
     }
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      float l = l_sum[r];
-      if (sink && sink[head] > -INFINITY) l += __builtin_amdgcn_exp2f(sink[head] * 1.4426950408889634f - m_run[r] * scale_log2);
-      if (16 * (RT * wave + r) + ln >= rows) continue;
-      const float inv = l == 0.f ? 0.f : 1.0f / l;
-      bf16_t* to = out + (size_t)(first + qoff + 16 * (RT * wave + r) + ln) * out_stride + (size_t)head * D + 4 * lg;
+    for (int r = 0; r < RT; ++r) write(first + qoff, rows, r, o[r], m_run[r], o[r][2 * ND][0]);
+  }
+  if constexpr (CUT) {
+    // ---- parts: at most two, the end of a block and the beginning of one ----
+    if (!cut_items) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // this wave's share of them has reached memory
+    __syncthreads();
+    int* const told = reinterpret_cast<int*>(Ks[0]);          // (LDS is full to the last byte, and nobody reads keys any more)
+    int* ticket = nullptr;
+    int of = 0;
+    unsigned long long left = cut_items;
+    for (int i = 0; left; ++i, left &= left - 1) {
+      const int item = __ffsll(left) - 1;
+      int n_parts, first_group;
+      parts_of(item, n_parts, first_group);
+      if ((int)threadIdx.x == i) {
+        ticket = parts.tickets + ((size_t)item * Hq + head) * TICKET;
+        of = n_parts;
+      }
+    }
+    if (ticket) told[threadIdx.x] = last_part(ticket, of);
+    __syncthreads();
+    for (int i = 0; cut_items; ++i, cut_items &= cut_items - 1) {
+      if (!__builtin_amdgcn_readfirstlane(told[i])) continue;
+      const int item = __ffsll(cut_items) - 1;
+      int n_parts, first_group;
+      parts_of(item, n_parts, first_group);
+      const int seq = work_seq[item], qoff = work_qoff[item], first = tab.q_start[seq], rows = min(ROWS, tab.q_start[seq + 1] - first - qoff);
+      const size_t first_part = (size_t)(first_group + item) * Hq + head;
 #pragma unroll
-      for (int dt = 0; dt < 2 * ND; ++dt) {
-        union { uint2 u; bf16_t e[4]; } x;
+      for (int r = 0; r < RT; ++r) {
+        // in the order of the keys; while one part is added the next one is on its way
+        struct Part { float2 ml, acc[4 * ND]; };
+        Part even, odd;
+        auto bring = [&](Part& x, int p) __attribute__((always_inline)) {
+          const size_t at = first_part + (size_t)p * Hq;
+          x.ml = get_shared2((const float*)(parts.ml + at * ENDS + r * 256 + threadIdx.x));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x.e[i] = float_to_bf16(o[r][dt][i] * inv);
-        *reinterpret_cast<uint2*>(to + 16 * dt) = x.u;
+          for (int j = 0; j < 4 * ND; ++j) x.acc[j] = get_shared2((const float*)(parts.acc + at * WORDS + (r * 4 * ND + j) * 256 + threadIdx.x));
+        };
+        f32x4_t o[2 * ND];
+#pragma unroll
+        for (int dt = 0; dt < 2 * ND; ++dt) o[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+        auto add = [&](const Part& x) __attribute__((always_inline)) {
+          // (a part that has seen no key has zero sums and a maximum of -inf)
+          const float top = max2(m, x.ml.x), to = top == -INFINITY ? 0.f : top;
+          const float keep = __builtin_amdgcn_exp2f((m - to) * scale_log2), f = __builtin_amdgcn_exp2f((x.ml.x - to) * scale_log2);
+          m = top;
+          l = fmaf(l, keep, x.ml.y * f);
+#pragma unroll
+          for (int dt = 0; dt < 2 * ND; ++dt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[dt][j] = fmaf(o[dt][j], keep, (j & 1 ? x.acc[2 * dt + j / 2].y : x.acc[2 * dt + j / 2].x) * f);
+        };
+        bring(even, 0);
+        for (int p = 0; p < n_parts; p += 2) {
+          if (p + 1 < n_parts) bring(odd, p + 1);
+          add(even);
+          if (p + 1 < n_parts) {
+            if (p + 2 < n_parts) bring(even, p + 2);
+            add(odd);
+          }
+        }
+        write(first + qoff, rows, r, o, m, l);
       }
     }
   }
@@ -958,7 +1026,7 @@ extern "C" int ptl_attention_prefill_f8(void* out, long out_stride, const void* 
   if (!f8_matrix_sizes(Hq, Hkv, D, page_size) || window < 0 || groups <= 0 || groups > 65535 || (block_rows != 64 && block_rows != 128) ||
       !(scale > 0.f) || ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 || q_stride % 8 || (uintptr_t)out % 8 || out_stride % 4)
     return PTL_ERR_ARG;
-  if (cap < 0 || (cap && (block_rows != 64 || n_work > 64 || cap > 4096 || !work || (uintptr_t)work % 8 || !tickets))) return PTL_ERR_ARG;
+  if (cap < 0 || (cap && (n_work > 64 || cap > 4096 || !work || (uintptr_t)work % 8 || !tickets))) return PTL_ERR_ARG;
   const F8Cache cache{k, v, k_scale, v_scale};
   const F8Tables tab{q_start, ctx_len, block_table, bt_stride};
   const PrefillF8Parts parts{(float2*)work, (float2*)(work + (size_t)(n_work + cap) * Hq * block_rows * D), tickets, cap};
@@ -971,10 +1039,11 @@ extern "C" int ptl_attention_prefill_f8(void* out, long out_stride, const void* 
   auto size = [&](auto nd) {
     constexpr int ND = decltype(nd)::value;
     if (block_rows == 64) {
-      if (cap) go(attn_prefill_f8_kernel<ND, 1, true>, n_work + cap);
+      if (cap) go(attn_prefill_f8_kernel<ND, 1, true>, cap);
       else go(attn_prefill_f8_kernel<ND, 1, false>, groups);
     } else {
-      go(attn_prefill_f8_kernel<ND, 2, false>, groups);
+      if (cap) go(attn_prefill_f8_kernel<ND, 2, true>, cap);
+      else go(attn_prefill_f8_kernel<ND, 2, false>, groups);
     }
   };
   if (D == 32) size(std::integral_constant<int, 1>{});

@@ -222,7 +222,26 @@ def attention_decode_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tenso
                                              int(window), sink_at, scale, stream), what)
 
 
-WHOLE_TILES = 6            # tiles of 64 keys up to which a block of query rows is not cut (csrc/attention_f8.hip)
+WORTH_TILES = 12           # tiles of 64 keys that blocks of query rows have to become shorter by to be cut (csrc/attention_f8.hip)
+
+
+def _prefill_resident(device: torch.device, num_heads: int, head_dim: int) -> int:
+    """Workgroups of a head that ``attention_prefill_f8`` runs at once."""
+    return compute_units(device) * (3 if head_dim <= 64 else 2) // num_heads
+
+
+def attention_prefill_f8_plan(device: torch.device, num_heads: int, head_dim: int, blocks_of_64: int, blocks_of_128: int,
+                              max_keys: int = 0):
+    """(block_rows, groups) for ``attention_prefill_f8``; arguments as of ``attention_prefill_mfma_plan``, which it follows but where few
+    blocks have many keys each: blocks of 128 rows, cut along their keys, from 4 of them on where the longest sequence has 160
+    keys for each (head sizes up to 64: 512). us in blocks of 64 and of 128 rows, 32 heads, rows behind keys: 1,100 behind 2,000 of
+    128 113 91, 1,531 behind 1,000 97 86, 512 behind 8,000 128 109, 2,048 alone 68 72, 500 behind 3,000 (4 blocks) 62 64, 200 behind 3,000 (2)
+    38 45; 1,024 behind 4,000 of 64 80 73, 2,048 behind 8,000 231 216, 700 behind 7,000 90 87, 2,048 behind 3,000 107 113, 1,500 behind 2,500
+    73 81."""
+    t = max(1, _prefill_resident(device, num_heads, head_dim))
+    wide = 4 * blocks_of_128 >= 5 * t or (blocks_of_128 >= 4 and max_keys >= (160 if head_dim > 64 else 512) * blocks_of_128)
+    rows, blocks = (128, blocks_of_128) if wide else (64, blocks_of_64)
+    return rows, max(1, blocks if blocks <= 2 * t else t)
 
 
 def attention_prefill_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -231,8 +250,8 @@ def attention_prefill_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
                          groups: int = 0, sink: Optional[torch.Tensor] = None, tickets: Optional[torch.Tensor] = None) -> None:
     """``attention_prefill_mfma`` over an 8-bit cache (``attention_f8_fits`` says for which sizes): the work list names query blocks
     of ``block_rows`` (64 or 128) rows, those with the most keys first; ``groups`` workgroups a head share it (0: one for
-    every block). Where blocks of 64 rows have a workgroup each and fill less than half of the GPU, their keys are dealt out to as
-    many as fill it;
+    every block). Where blocks have a workgroup each and these fill less than the GPU, blocks are cut along their keys, on the device and
+    by the contexts that it finds there.
     ``tickets``: zeros that such launches on one stream may share, TICKET * blocks * query heads (else they are made)."""
     what = "attention_prefill_f8"
     stream = _launch_stream(what, out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, block_table, sink, work_seq, work_qoff,
@@ -252,9 +271,10 @@ def attention_prefill_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
         return
     groups = min(n, groups, 65535) if groups > 0 else min(n, 65535)
     cap, work, work_at, tickets_at = 0, None, None, None
-    if groups == n <= 64 and block_table.shape[1] * page_size > 64 * WHOLE_TILES:
-        resident = compute_units(q.device) * (3 if D <= 64 else 2) // Hq        # workgroups of a head that run at once
-        if 2 * n <= resident and block_rows == 64:
+    if groups == n <= 64 and block_table.shape[1] * page_size > 64 * WORTH_TILES:
+        # (blocks of 64 rows that fill more than half of it are as fast whole, of 128 rows five sixths: csrc/attention_f8.hip has the figures)
+        resident = _prefill_resident(q.device, Hq, D)
+        if 2 * n <= resident if block_rows == 64 else 6 * n <= 5 * resident:
             cap = resident
             work = torch.empty((n + cap) * Hq * block_rows * (D + 8), dtype=torch.float32, device=q.device)
             tickets = _tickets(tickets, TICKET * n * Hq, q, what)

@@ -287,7 +287,7 @@ class PagedAttention(Part):
         if n_dec == ctx.num_seqs:
             return
         keys = max(ctx.ctx_lens[n_dec:])
-        rows, groups = ops.attention_prefill_mfma_plan(
+        rows, groups = ops.attention_prefill_f8_plan(
             q.device, self.num_heads, D, ctx.work[PORTIONS_64][0].numel(), ctx.work[PORTIONS_128][0].numel(),
             min(keys, window) if window else keys)
         ops.attention_prefill_f8(out, q, *held, *tables, *ctx.work[PORTIONS_128 if rows == 128 else PORTIONS_64], self.scale, window,

@@ -41,3 +41,15 @@ def test_which_sizes_the_matrix_cores_take():
         assert not fits(torch.float32, 32, 8, D, 16) and not fits(torch.bfloat16, 32, 8, D, 8)
         assert not fits(torch.bfloat16, 32, 8, D, 24) and not fits(torch.bfloat16, 7, 2, D, 16)
     assert not fits(torch.bfloat16, 8, 8, 160, 16) and not fits(torch.bfloat16, 8, 8, 48, 16) and not fits(torch.bfloat16, 8, 0, 64, 16)
+
+
+def test_the_plan_of_prompt_portions(monkeypatch):
+    """Blocks of 128 rows where there are many, or some and many keys for each; a workgroup a block up to twice what runs at once."""
+    from pytriton_llama_amd import ops
+    from pytriton_llama_amd.ops import cache_f8
+    monkeypatch.setattr(cache_f8, "compute_units", lambda device: 256)
+    plan = lambda D, rows, keys: ops.attention_prefill_f8_plan("cuda", 32, D, -(-rows // 64), -(-rows // 128), keys)   # noqa: E731
+    assert plan(128, 2048, 2048) == (64, 32) and plan(128, 2048, 2748) == (128, 16) and plan(128, 1531, 7676) == (128, 12)
+    assert plan(128, 384, 100000) == (64, 6) and plan(128, 8192, 8192) == (128, 16)
+    assert plan(64, 2048, 5048) == (64, 32) and plan(64, 1024, 5024) == (128, 8) and plan(64, 2048, 2048) == (64, 32)
+    assert ops.attention_prefill_f8_plan("cuda", 1024, 64, 2, 1, 64) == (64, 2)

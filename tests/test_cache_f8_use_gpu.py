@@ -168,6 +168,32 @@ def test_few_blocks_are_cut_along_their_keys(ops, seqs, D, P, window):
         assert not tickets.any()
 
 
+@pytest.mark.parametrize("D,window", [(64, 0), (128, 0), (96, 900), (32, 0)])
+@pytest.mark.parametrize("seqs", CUTS + [[(300, 2000), (129, 1400), (1, 3), (2, 2)]], ids=range(len(CUTS) + 1))
+def test_few_blocks_of_128_rows_are_cut_along_their_keys(ops, seqs, D, window):
+    s = Step(torch.bfloat16, 4, 2, D, 16, seqs, window, seed=len(seqs) + D, spread=2.0).device()
+    work = s.blocks(128)
+    tickets = torch.zeros(4 * work[0].numel() * 4, dtype=torch.int32, device="cuda")
+    for _ in range(2):
+        s.out.fill_(77.0)
+        ops.attention_prefill_f8(s.out, s.qd, *s.cache, *s.tables, *work, s.scale, window, 128, tickets=tickets)
+        s.check(matrix_cores=True)
+        assert not tickets.any()
+
+
+@pytest.mark.parametrize("rows", [64, 128])
+@pytest.mark.parametrize("heads", [16, 32])
+def test_blocks_share_few_workgroups(ops, heads, rows):
+    """So many heads that the workgroups of one are few: each has ends of blocks and several blocks, short ones and one without
+    keys among them."""
+    seqs = [(30, 900), (200, 1000), (1, 0), (1, 1300), (65, 65), (1, 1)]
+    s = Step(torch.bfloat16, heads, 1, 32, 16, seqs, 0, seed=heads, spread=2.0).device()
+    work = s.blocks(rows)
+    assert 2 * work[0].numel() <= ops.compute_units(s.qd.device) * 3 // heads
+    ops.attention_prefill_f8(s.out, s.qd, *s.cache, *s.tables, *work, s.scale, 0, rows)
+    s.check(matrix_cores=True)
+
+
 def test_rows_without_keys_and_without_a_sink_of_their_own(ops):
     """A sink of -inf is no sink: rows without keys are zeros, the others what they are without."""
     s = Step(torch.bfloat16, 4, 2, 64, 16, [(1, 0), (1, 40), (1, 0)], 0, seed=3).device()
