@@ -599,7 +599,7 @@ extern "C" int ptl_attention_decode_f8(void* out, long out_stride, const void* q
 // workgroup has a part of a block, blocks as a whole, and a part of one. It writes the sums of parts to the workspace as its lanes
 // hold them and, its tiles done, counts them; who is last of a block's merges them. (A part costs some 8 us, ten tiles: the writes' way
 // to memory, the count, and each part's way back, which is hidden behind the addition of the one before.) us, not cut and
-// cut, 32 heads, rows behind keys: blocks of 64 rows 200 behind 3,000 of 128 67.7 38.4, 512 behind 8,000 of 128 178 128, 512 behind 1,024
+// cut, 32 heads, rows behind keys: blocks of 64 rows 200 behind 3,000 of 128 67.7 37.4, 512 behind 8,000 of 128 178 122, 512 behind 1,024
 // of 64 23.4 22.4, but 700 of 128 (11 blocks, 16 workgroups) 19.7 21.4, 1,500 behind 500 of 64 (24, 24) 34.2 42.5; of 128 rows 512 behind
 // 8,000 of 128 250 109, 1,100 behind 6,000 (9, 16) 253 180, 1,531 behind 6,145 (12, 16) 279 243, 1,600 behind 6,000 (13) 272 255, 1,700 (14)
 // 278 277, 2,048 behind 2,048 (16) 141 163; 1,000 behind 8,000 of 64 (8, 24) 183 114.
@@ -628,8 +628,15 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
   constexpr bool STAGED = RT == 2 && D % 64 == 0;
   __shared__ __attribute__((aligned(16))) bf16_t Ks[2][BN * D], Vs[2][BN * D];
   __shared__ __attribute__((aligned(16))) uint8_t staged[STAGED ? 4 : 1][2][STAGED ? 16 * D : 16];
-  // piece c of row r lies at c ^ swz(r), so that neither product's reads meet in a bank
+  // Piece c of row r lies at c ^ swz(r), so that what 64 lanes read at once lies in different banks: of keys a piece of 16 rows (in fours,
+  // beside the next piece of other fours), of values two pieces of 8 rows. A row of 128 goes over all banks: keys need 16 places
+  // there, values 8 for pairs. That takes twelve more registers for addresses, which two row tiles do not have: they share
+  // r & 7, and a third of LDS's cycles are conflicts (made anew for every tile addresses cost more than that, 245 us where these take
+  // 242; one row tile: 1,531 rows behind 6,145 keys, 32 heads, 312 with r & 7, 300 so).
+  constexpr bool WIDE = D == 128 && RT == 1;
   auto swz = [](int r) { return PIECES % 8 == 0 ? (r & 7) : ((r >> 1) & 3); };
+  auto key_swz = [&](int r) { return WIDE ? r & 15 : swz(r); };
+  auto value_swz = [&](int r) { return WIDE ? 2 * (r & 7) : swz(r); };
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 15, lg = lane >> 4;
   // heads run along x, which the eight dies take in turn: die c gets heads c Hq / 8 .. of which a kv head's lie together
@@ -644,24 +651,27 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
   const float lazy = 8.0f / scale_log2;             // (raw scores: the maximum follows only where they pass it by 2^8)
   // Wave w brings rows 16 w .. +15 of a tile: 16 D bytes side by side in one page, lane l the 8 codes from 512 i + 8 l on of them
   // (addresses that differ from another one by a constant are that one and the constant: registers are short at D = 128)
-  constexpr int STORES = D == 128 ? 2 : D == 64 ? 1 : ND;     // of D = 128 and 64: every 8 rows the same piece lies in the same place
-  int plds[STORES];
+  constexpr int VALUE_STORES = D == 128 ? 2 : D == 64 ? 1 : ND;      // of D = 128 and 64: every 8 rows the same piece lies in the same place
+  constexpr int KEY_STORES = WIDE ? ND : VALUE_STORES;
+  int key_to[KEY_STORES], value_to[VALUE_STORES];
 #pragma unroll
-  for (int i = 0; i < STORES; ++i) {
+  for (int i = 0; i < KEY_STORES; ++i) {
     const int r = (64 * i + lane) / PIECES, c = 64 * i + lane - r * PIECES;
-    plds[i] = (16 * wave + r) * D + (c ^ swz(r)) * 8;
+    key_to[i] = (16 * wave + r) * D + (c ^ key_swz(r)) * 8;
+    if (i < VALUE_STORES) value_to[i] = (16 * wave + r) * D + (c ^ value_swz(r)) * 8;
   }
-  auto store_at = [&](int i) { return plds[i % STORES] + i / STORES * 8 * D; };
+  auto key_store_at = [&](int i) { return key_to[i % KEY_STORES] + i / KEY_STORES * 8 * D; };
+  auto value_store_at = [&](int i) { return value_to[i % VALUE_STORES] + i / VALUE_STORES * 8 * D; };
   // where this lane reads: the first product takes row 16 kt + ln, piece 4 kk + lg; the second points at row
   // 32 half + 16 j + 4 lg + ln / 4, elements 16 dt + 4 (ln % 4) .. +3
-  constexpr int SWAPPED = PIECES % 8 == 0 ? 8 : 4;            // pieces change places within so many
+  constexpr int SWAPPED = WIDE ? 16 : PIECES % 8 == 0 ? 8 : 4;       // pieces change places within so many
   int k_at[SWAPPED / 4], v_at[SWAPPED / 2];
 #pragma unroll
-  for (int kk = 0; kk < SWAPPED / 4; ++kk) k_at[kk] = ln * D + 8 * ((4 * kk + lg) ^ swz(ln));
+  for (int kk = 0; kk < SWAPPED / 4; ++kk) k_at[kk] = ln * D + 8 * ((4 * kk + lg) ^ key_swz(ln));
   {
     const int r = 4 * lg + (ln >> 2);
 #pragma unroll
-    for (int dt = 0; dt < SWAPPED / 2; ++dt) v_at[dt] = r * D + 8 * ((2 * dt + ((ln & 3) >> 1)) ^ swz(r)) + 4 * (ln & 1);
+    for (int dt = 0; dt < SWAPPED / 2; ++dt) v_at[dt] = r * D + 8 * ((2 * dt + ((ln & 3) >> 1)) ^ value_swz(r)) + 4 * (ln & 1);
   }
   auto key_at = [&](int kk) { return k_at[kk % (SWAPPED / 4)] + kk / (SWAPPED / 4) * 8 * SWAPPED; };
   auto value_at = [&](int dt) { return v_at[dt % (SWAPPED / 2)] + dt / (SWAPPED / 2) * 8 * SWAPPED; };
@@ -827,8 +837,8 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
       }
 #pragma unroll
       for (int i = 0; i < ND; ++i) {
-        *reinterpret_cast<bf16x8_t*>(Kb + store_at(i)) = eight_bf16(kc[i].x, kc[i].y, ks);
-        *reinterpret_cast<bf16x8_t*>(Vb + store_at(i)) = eight_bf16(vc[i].x, vc[i].y, vs);
+        *reinterpret_cast<bf16x8_t*>(Kb + key_store_at(i)) = eight_bf16(kc[i].x, kc[i].y, ks);
+        *reinterpret_cast<bf16x8_t*>(Vb + value_store_at(i)) = eight_bf16(vc[i].x, vc[i].y, vs);
       }
       // what was read is in registers: the next tile's codes may come to its place (free here: the products read none of it)
       if constexpr (STAGED) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

@@ -235,7 +235,7 @@ def attention_prefill_f8_plan(device: torch.device, num_heads: int, head_dim: in
     """(block_rows, groups) for ``attention_prefill_f8``; arguments as of ``attention_prefill_mfma_plan``, which it follows but where few
     blocks have many keys each: blocks of 128 rows, cut along their keys, from 4 of them on where the longest sequence has 160
     keys for each (head sizes up to 64: 512). us in blocks of 64 and of 128 rows, 32 heads, rows behind keys: 1,100 behind 2,000 of
-    128 113 91, 1,531 behind 1,000 97 86, 512 behind 8,000 128 109, 2,048 alone 68 72, 500 behind 3,000 (4 blocks) 62 64, 200 behind 3,000 (2)
+    128 113 91, 1,531 behind 1,000 97 86, 512 behind 8,000 122 109, 2,048 alone 65 72, 500 behind 3,000 (4 blocks) 62 64, 200 behind 3,000 (2)
     38 45; 1,024 behind 4,000 of 64 80 73, 2,048 behind 8,000 231 216, 700 behind 7,000 90 87, 2,048 behind 3,000 107 113, 1,500 behind 2,500
     73 81."""
     t = max(1, _prefill_resident(device, num_heads, head_dim))
