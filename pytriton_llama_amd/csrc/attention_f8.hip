@@ -187,16 +187,24 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return
 // ===========================================================================
 // ptl_attention_decode_f8: the sequences of a step that bring one token each.
 //
-// The keys of a (sequence, kv head) pair are cut into parts of ``piece`` units of 128 keys, the same piece for all sequences: as
+// The keys of a (sequence, kv head) pair are cut into parts of ``piece`` units, the same piece for all sequences: as
 // long as makes some ``cap`` parts of all of them, a workgroup a compute unit. (Sum of ceil(n_s / piece) <= cap + sequences, which
 // the launch has room for.) Every workgroup finds the piece and its own part from the context lengths on the device, so a
 // recorded launch suits whatever contexts it is replayed with. A pair's parts are merged by the workgroup that is done last
-// (a ticket), in the order of the keys. More and smaller parts hide more latency, fewer meet sooner and leave no
-// second round: us with one, two and three workgroups a compute unit, 8 kv heads: 1 x 8,000 keys of 64 10.6 12.7 12.6, 8 x 2,048 of 64
-// 12.7 12.1 12.5, 64 x 61 to 2,610 of 64 25.4 26.8 26.6; 4 x 3,000 of 128 13.7 15.0 16.0, 8 x 5,000 to 7,000 of 128 27.3 26.2 29.0,
-// 20 x 130 to 2,900 of 128 23.5 21.6 22.0, 2 x 120,000 of 128 95.8 95.5 98.4.
+// (a ticket), in the order of the keys. Two parts a compute unit: 8 x 2,048 keys of 64, 8 kv heads, 10.5 us instead of 11.1, but 64 x 61 to
+// 2,610 of 64 27 instead of 22, 8 x 5,000 to 7,000 of 128 31 instead of 25.
 //
-// A workgroup has four waves, which take tiles of 32 keys in turn. Both products are transposed, as in attention_decode.h:
+// A workgroup has eight waves, which take tiles of 32 keys in turn (a unit: 256), as long as there are no more pairs than the GPU runs such
+// workgroups at once, two a compute unit up to D = 64, else one: what waves share in LDS need not go through memory. More pairs, then
+// most of them not cut, have workgroups of four waves (a unit: 128), of which three or four run where one of eight does. us with four and
+// eight: 1 x 300 of 64 5.6 5.2, 8 x 2,048 12.2 11.1, 16 x 1,000 12.9 8.6, 64 x 61 to 2,610 24.9 22.1, 128 x 300 to 1,000 21.5 22.9; 4 x 3,000
+// of 128 14.2 13.4, 8 x 5,000 to 7,000 26.1 24.7, 32 x 100 to 5,000 61.7 47.4, 64 x 100 to 1,000 21.2 24.9. (Sixteen waves: 16 x 1,000 of
+// 64 8.2, 8 x 2,048 11.2, 64 x 61 to 2,610 25.)
+//
+// What bounds it: 2 x 120,000 keys of 128 take 89 us, 5.5 TB/s of codes (a copy of as many bytes reaches 4.8 both ways). Few keys: a
+// chain of the context lengths, the table, the codes, and for a pair in parts of their way to memory and back, some 3 us.
+//
+// Both products are transposed, as in attention_decode.h:
 //   S^T[key, head] = K . Q^T        A = K: lane (ln, lg) has key ln's k-values, straight from memory
 //   O^T[d, head]  += V^T . P^T      B = P^T: what a lane has of S^T; A = V^T[d, key]
 // For the second a lane needs one d of the 8 keys that its P^T values belong to. It loads D / 16 neighbouring elements of each of those
@@ -207,22 +215,21 @@ struct DecodeF8Parts {
   int* tickets;                    // [sequence][kv head][head tile][TICKET]
 };
 
-constexpr int UNIT_F8 = 128;       // keys of a workgroup's turn
 constexpr int MOST_PARTS_F8 = 128; // parts of a pair
 constexpr int WHOLE_F8 = 4;        // units up to which a pair is not cut: a turn is some 0.8 us, parts that meet cost 3
 
-template <int A, int B>
-__global__ void __launch_bounds__(256, A + B <= 1 ? 4 : 3)
+template <int A, int B, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, A + B <= 1 ? 4 : 3)
 attn_decode_f8_kernel(const int32_t* __restrict__ ctx_len, const int32_t* __restrict__ block_table, const uint8_t* __restrict__ k_cache,
                       const uint8_t* __restrict__ v_cache, int n_seq, int Hkv, int cap, int bt_stride, int page_shift,
                       const bf16_t* __restrict__ q, long q_stride, const float* __restrict__ k_scale,
                       const float* __restrict__ v_scale, int Hq, bf16_t* __restrict__ out, long out_stride,
                       const int32_t* __restrict__ q_start, DecodeF8Parts parts, int window, const float* __restrict__ sink,
                       float scale_log2) {
-  constexpr int D = 64 * A + 32 * B, NT = D / 16, STEPS = D / 32;
+  constexpr int D = 64 * A + 32 * B, NT = D / 16, STEPS = D / 32, UNIT_F8 = 32 * WAVES, THREADS = 64 * WAVES;
   constexpr int REGION = D == 32 ? 608 : 16 * D + 32;         // floats of a wave's sums
   static_assert(4 * REGION >= MOST_PARTS_F8 * 16 + 192 * 2, "the merge's weights and sums lie there too");
-  __shared__ __attribute__((aligned(16))) float regions[4][REGION];
+  __shared__ __attribute__((aligned(16))) float regions[WAVES][REGION];
   __shared__ int last;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 15, lg = lane >> 4;
@@ -462,14 +469,14 @@ attn_decode_f8_kernel(const int32_t* __restrict__ ctx_len, const int32_t* __rest
     out[(size_t)row * out_stride + (size_t)head * D + d] = float_to_bf16(l == 0.f ? 0.f : a / l);       // (no keys: zeros)
   };
   const size_t group = ((size_t)u * Hkv + kvh) * G + 16 * tile;             // this part's first head
-  for (int i = threadIdx.x; i < GT * D; i += 256) {
+  for (int i = threadIdx.x; i < GT * D; i += THREADS) {
     const int h = i / D, d = i - h * D;
     float m = -INFINITY, l = 0.f, a = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) m = fmaxf(m, regions[w][16 * D + 2 * h]);
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, regions[w][16 * D + 2 * h]);
     const float to = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const float f = __builtin_amdgcn_exp2f(regions[w][16 * D + 2 * h] - to);
       l = fmaf(regions[w][16 * D + 2 * h + 1], f, l);
       a = fmaf(regions[w][h * D + d], f, a);
@@ -486,7 +493,7 @@ attn_decode_f8_kernel(const int32_t* __restrict__ ctx_len, const int32_t* __rest
   __syncthreads();
   if (threadIdx.x == 0) last = last_part(parts.tickets + (((size_t)seq * Hkv + kvh) * tiles + tile) * TICKET, n_parts);
   __syncthreads();
-  if (!last) return;
+  if (!last || threadIdx.x >= 256) return;
   // ---- the last workgroup of the pair merges its parts ----
   // A thread takes two columns of AHEAD parts at a time; where that leaves threads, two or four groups of them share the parts.
   // What they read first is on its way while the parts' weights are made (parts that are none weigh nothing): a part
@@ -574,14 +581,22 @@ extern "C" int ptl_attention_decode_f8(void* out, long out_stride, const void* q
   int shift = 0;
   while (1 << shift < page_size) ++shift;
   const DecodeF8Parts parts{acc, ml, tickets};
-  auto go = [&](auto kernel) {
-    kernel<<<grid, 256, 0, stream>>>(ctx_len, block_table, k, v, n_seq, Hkv, cap, bt_stride, shift, (const bf16_t*)q, q_stride, k_scale,
-                                     v_scale, Hq, (bf16_t*)out, out_stride, q_start, parts, window, sink, scale * 1.4426950408889634f);
+  auto go = [&](auto kernel, int threads) {
+    kernel<<<grid, threads, 0, stream>>>(ctx_len, block_table, k, v, n_seq, Hkv, cap, bt_stride, shift, (const bf16_t*)q, q_stride, k_scale,
+                                         v_scale, Hq, (bf16_t*)out, out_stride, q_start, parts, window, sink, scale * 1.4426950408889634f);
   };
-  if (D == 32) go(attn_decode_f8_kernel<0, 1>);
-  else if (D == 64) go(attn_decode_f8_kernel<1, 0>);
-  else if (D == 96) go(attn_decode_f8_kernel<1, 1>);
-  else go(attn_decode_f8_kernel<2, 0>);
+  const bool eight = (long)n_seq * Hkv * grid.y <= (long)compute_units() * (D <= 64 ? 2 : 1);
+  auto size = [&](auto a, auto b) {
+    constexpr int A = decltype(a)::value, B = decltype(b)::value;
+    if (eight) go(attn_decode_f8_kernel<A, B, 8>, 512);
+    else go(attn_decode_f8_kernel<A, B, 4>, 256);
+  };
+  constexpr std::integral_constant<int, 0> none{};
+  constexpr std::integral_constant<int, 1> one{};
+  if (D == 32) size(none, one);
+  else if (D == 64) size(one, none);
+  else if (D == 96) size(one, one);
+  else size(std::integral_constant<int, 2>{}, none);
   return ptl_launch_status();
 }
 

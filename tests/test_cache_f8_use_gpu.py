@@ -152,6 +152,21 @@ def test_recorded_prompt_portions(ops, rows):
         s.check(matrix_cores=True)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,window", [(16, 8, 64, 0), (16, 8, 128, 0), (16, 8, 96, 100), (16, 8, 32, 0)])
+@pytest.mark.parametrize("n", [31, 33, 64, 66])
+def test_decode_with_workgroups_of_four_and_of_eight_waves(ops, Hq, Hkv, D, window, n):
+    """Around the numbers of pairs where the launch changes from one to the other (256 and 512 on a GPU of 256 compute units), with
+    contexts around the ends of both's turns and one that is cut."""
+    contexts = [(0, 1, 31, 32, 33, 127, 128, 129, 255, 256, 257, 511, 513)[i % 13] for i in range(n - 1)] + [1500]
+    s = Step(torch.bfloat16, Hq, Hkv, D, 16, [(1, c) for c in contexts], window, seed=n + D, spread=2.0).device()
+    tickets = torch.zeros(4 * n * Hkv, dtype=torch.int32, device="cuda")
+    for _ in range(2):
+        s.out.fill_(77.0)
+        ops.attention_decode_f8(s.out, s.qd, *s.cache, *s.tables, n, s.scale, window, tickets=tickets)
+        s.check(matrix_cores=True)
+        assert not tickets.any()
+
+
 CUTS = [[(64, 5000)], [(1, 3000), (63, 2999), (65, 1100)], [(200, 3000)], [(64, 64), (64, 900), (17, 1500), (3, 385), (5, 384)]]
 
 
