@@ -55,7 +55,10 @@ def parse_ids(s: str) -> List[int]:
 
 
 def main(argv: Optional[List[str]] = None) -> int:
-    args = build_parser().parse_args(argv)
+    parser = build_parser()
+    args = parser.parse_args(argv)
+    if args.samples < 1:
+        parser.error(f"--samples: one completion at least, got {args.samples}")
     from .generate import GenerateStreamText
 
     folder = args.checkpoints_dir

@@ -200,6 +200,8 @@ class Engine:
             raise ValueError("one SamplingParams for every branch, or one for all")
         if any(p.max_new_tokens <= n for p in params):
             raise ValueError(f"a branch that starts with {n} tokens of output needs max_new_tokens beyond that")
+        if n and any(p.logprobs and not req.params.logprobs for p in params):
+            raise ValueError(f"request {request_id!r} has no log-probabilities of the {n} tokens its branch starts with")
         branches = []
         for p in params:
             b = Request(self._new_id(), req.prompt_array, p, req.output[:n], req.output_logprobs[:n])

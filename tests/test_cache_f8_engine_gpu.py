@@ -202,6 +202,30 @@ def test_branches_while_generating(folders, cache_dtype, graphs):
     assert e.runner.manager.paged[0].pool.num_free == 24
 
 
+def test_log_probabilities_of_branches(folders):
+    """One a token, those of the tokens they share as well; not where the request did not keep them."""
+    import dataclasses
+    from pytriton_llama_amd.engine import SamplingParams
+    e = engine(folders["C"], cache_dtype="float8_e4m3fn", seqs=4, pages=40)
+    prompt = random_sequences(300, [19], seed=4)["r0"]
+    keeps = SamplingParams(temperature=0.0, max_new_tokens=9, ignore_eos=True, logprobs=True)
+    drops = dataclasses.replace(keeps, logprobs=False)
+    a, b = e.add_request(prompt, keeps), e.add_request(prompt, drops)
+    for _ in range(4):
+        e.step()
+    n = len(e.requests[a].output)
+    assert n > 2
+    made = e.fork(a) + e.fork(b, keeps, num_output=0)
+    with pytest.raises(ValueError):
+        e.fork(b, keeps)
+    reqs = {r: e.requests[r] for r in [a, b] + made}
+    assert reqs[made[0]].output_logprobs == reqs[a].output_logprobs
+    while e.has_work:
+        e.step()
+    assert [len(reqs[r].output_logprobs) for r in [a, b] + made] == [9, 0, 9, 9]
+    assert reqs[made[0]].output == reqs[a].output == reqs[made[1]].output
+
+
 def test_branches_are_preempted_like_others(folders):
     """Few pages: branches give way and are computed again; shared pages stay with who holds them."""
     from pytriton_llama_amd.engine import SamplingParams

@@ -203,3 +203,11 @@ def test_other_models_refuse(module):
     model = build_model(next(iter(table.values()))[0])
     with pytest.raises(ValueError, match="engine's type only"):
         model.cache_layers_in(F8)
+
+
+@pytest.mark.parametrize("samples", ["0", "-2"])
+def test_the_command_line_refuses_no_samples(samples, capsys):
+    from pytriton_llama_amd import cli
+    with pytest.raises(SystemExit):
+        cli.main(["--checkpoints_dir", "nowhere", "--samples", samples])
+    assert "--samples" in capsys.readouterr().err
