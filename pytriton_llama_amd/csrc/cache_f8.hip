@@ -8,6 +8,7 @@
 // stored as NaN and takes no part in the scale.
 #include "common.h"
 #include "device.h"
+#include <type_traits>
 
 // 2^e for -126 <= e <= 127
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
@@ -37,7 +38,8 @@ __device__ __forceinline__ uint32_t two_codes(float a, float b) {
 // The first workgroups store, a wave a task (row that begins a run, kv head, keys or values): a block belongs to one wave and no two
 // waves write one scale. Up to DIRECT rows every row has its tasks, and the waves of rows that begin nothing leave. Beyond, a
 // workgroup makes the list of the rows that begin a run (of LISTED rows at a time) and its waves take their share of the
-// tasks; with a workgroup for every row 2,048 rows, 8 kv heads of 128, took 71 us, from lists they take 17.6.
+// tasks; with a workgroup for every row 2,048 rows, 8 kv heads of 128, took 71 us, from lists they took 17.6, and where the four tasks of a
+// workgroup are of one run, whose angles they make together, they take 15.1.
 // A wave takes the rows of its run a chunk at a time, holds their numbers of a head and finds the largest; a run of one chunk (16 rows
 // of 128) is then written from the registers, a longer one read and rotated again. Behind them the workgroups that rotate the queries, a
 // row a wave.
@@ -60,8 +62,9 @@ struct RowFactor {
   }
 };
 
-// The run that begins at row t0, if one does: its keys or values of head h. A wave's work, or (TEAM) that of the workgroup's four.
-template <typename T, int VEC, bool TEAM, bool SCALED>
+// The run that begins at row t0, if one does: its keys or values of head h. A wave's work, or (TEAM) that of the workgroup's four. SHARED: the
+// workgroup's waves are at the same run, of one chunk, and make its angles together.
+template <typename T, int VEC, bool TEAM, bool SHARED, bool SCALED>
 __device__ __forceinline__ void
 store_run(int t0, int h, bool values, int lane, int wave, float2* __restrict__ table, float* __restrict__ largest_of_wave, const T* __restrict__ k, const T* __restrict__ v,
           long row_stride, const int32_t* __restrict__ positions, const float* __restrict__ inv_freq,
@@ -97,6 +100,15 @@ store_run(int t0, int h, bool values, int lane, int wave, float2* __restrict__ t
   uint8_t* const rows = (values ? v_cache : k_cache) + ((size_t)page * Hkv + h) * page_size * D;
   const float old = off > 0 ? *scale : 0.f;
 
+  auto meet = [] {
+    if constexpr (SHARED) {
+      __syncthreads();
+    } else {                                                      // (a wave's own LDS)
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+  };
   // rows r0 .. of the run, as many as a chunk has: a and b hold item lane + 64 it of them, VEC pairs of one row
   auto load = [&](int r0, float (&a)[HELD][VEC], float (&b)[HELD][VEC]) __attribute__((always_inline)) {
     const int count = min(chunk, n - r0), items = count * per_row;
@@ -114,19 +126,17 @@ store_run(int t0, int h, bool values, int lane, int wave, float2* __restrict__ t
         if (lane == 0) row_factor[r] = f;
       }
     }
-    if (turn) {
+    if (SHARED ? inv_freq != nullptr : turn) {
       // the angles' cosines and sines once for the chunk, an angle a lane (sincosf is some hundred instructions: in the loop below
       // they would be 16 times as many, and a launch that has one row a wave is the time of fetching them)
-      for (int i = lane; i < count * half; i += 64) {
+      for (int i = SHARED ? threadIdx.x : lane; i < count * half; i += SHARED ? 256 : 64) {
         const int r = i / half;
         float s, c;
         sincosf((float)positions[t0 + r0 + r] * inv_freq[i - r * half], &s, &c);
         table[i] = make_float2(c, s);
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");        // (the wave's own LDS: written above, read below)
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    meet();                                                       // (LDS: written above, read below)
 #pragma unroll
     for (int it = 0; it < HELD; ++it) {
       const int i = min(lane + 64 * it, items - 1);
@@ -142,9 +152,7 @@ store_run(int t0, int h, bool values, int lane, int wave, float2* __restrict__ t
         b[it][e] = turn ? x2 * cs.x + x1 * cs.y : x2;
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    meet();
     return items;
   };
   auto largest_of = [&](const float (&a)[VEC], float m) {
@@ -293,7 +301,7 @@ rope_store_f8_kernel(T* __restrict__ q_out, const T* __restrict__ q, const T* __
   if (T_ <= DIRECT) {
     const int task = blockIdx.x * 4 + wave, t = task / (2 * Hkv), rest = task - t * 2 * Hkv;
     if (t < T_)
-      store_run<T, VEC, false, SCALED>(t, rest >> 1, rest & 1, lane, wave, tables[wave], nullptr, k, v, row_stride, positions, inv_freq, slots,
+      store_run<T, VEC, false, false, SCALED>(t, rest >> 1, rest & 1, lane, wave, tables[wave], nullptr, k, v, row_stride, positions, inv_freq, slots,
                                k_cache, v_cache, k_scale, v_scale, T_, Hkv, D, page_size, slots_in_all, factor, row_factors[wave]);
     return;
   }
@@ -338,13 +346,18 @@ rope_store_f8_kernel(T* __restrict__ q_out, const T* __restrict__ q, const T* __
       total = __builtin_amdgcn_readfirstlane(total) * 2 * Hkv;
       for (; next < total; next += step) {
         const int run = next / (2 * Hkv), task = next - run * 2 * Hkv, t0 = seg + __builtin_amdgcn_readfirstlane((int)list[run]);
+        auto store = [&](auto together, auto same_run, float2* table) __attribute__((always_inline)) {
+          store_run<T, VEC, decltype(together)::value, decltype(same_run)::value, SCALED>(
+              t0, task >> 1, task & 1, lane, wave, table, largest_of_wave, k, v, row_stride, positions, inv_freq, slots, k_cache, v_cache,
+              k_scale, v_scale, T_, Hkv, D, page_size, slots_in_all, factor, row_factors[wave]);
+        };
         if (team) {
-          store_run<T, VEC, true, SCALED>(t0, task >> 1, task & 1, lane, wave, tables[wave], largest_of_wave, k, v, row_stride, positions, inv_freq,
-                                  slots, k_cache, v_cache, k_scale, v_scale, T_, Hkv, D, page_size, slots_in_all, factor, row_factors[wave]);
+          store(std::true_type{}, std::false_type{}, tables[wave]);
           __syncthreads();                            // (the waves' largest numbers have been read)
+        } else if (Hkv % 2 == 0) {                    // four tasks, of one run
+          store(std::false_type{}, std::true_type{}, tables[0]);
         } else {
-          store_run<T, VEC, false, SCALED>(t0, task >> 1, task & 1, lane, wave, tables[wave], nullptr, k, v, row_stride, positions, inv_freq, slots,
-                                   k_cache, v_cache, k_scale, v_scale, T_, Hkv, D, page_size, slots_in_all, factor, row_factors[wave]);
+          store(std::false_type{}, std::false_type{}, tables[wave]);
         }
       }
       next -= total;

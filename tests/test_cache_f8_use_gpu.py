@@ -273,6 +273,43 @@ def test_pages_that_sequences_share(ops):
         assert torch.equal(out[i], oi[0])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("Hq,Hkv,D,P", [(4, 2, 64, 16), (8, 8, 128, 16), (3, 3, 64, 16), (2, 1, 96, 16), (4, 2, 34, 7), (6, 2, 128, 32), (2, 1, 64, 64)])
+@pytest.mark.parametrize("lengths", [[129], [1, 1, 200, 1], [700, 1, 1, 1598], [1] * 150 + [2000]], ids=["129", "203", "2300", "2150"])
+def test_a_call_of_many_rows_stores_what_calls_of_a_page_store(ops, dtype, Hq, Hkv, D, P, lengths):
+    """Sequences that begin inside of pages, some rows that are not stored among them: one call, and a call for every page."""
+    g = torch.Generator().manual_seed(D + len(lengths))
+    slots, pages, pieces = [], 0, []
+    order = torch.randperm(sum(n // P + 2 for n in lengths), generator=g).tolist()
+    for i, n in enumerate(lengths):
+        off = (5 * i) % P if n > 1 else 3 % P                # (what lies before: an earlier step's)
+        at = 0
+        while at < n:
+            take = min(P - off, n - at)
+            pieces.append((len(slots), take))
+            slots += [order[pages] * P + off + j for j in range(take)]
+            pages, at, off = pages + 1, at + take, 0
+        slots += [-1] * (i % 3)
+    T, total = len(slots), len(order)
+    x = (torch.randn(T, (Hq + 2 * Hkv) * D, generator=g) * torch.exp(2 * torch.randn(T, 1, generator=g))).to(dtype).cuda()
+    q, k, v = (x[:, a * D:b * D].view(T, b - a, D) for a, b in ((0, Hq), (Hq, Hq + Hkv), (Hq + Hkv, Hq + 2 * Hkv)))
+    positions, sd = i32([(7 * t) % 4001 for t in range(T)]), i32(slots)
+    inv_freq = (500000.0 ** (-torch.arange(0, D, 2) / D)).cuda()
+    codes = torch.randint(0, 127, (2, total, Hkv, P, D), generator=g, dtype=torch.uint8)
+    scales = 2.0 ** torch.randint(-9, 3, (2, total, Hkv), generator=g)
+    caches = [[codes[0].cuda().view(F8), codes[1].cuda().view(F8), scales[0].cuda(), scales[1].cuda()] for _ in range(2)]
+    for _ in range(2):
+        got = ops.rope_store_f8(q, k, v, positions, inv_freq, sd, *caches[0])
+    want = torch.empty_like(got)
+    for first, n in pieces:
+        s = slice(first, first + n)
+        want[s] = ops.rope_store_f8(q[s], k[s], v[s], positions[s], inv_freq, sd[s], *caches[1])
+    stored = (sd >= 0).cpu()
+    assert torch.equal(got.cpu()[stored], want.cpu()[stored])
+    for a, b in zip(bits(caches[0]), bits(caches[1])):
+        assert torch.equal(a, b)
+
+
 def test_offsets_that_pass_32_bits(ops):
     """Pools of 4.5 GiB, of which the last pages are used."""
     Hq, Hkv, D, P = 8, 8, 128, 16
