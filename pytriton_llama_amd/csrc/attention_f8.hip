@@ -201,7 +201,8 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return
 // of 128 14.2 13.4, 8 x 5,000 to 7,000 26.1 24.7, 32 x 100 to 5,000 61.7 47.4, 64 x 100 to 1,000 21.2 24.9. (Sixteen waves: 16 x 1,000 of
 // 64 8.2, 8 x 2,048 11.2, 64 x 61 to 2,610 25.)
 //
-// What bounds it: 2 x 120,000 keys of 128 take 89 us, 5.5 TB/s of codes (a copy of as many bytes reaches 4.8 both ways). Few keys: a
+// What bounds it: 2 x 120,000 keys of 128 take 89 us, 5.5 TB/s of codes in pieces of 2 KB (a copy reaches 4.8 both ways, a
+// plain stream of reads 7.1; three or four tiles a wave on their way instead of two change nothing: 89.7, 90.3). Few keys: a
 // chain of the context lengths, the table, the codes, and for a pair in parts of their way to memory and back, some 3 us.
 //
 // Both products are transposed, as in attention_decode.h:
