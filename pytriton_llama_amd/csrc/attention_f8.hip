@@ -247,12 +247,12 @@ attn_decode_f8_kernel(const int32_t* __restrict__ ctx_len, const int32_t* __rest
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
   // (a sequence's last part is half a piece on average, so that many fewer whole ones fit ``cap`` parts)
-  const int whole = max(cap - n_seq / 2, (3 * cap + 3) / 4);
+  const int whole = max(max(cap - n_seq / 2, (3 * cap + 3) / 4), 1);
   const int piece = __builtin_amdgcn_readfirstlane(max(1, (total + whole - 1) / whole));
   int seq = -1, split = 0, n_parts = 0, before = 0;
   for (int s0 = 0; s0 < n_seq && seq < 0; s0 += 64) {
     const int units = s0 + lane < n_seq ? units_of(s0 + lane) : 0;
-    const int mine = s0 + lane < n_seq ? (units <= WHOLE_F8 ? 1 : (units + piece - 1) / piece) : 0;
+    const int mine = s0 + lane < n_seq ? (units <= WHOLE_F8 || !cap ? 1 : (units + piece - 1) / piece) : 0;
     int upto = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -567,14 +567,15 @@ static bool f8_matrix_sizes(int Hq, int Hkv, int D, int page_size) {
          (page_size & (page_size - 1)) == 0 && (long)Hkv * D * page_size < 1l << 31;
 }
 
+// cap 0: no pair is cut (then there is no workspace)
 extern "C" int ptl_attention_decode_f8(void* out, long out_stride, const void* q, long q_stride, const uint8_t* k, const uint8_t* v,
                                        const float* k_scale, const float* v_scale, const int32_t* q_start, const int32_t* ctx_len,
                                        const int32_t* block_table, int bt_stride, float* acc, float* ml, int* tickets, int cap,
                                        int n_seq, int Hq, int Hkv, int D, int page_size, int window, const float* sink, float scale,
                                        hipStream_t stream) {
   if (n_seq <= 0) return PTL_OK;
-  if (!f8_matrix_sizes(Hq, Hkv, D, page_size) || cap <= 0 || cap > MOST_PARTS_F8 || n_seq >= 1 << 24 || window < 0 || !acc || !ml || !tickets ||
-      ((uintptr_t)ml % 8) || ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 || q_stride % 8)
+  if (!f8_matrix_sizes(Hq, Hkv, D, page_size) || cap < 0 || cap > MOST_PARTS_F8 || n_seq >= 1 << 24 || window < 0 ||
+      (cap && (!acc || !ml || !tickets || (uintptr_t)ml % 8)) || ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) % 16 || q_stride % 8)
     return PTL_ERR_ARG;
   const long groups = (long)(n_seq + cap) * Hkv;
   if (groups >= 1l << 31) return PTL_ERR_ARG;

@@ -192,6 +192,7 @@ def attention_f8_fits(dtype: torch.dtype, num_heads: int, num_kv_heads: int, hea
 
 
 MOST_PARTS_F8 = 128        # parts of a (sequence, kv head) pair (csrc/attention_f8.hip)
+WHOLE_KEYS_F8 = 512        # keys of a pair that is never cut
 
 
 def attention_decode_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -208,18 +209,23 @@ def attention_decode_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tenso
     if unaligned[0] or not attention_f8_fits(q.dtype, Hq, Hkv, D, page_size):
         raise KernelError(f"{what}: needs bfloat16, a head size of 32/64/96/128, a page size from 16 on that is a power of two, "
                           "aligned q rows")
-    if not 0 <= n_seq <= ctx_len.numel():
-        raise KernelError(f"{what}: tables are shorter than n_seq")
+    if not 0 <= n_seq <= ctx_len.numel() or n_seq > q.shape[0]:
+        raise KernelError(f"{what}: tables, or q, are shorter than n_seq")
     if n_seq == 0:
         return
-    tiles = -(-(Hq // Hkv) // 16)
-    cap = max(1, min(MOST_PARTS_F8, compute_units(q.device) // (Hkv * tiles)))         # a workgroup a compute unit
-    heads = (n_seq + cap) * Hq                                                       # (room for parts: csrc/attention_f8.hip)
-    parts = torch.empty(heads * (D + 2), dtype=torch.float32, device=q.device)
-    tickets = _tickets(tickets, TICKET * n_seq * Hkv * tiles, q, what)
-    at = parts.data_ptr()
-    _check(_entry("ptl_attention_decode_f8")(*args, at, at + 4 * heads * D, tickets.data_ptr(), cap, int(n_seq), Hq, Hkv, D, page_size,
-                                             int(window), sink_at, scale, stream), what)
+    cap, parts_at, ends_at, tickets_at = 0, None, None, None
+    if tickets is not None:
+        _tickets(tickets, 0, q, what)                        # (checks)
+    if block_table.shape[1] * page_size > WHOLE_KEYS_F8:
+        tiles = -(-(Hq // Hkv) // 16)
+        cap = max(1, min(MOST_PARTS_F8, compute_units(q.device) // (Hkv * tiles)))     # a workgroup a compute unit
+        heads = (n_seq + cap) * Hq                                                   # (room for parts: csrc/attention_f8.hip)
+        parts = torch.empty(heads * (D + 2), dtype=torch.float32, device=q.device)
+        tickets = _tickets(tickets, TICKET * n_seq * Hkv * tiles, q, what)
+        parts_at, tickets_at = parts.data_ptr(), tickets.data_ptr()
+        ends_at = parts_at + 4 * heads * D
+    _check(_entry("ptl_attention_decode_f8")(*args, parts_at, ends_at, tickets_at, cap, int(n_seq), Hq, Hkv, D, page_size, int(window), sink_at,
+                                             scale, stream), what)
 
 
 WORTH_TILES = 12           # tiles of 64 keys that blocks of query rows have to become shorter by to be cut (csrc/attention_f8.hip)

@@ -385,6 +385,8 @@ def test_what_the_operators_refuse(ops):
         ops.attention_prefill_f8(odd.out, odd.qd, *odd.cache, *odd.tables, *odd.blocks(64), odd.scale)
     with pytest.raises(KernelError):                          # more sequences than the tables have
         ops.attention_decode_f8(s.out, s.qd, *s.cache, *s.tables, 3, s.scale)
+    with pytest.raises(KernelError):                          # more sequences than queries
+        ops.attention_decode_f8(s.out[:1], s.qd[:1], *s.cache, *s.tables, 2, s.scale)
     with pytest.raises(KernelError):
         attention("decode", tickets=torch.zeros(64, device="cuda"))
     with pytest.raises(KernelError):
