@@ -88,6 +88,32 @@ def test_steps(folders, monkeypatch, name, page, dtype, graphs):
     runner.manager.check()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_prompts_at_full_widths(tmp_path, gpu_device, monkeypatch, dim):
+    """32 heads on 8, two layers: portions whose few blocks are cut along their keys, recorded and not, and decode steps with and
+    without parts, one and several sequences."""
+    from pytriton_llama_amd.engine.batch import StepEntry
+    from pytriton_llama_amd.weights import write_random_model
+    cfg = dict(tiny("A")[0], num_hidden_layers=2, hidden_size=512, num_attention_heads=32, num_key_value_heads=8, head_dim=dim,
+               intermediate_size=512, max_position_embeddings=4096)
+    folder = str(tmp_path)
+    write_random_model(cfg, folder, seed=5, dtype=torch.float32, std=0.06)
+    runner = load(folder, torch.bfloat16, 16, 420, 4096, True)
+    seqs = random_sequences(256, [2813, 700, 40], seed=dim)
+    fed = dict.fromkeys(seqs, 0)
+    for step in [[("r0", 1400)], [("r0", 700)], [("r0", 700)], [("r0", 1)], [("r0", 1), ("r1", 600)], [("r2", 20), ("r0", 1), ("r1", 1)],
+                 [("r0", 1), ("r1", 1), ("r2", 1)], [("r0", 1), ("r1", 1), ("r2", 1)], [("r0", 1)]]:
+        entries = [StepEntry(r, seqs[r][fed[r]:fed[r] + n], [n - 1]) for r, n in step]
+        logits = runner.step(entries).float().cpu()
+        runner.manager.check()
+        for r, n in step:
+            fed[r] += n
+        for row, (r, n) in enumerate(step):
+            if r != "r0" or n > 1 or len(step) == 3:            # (the long one's plain form takes seconds)
+                want = last_logits(runner, folder, r, seqs[r][:fed[r]], monkeypatch, torch.bfloat16)
+                assert (logits[row] - want).abs().max() <= TOL[torch.bfloat16] * want.abs().max(), (r, fed[r])
+
+
 def test_first_layer_holds_the_rounded_keys(folders):
     """The first layer's keys and values do not depend on the cache: what it holds is them, rounded."""
     from pytriton_llama_amd.engine.batch import StepEntry
