@@ -81,6 +81,7 @@ class StepContext:
     ctx_lens: List[int] = field(default_factory=list)     # upper bounds of its size class)
     max_q_len: int = 0
     max_ctx_len: int = 0
+    lens_are_bounds: bool = False              # q_lens and ctx_lens are such bounds
     tickets: Optional[torch.Tensor] = None     # int32 zeros, ops.TICKET a single-token sequence and kv head: the workgroups of
                                                # a launch that share a sequence's keys count in them who is done, and leave zeros
     rotations: Optional[Rotations] = None      # while a model's forward runs: the cosines and sines of the rows

@@ -68,6 +68,7 @@ class _Recorded:
         # recording: planned for the longest context and the most rows
         self.ctx = self.layout.context([1] * B + [sizes.multi_tokens] * m, [max_model_len] * (B + m),
                                        logit_rows_are_identity=(m == 0))
+        self.ctx.lens_are_bounds = True
         self.graph = None
         self.logits = None
         self.copied = None                 # event: the last copy of the pinned buffer has been made

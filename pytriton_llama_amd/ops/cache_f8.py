@@ -237,16 +237,24 @@ def _prefill_resident(device: torch.device, num_heads: int, head_dim: int) -> in
 
 
 def attention_prefill_f8_plan(device: torch.device, num_heads: int, head_dim: int, blocks_of_64: int, blocks_of_128: int,
-                              max_keys: int = 0):
+                              max_keys: int = 0, bound: bool = False):
     """(block_rows, groups) for ``attention_prefill_f8``; arguments as of ``attention_prefill_mfma_plan``, which it follows but where few
-    blocks have many keys each: blocks of 128 rows, cut along their keys, from 4 of them on where the longest sequence has 160
-    keys for each (head sizes up to 64: 512). us in blocks of 64 and of 128 rows, 32 heads, rows behind keys: 1,100 behind 2,000 of
-    128 113 91, 1,531 behind 1,000 97 86, 512 behind 8,000 122 109, 2,048 alone 65 72, 500 behind 3,000 (4 blocks) 62 64, 200 behind 3,000 (2)
-    38 45; 1,024 behind 4,000 of 64 80 73, 2,048 behind 8,000 231 216, 700 behind 7,000 90 87, 2,048 behind 3,000 107 113, 1,500 behind 2,500
-    73 81."""
+    blocks have many keys each: blocks of 128 rows, cut along their keys, from 4 of them on where the longest sequence has 512
+    keys for each; 192 at head sizes above 64 if the blocks of 64 rows have no workgroup each at once. us in blocks of 64 and of 128
+    rows, 32 heads, rows behind keys: 1,024 behind 1,000 of 128 50 57, 900 behind 4,000 128 123, 512 behind 8,000 122 109, 500 behind 3,000
+    (4 blocks) 62 64, 200 behind 3,000 (2) 38 45; 1,100 behind 1,500 103 80, 1,536 behind 500 66 71, 1,531 behind 1,000 97 86, 2,048
+    alone 65 72; 1,024 behind 4,000 of 64 80 73, 2,048 behind 8,000 231 216, 2,048 behind 3,000 107 113, 1,500 behind 2,500 73 81.
+
+    ``bound``: max_keys is only a bound of what the sequences will have (a step that is recorded). Then blocks of 128 rows are for
+    head sizes above 64, a bound from 4,096 on and blocks of 64 rows that have no workgroup each at once: 2,048 rows of 128 lose 7 us
+    by them where the prompt begins and win 24 behind 2,048 keys; 1,024 rows lose 17 and win 8 behind 6,000."""
     t = max(1, _prefill_resident(device, num_heads, head_dim))
-    wide = 4 * blocks_of_128 >= 5 * t or (blocks_of_128 >= 4 and max_keys >= (160 if head_dim > 64 else 512) * blocks_of_128)
-    rows, blocks = (128, blocks_of_128) if wide else (64, blocks_of_64)
+    few = blocks_of_64 <= t
+    if bound:
+        long = not few and head_dim > 64 and max_keys >= 4096
+    else:
+        long = blocks_of_128 >= 4 and max_keys >= (192 if head_dim > 64 and not few else 512) * blocks_of_128
+    rows, blocks = (128, blocks_of_128) if long or 4 * blocks_of_128 >= 5 * t else (64, blocks_of_64)
     return rows, max(1, blocks if blocks <= 2 * t else t)
 
 

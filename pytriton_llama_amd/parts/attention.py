@@ -289,6 +289,6 @@ class PagedAttention(Part):
         keys = max(ctx.ctx_lens[n_dec:])
         rows, groups = ops.attention_prefill_f8_plan(
             q.device, self.num_heads, D, ctx.work[PORTIONS_64][0].numel(), ctx.work[PORTIONS_128][0].numel(),
-            min(keys, window) if window else keys)
+            min(keys, window) if window else keys, ctx.lens_are_bounds)
         ops.attention_prefill_f8(out, q, *held, *tables, *ctx.work[PORTIONS_128 if rows == 128 else PORTIONS_64], self.scale, window,
                                  rows, groups, sink=self.sink)

@@ -48,8 +48,15 @@ def test_the_plan_of_prompt_portions(monkeypatch):
     from pytriton_llama_amd import ops
     from pytriton_llama_amd.ops import cache_f8
     monkeypatch.setattr(cache_f8, "compute_units", lambda device: 256)
-    plan = lambda D, rows, keys: ops.attention_prefill_f8_plan("cuda", 32, D, -(-rows // 64), -(-rows // 128), keys)   # noqa: E731
-    assert plan(128, 2048, 2048) == (64, 32) and plan(128, 2048, 2748) == (128, 16) and plan(128, 1531, 7676) == (128, 12)
-    assert plan(128, 384, 100000) == (64, 6) and plan(128, 8192, 8192) == (128, 16)
+
+    def plan(D, rows, keys, bound=False):
+        return ops.attention_prefill_f8_plan("cuda", 32, D, -(-rows // 64), -(-rows // 128), keys, bound)
+
+    assert plan(128, 2048, 2048) == (64, 32) and plan(128, 2048, 4096) == (128, 16) and plan(128, 1531, 7676) == (128, 12)
+    assert plan(128, 1536, 2036) == (64, 24) and plan(128, 1531, 2531) == (128, 12)
+    assert plan(128, 1024, 2024) == (64, 16) and plan(128, 1024, 5024) == (128, 8) and plan(128, 384, 100000) == (64, 6)
+    assert plan(128, 8192, 8192) == (128, 16)
     assert plan(64, 2048, 5048) == (64, 32) and plan(64, 1024, 5024) == (128, 8) and plan(64, 2048, 2048) == (64, 32)
+    assert plan(128, 1024, 8192, True) == (64, 16) and plan(128, 1152, 8192, True) == (128, 9) and plan(128, 1152, 4000, True) == (64, 18)
+    assert plan(64, 2048, 100000, True) == (64, 32) and plan(64, 4096, 100000, True) == (128, 32)
     assert ops.attention_prefill_f8_plan("cuda", 1024, 64, 2, 1, 64) == (64, 2)
