@@ -23,58 +23,68 @@ struct F8Tables {
 
 // ===========================================================================
 // ptl_attention_generic_f8: float32 arithmetic on the vector units, for every type of query, head size (up to 640), page size
-// and number of heads. A workgroup has one query row of one head; its four waves take the keys 64 at a time in turn, a lane a key
-// for the scores and a lane every 64th column for the values.
-template <typename T, int NACC>
-__global__ void __launch_bounds__(256)
+// and number of heads. A workgroup has one query row of one head; its waves take the keys 64 at a time in turn, a lane a key
+// for the scores (rows of a multiple of 16 elements by 16 bytes) and a lane every 64th column for the values, of which a wave asks for AHEAD
+// rows before it uses one: with one at a time a turn was 64 ways to memory. Few rows have sixteen waves, more than two a compute unit
+// four: us with sixteen and four, float32, 32 heads of 64 on 8: 32 x 2,000 keys 82 45, 64 x 100 to 1,000 113 31, 60 rows behind 300 42 16,
+// 200 behind 700 153 71.
+//
+// What bounds it: few rows the chain of a turn, some 3 us (1 x 1,000 keys 7.8 us, 1 x 4,000 18.3, 8 x 2,048 27.2), many the vector units, which
+// have every key row anew for every query row (200 rows behind 700: 18 TFLOP/s).
+template <typename T, int NACC, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES)
 attn_generic_f8_kernel(T* __restrict__ out, long out_stride, const T* __restrict__ q, long q_stride, F8Cache cache, F8Tables tab,
                        const int32_t* __restrict__ work_seq, const int32_t* __restrict__ work_qoff, int Hq, int Hkv, int D,
                        int page_size, int window, const float* __restrict__ sink, float scale) {
-  extern __shared__ float lds[];
-  __shared__ float ps[4][64];              // a tile's probabilities times the values' scales
-  __shared__ long at[4][64];               // where its value rows lie
-  __shared__ float ends[4][2];
+  constexpr int AHEAD = NACC <= 2 ? 16 : NACC <= 4 ? 8 : 4, THREADS = 64 * WAVES;
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  __shared__ float ps[WAVES][64];          // a tile's probabilities times the values' scales
+  __shared__ long at[WAVES][64];           // where its value rows lie
+  __shared__ float ends[WAVES][2];
   float* qs = lds;                         // [D]
-  float* sums = lds + D;                   // [4][D]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int item = blockIdx.x >> 4, head = blockIdx.y;
-  const int seq = work_seq[item], r = work_qoff[item] + (blockIdx.x & 15);
+  float* sums = lds + D;                   // [WAVES][D]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // heads run fastest over the workgroups, which the eight dies take in turn: die c gets heads c Hq / 8 .. of which a kv head's lie together
+  // (rows fastest, the first rows of blocks, decoding requests', would all be one die's)
+  const int place = blockIdx.x / Hq, i_head = blockIdx.x - place * Hq;
+  const int item = place >> 4, head = Hq % 8 == 0 ? (i_head % 8) * (Hq / 8) + i_head / 8 : i_head;
+  const int seq = work_seq[item], r = work_qoff[item] + (place & 15);
   const int first = tab.q_start[seq], rows = tab.q_start[seq + 1] - first, ctx = tab.ctx_len[seq];
   if (r >= rows) return;
   const int row = first + r, pos = ctx - rows + r, kvh = head / (Hq / Hkv);
   const int32_t* bt = tab.block_table + (size_t)seq * tab.bt_stride;
-  for (int d = threadIdx.x; d < D; d += 256) qs[d] = to_float<T>(q[(size_t)row * q_stride + (size_t)head * D + d]);
+  for (int d = threadIdx.x; d < D; d += THREADS) qs[d] = to_float<T>(q[(size_t)row * q_stride + (size_t)head * D + d]);
   __syncthreads();
   const int lo = window > 0 ? max(0, pos - window + 1) : 0;
   float m = -INFINITY, l = 0.f, acc[NACC];
 #pragma unroll
   for (int a = 0; a < NACC; ++a) acc[a] = 0.f;
-  const bool words = D % 4 == 0;
-  for (int k0 = lo + 64 * wave; k0 <= pos; k0 += 256) {
-    const int key = k0 + lane, n = min(64, pos + 1 - k0);
-    float s = -INFINITY, vs = 0.f;
-    long row_at = 0;
-    if (lane < n) {
-      const int slot = key / page_size, page = bt[slot];
-      const size_t block = (size_t)page * Hkv + kvh;
-      row_at = (block * page_size + (key - slot * page_size)) * D;
-      const uint8_t* kr = cache.k + row_at;
-      float dot = 0.f;
-      if (words) {
-        for (int d = 0; d < D; d += 4) {
-          const int x = *reinterpret_cast<const int*>(kr + d);
-          const auto e = __builtin_amdgcn_cvt_pk_f32_fp8(x, false), f = __builtin_amdgcn_cvt_pk_f32_fp8(x, true);
-          dot = fmaf(e[0], qs[d], dot);
-          dot = fmaf(e[1], qs[d + 1], dot);
-          dot = fmaf(f[0], qs[d + 2], dot);
-          dot = fmaf(f[1], qs[d + 3], dot);
-        }
-      } else {
-        for (int d = 0; d < D; ++d) dot = fmaf(__builtin_amdgcn_cvt_f32_fp8((int)kr[d], 0), qs[d], dot);
+  auto four = [&](uint32_t x, const float* y, float dot) __attribute__((always_inline)) {
+    const auto e = __builtin_amdgcn_cvt_pk_f32_fp8((int)x, false), f = __builtin_amdgcn_cvt_pk_f32_fp8((int)x, true);
+    return fmaf(f[1], y[3], fmaf(f[0], y[2], fmaf(e[1], y[1], fmaf(e[0], y[0], dot))));
+  };
+  for (int k0 = lo + 64 * wave; k0 <= pos; k0 += THREADS) {
+    const int n = min(64, pos + 1 - k0), key = k0 + min(lane, n - 1);        // (lanes behind the last key: that one, weight zero)
+    const int slot = key / page_size, page = bt[slot];
+    const size_t block = (size_t)page * Hkv + kvh;
+    const long row_at = (block * page_size + (key - slot * page_size)) * D;
+    const float ks = cache.k_scale[block], vs = cache.v_scale[block];
+    const uint8_t* kr = cache.k + row_at;
+    float dot = 0.f;
+    if (D % 16 == 0) {
+#pragma unroll 4
+      for (int d = 0; d < D; d += 16) {
+        const uint4 x = *reinterpret_cast<const uint4*>(kr + d);
+        dot = four(x.w, qs + d + 12, four(x.z, qs + d + 8, four(x.y, qs + d + 4, four(x.x, qs + d, dot))));
       }
-      s = dot * cache.k_scale[block] * scale;
-      vs = cache.v_scale[block];
+    } else if (D % 4 == 0) {
+#pragma unroll 8
+      for (int d = 0; d < D; d += 4) dot = four(*reinterpret_cast<const uint32_t*>(kr + d), qs + d, dot);
+    } else {
+#pragma unroll 8
+      for (int d = 0; d < D; ++d) dot = fmaf(__builtin_amdgcn_cvt_f32_fp8((int)kr[d], 0), qs[d], dot);
     }
+    const float s = lane < n ? dot * ks * scale : -INFINITY;
     const float top = fmaxf(m, wave_max(s));
     const float to = top == -INFINITY ? 0.f : top, keep = expf(m - to);
     const float p = lane < n ? expf(s - to) : 0.f;
@@ -87,13 +97,20 @@ attn_generic_f8_kernel(T* __restrict__ out, long out_stride, const T* __restrict
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
     for (int a = 0; a < NACC; ++a) acc[a] *= keep;
-    for (int j = 0; j < n; ++j) {
-      const float pj = ps[wave][j];
-      const uint8_t* vr = cache.v + at[wave][j];
+    for (int j0 = 0; j0 < n; j0 += AHEAD) {
+      uint8_t x[AHEAD][NACC];
 #pragma unroll
-      for (int a = 0; a < NACC; ++a) {
-        const int d = lane + 64 * a;
-        if (d < D) acc[a] = fmaf(__builtin_amdgcn_cvt_f32_fp8((int)vr[d], 0), pj, acc[a]);
+      for (int j = 0; j < AHEAD; ++j) {
+        const uint8_t* vr = cache.v + at[wave][j0 + j];
+#pragma unroll
+        for (int a = 0; a < NACC; ++a) x[j][a] = vr[min(lane + 64 * a, D - 1)];
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const float pj = ps[wave][j0 + j];
+        // (rows behind the last key are the last one's: where that is NaN so is the result)
+#pragma unroll
+        for (int a = 0; a < NACC; ++a) acc[a] = fmaf(__builtin_amdgcn_cvt_f32_fp8((int)x[j][a], 0), pj, acc[a]);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -107,19 +124,19 @@ attn_generic_f8_kernel(T* __restrict__ out, long out_stride, const T* __restrict
   __syncthreads();
   float top = sink ? sink[head] : -INFINITY;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, ends[w][0]);
+  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, ends[w][0]);
   const float to = top == -INFINITY ? 0.f : top;
-  float total = sink ? expf(sink[head] - to) : 0.f, f[4];
+  float total = sink ? expf(sink[head] - to) : 0.f, f[WAVES];
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     f[w] = expf(ends[w][0] - to);
     total += ends[w][1] * f[w];
   }
   const float inv = total == 0.f ? 0.f : 1.0f / total;            // (a row without keys: zeros)
-  for (int d = threadIdx.x; d < D; d += 256) {
+  for (int d = threadIdx.x; d < D; d += THREADS) {
     float a = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) a = fmaf(sums[w * D + d], f[w], a);
+    for (int w = 0; w < WAVES; ++w) a = fmaf(sums[w * D + d], f[w], a);
     out[(size_t)row * out_stride + (size_t)head * D + d] = from_float<T>(a * inv);
   }
 }
@@ -127,32 +144,36 @@ attn_generic_f8_kernel(T* __restrict__ out, long out_stride, const T* __restrict
 extern "C" int ptl_attention_generic_f8(void* out, long out_stride, const void* q, long q_stride, const uint8_t* k, const uint8_t* v,
                                         const float* k_scale, const float* v_scale, const int32_t* q_start, const int32_t* ctx_len,
                                         const int32_t* block_table, int bt_stride, const int32_t* work_seq, const int32_t* work_qoff,
-                                        int n_work, int Hq, int Hkv, int D, int page_size, int window, const float* sink, float scale,
-                                        int dtype, hipStream_t stream) {
+                                        int n_work, int T, int Hq, int Hkv, int D, int page_size, int window, const float* sink,
+                                        float scale, int dtype, hipStream_t stream) {
   if (n_work <= 0) return PTL_OK;
   if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq > 65535 || D <= 0 || D > 640 || page_size <= 0 || n_work >= 1 << 26 || window < 0)
     return PTL_ERR_ARG;
   const F8Cache cache{k, v, k_scale, v_scale};
   const F8Tables tab{q_start, ctx_len, block_table, bt_stride};
-  const dim3 grid(16 * n_work, Hq);
-  const size_t lds = 5 * (size_t)D * sizeof(float);
-  auto go = [&](auto kernel, auto* o, auto* x) {
-    kernel<<<grid, 256, lds, stream>>>(o, out_stride, x, q_stride, cache, tab, work_seq, work_qoff, Hq, Hkv, D, page_size, window,
-                                       sink, scale);
+  const long groups = 16l * n_work * Hq;
+  if (groups >= 1l << 31) return PTL_ERR_ARG;
+  const dim3 grid((unsigned)groups);
+  const bool many = (long)T * Hq > 2l * compute_units();          // (T: rows of q, a workgroup each and head)
+  auto go = [&](auto kernel, int waves, auto* o, auto* x) {
+    kernel<<<grid, 64 * waves, (1 + waves) * (size_t)D * sizeof(float), stream>>>(o, out_stride, x, q_stride, cache, tab, work_seq, work_qoff,
+                                                                                  Hq, Hkv, D, page_size, window, sink, scale);
   };
-  if (dtype == PTL_DTYPE_F32) {
-    auto *o = (float*)out; auto* x = (const float*)q;
-    if (D <= 128) go(attn_generic_f8_kernel<float, 2>, o, x);
-    else if (D <= 256) go(attn_generic_f8_kernel<float, 4>, o, x);
-    else go(attn_generic_f8_kernel<float, 10>, o, x);
-  } else if (dtype == PTL_DTYPE_BF16) {
-    auto *o = (bf16_t*)out; auto* x = (const bf16_t*)q;
-    if (D <= 128) go(attn_generic_f8_kernel<bf16_t, 2>, o, x);
-    else if (D <= 256) go(attn_generic_f8_kernel<bf16_t, 4>, o, x);
-    else go(attn_generic_f8_kernel<bf16_t, 10>, o, x);
-  } else {
-    return PTL_ERR_ARG;
-  }
+  auto size = [&](auto* o, auto* x) {
+    using T = std::remove_pointer_t<decltype(o)>;
+    auto columns = [&](auto nacc) {
+      constexpr int NACC = decltype(nacc)::value;
+      if (many) go(attn_generic_f8_kernel<T, NACC, 4>, 4, o, x);
+      else go(attn_generic_f8_kernel<T, NACC, 16>, 16, o, x);
+    };
+    if (D <= 64) columns(std::integral_constant<int, 1>{});
+    else if (D <= 128) columns(std::integral_constant<int, 2>{});
+    else if (D <= 256) columns(std::integral_constant<int, 4>{});
+    else columns(std::integral_constant<int, 10>{});
+  };
+  if (dtype == PTL_DTYPE_F32) size((float*)out, (const float*)q);
+  else if (dtype == PTL_DTYPE_BF16) size((bf16_t*)out, (const bf16_t*)q);
+  else return PTL_ERR_ARG;
   return ptl_launch_status();
 }
 

@@ -24,7 +24,7 @@ CACHE_F8 = torch.float8_e4m3fn          # the codes' type
 _TYPES = {"p": ctypes.c_void_p, "l": ctypes.c_long, "i": ctypes.c_int, "f": ctypes.c_float}
 # entry -> library, types of its arguments (p: address, l: long, i: int, f: float)
 _ENTRIES = {"ptl_rope_store_f8": ("cache_f8", "pppplppppppp" "iiiiii" "piif" "ip"), "ptl_copy_pages": ("cache_f8", "pippip"),
-            "ptl_attention_generic_f8": ("attention_f8", "plplppppppp" "ipp" "iiiiii" "pfip"),
+            "ptl_attention_generic_f8": ("attention_f8", "plplppppppp" "ipp" "iiiiiii" "pfip"),
             "ptl_attention_decode_f8": ("attention_f8", "plplppppppp" "ippp" "iiiiiii" "pfp"),
             "ptl_attention_prefill_f8": ("attention_f8", "plplppppppp" "ipp" "iiippiiiiii" "pfp")}
 _loaded = {}
@@ -179,8 +179,8 @@ def attention_generic_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
     if not 0 < D <= 640 or Hq > 65535:
         raise KernelError(f"{what}: head size {D} exceeds the kernel's limit of 640 (or {Hq} heads that of 65,535)")
     n = _work(what, work_seq, work_qoff)
-    _check(_entry("ptl_attention_generic_f8")(*args, work_seq.data_ptr(), work_qoff.data_ptr(), n, Hq, Hkv, D, page_size, int(window),
-                                              sink_at, scale, _dtype_code(q), stream), what)
+    _check(_entry("ptl_attention_generic_f8")(*args, work_seq.data_ptr(), work_qoff.data_ptr(), n, q.shape[0], Hq, Hkv, D, page_size,
+                                              int(window), sink_at, scale, _dtype_code(q), stream), what)
 
 
 def attention_f8_fits(dtype: torch.dtype, num_heads: int, num_kv_heads: int, head_dim: int, page_size: int) -> bool:
