@@ -10,8 +10,8 @@ properties once, and entries know their arguments' types, so that addresses go a
 """
 from __future__ import annotations
 
+import array
 import ctypes
-import itertools
 from typing import Optional, Sequence
 
 import torch
@@ -298,8 +298,8 @@ def attention_prefill_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
 
 
 def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[int]) -> None:
-    """Page src[i] -> page dst[i] in all layers of every pool [layers, pages, ...] (contiguous, up to 16 of them, any dtype), one
-    launch. src, dst: page numbers on the host; no page may be written twice, or both read and written (one may be read many
+    """Page src[i] -> page dst[i] in all layers of every pool [layers, pages, ...] (contiguous, up to 16 of them, any dtype), a
+    launch for 256 pages. src, dst: page numbers on the host; no page may be written twice, or both read and written (one may be read many
     times). The numbers go with the launch: nothing is uploaded, and a recorded launch keeps its own."""
     src, dst = list(src), list(dst)
     n = len(src)
@@ -323,6 +323,6 @@ def copy_pages(pools: Sequence[torch.Tensor], src: Sequence[int], dst: Sequence[
         raise KernelError("copy_pages: a page is written twice, or read and written")
     if n == 0 or not desc:
         return
-    numbers, described = (ctypes.c_int32 * (2 * n))(*itertools.chain(src, dst)), (ctypes.c_long * len(desc))(*desc)
-    at = ctypes.addressof(numbers)
-    _check(_entry("ptl_copy_pages")(ctypes.addressof(described), len(desc) // 4, at, at + 4 * n, n, stream), "copy_pages")
+    numbers, described = array.array("i", src + dst), array.array("l", desc)
+    at = numbers.buffer_info()[0]
+    _check(_entry("ptl_copy_pages")(described.buffer_info()[0], len(desc) // 4, at, at + 4 * n, n, stream), "copy_pages")
