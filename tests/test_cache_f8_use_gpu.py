@@ -167,6 +167,41 @@ def test_decode_with_workgroups_of_four_and_of_eight_waves(ops, Hq, Hkv, D, wind
         assert not tickets.any()
 
 
+def test_recorded_copies_keep_their_pages(ops):
+    """What a recorded copy copies was said when it was recorded; a recorded store of many rows takes its slots from where they are."""
+    g = torch.Generator().manual_seed(0)
+    pools = [torch.randint(0, 256, (2, 600, 3, 5), generator=g, dtype=torch.uint8).cuda(), torch.randn(2, 600, 16, generator=g).cuda()]
+    src, dst = list(range(300)), list(range(599, 299, -1))
+    q = torch.randn(200, 6, 64, generator=g).to(torch.bfloat16).cuda()
+    cache = [p[0] for p in empty_cache(1, 40, 2, 16, 64)]
+    slots, positions, inv_freq = i32(range(200)), i32(range(200)), torch.ones(32, device="cuda") / 7
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.copy_pages(pools, src[:1], dst[:1])
+        ops.rope_store_f8(q[:, :2], q[:, 2:4], q[:, 4:], positions, inv_freq, slots, *cache)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.copy_pages(pools, src, dst)
+        turned = ops.rope_store_f8(q[:, :2], q[:, 2:4], q[:, 4:], positions, inv_freq, slots, *cache)
+    src[:], dst[:] = [5] * 300, [7] * 300
+    for turn in range(4):
+        for p in pools:
+            p[:, :300].copy_(torch.randint(0, 256, p[:, :300].shape, generator=g).to(p.dtype))
+        q.copy_(torch.randn(q.shape, generator=g).to(q.dtype))
+        slots.copy_(i32([16 * turn + i + turn for i in range(200)]))
+        want = [p.clone() for p in pools]
+        for w in want:
+            w[:, list(range(599, 299, -1))] = w[:, :300]
+        own = [t.view(torch.uint8).clone().view(F8) if t.dtype == F8 else t.clone() for t in cache]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, w) for p, w in zip(pools, want))
+        assert torch.equal(ops.rope_store_f8(q[:, :2], q[:, 2:4], q[:, 4:], positions, inv_freq, slots, *own), turned)
+        assert all(torch.equal(a, b) for a, b in zip(bits(cache), bits(own)))
+
+
 CUTS = [[(64, 5000)], [(1, 3000), (63, 2999), (65, 1100)], [(200, 3000)], [(64, 64), (64, 900), (17, 1500), (3, 385), (5, 384)]]
 
 
