@@ -185,7 +185,9 @@ class Engine:
         with. A branch draws numbers of its own unless its params name a seed: one that shares the seed
         repeats the request. What the request has in the cache is shared where that is possible
         (CacheManager.fork) and there is room to run; otherwise the branch waits and is computed from its tokens,
-        like a preempted request. Returns the new requests' ids."""
+        like a preempted request. (A page in 8 bits that is copied keeps the scale of all it held, later tokens of the
+        request's too: numbers below 2^-14 of the page's largest may be rounded otherwise than in a run by itself.)
+        Returns the new requests' ids."""
         req = self.requests.get(request_id)
         if req is None or req.status == FINISHED:
             raise ValueError(f"request {request_id!r} is not one that can branch")

@@ -252,6 +252,44 @@ def test_log_probabilities_of_branches(folders):
     assert reqs[made[0]].output == reqs[a].output == reqs[made[1]].output
 
 
+@pytest.mark.parametrize("cache_dtype", [None, "float8_e4m3fn"])
+@pytest.mark.parametrize("seed", range(3))
+def test_branches_and_aborts_in_random_order(folders, cache_dtype, seed):
+    """Requests come, branch and are aborted between steps, some under way, with too few pages for all: every page is held by whom it is
+    counted for, and each ends with the tokens that it began with and as many as it was to have."""
+    import random
+    from pytriton_llama_amd.engine import SamplingParams
+    rng = random.Random(seed)
+    e = engine(folders["C"], cache_dtype=cache_dtype, graphs=True, seqs=5, pages=22)
+    free = e.runner.manager.paged[0].pool.num_free
+    live, began = {}, {}
+    for turn in range(60):
+        act = rng.random()
+        if act < 0.25 and len(live) < 9:
+            p = SamplingParams(temperature=1.0, max_new_tokens=rng.randint(1, 24), seed=rng.randint(0, 99), ignore_eos=True)
+            rid = e.add_request([rng.randrange(300) for _ in range(rng.randint(1, 45))], p)
+            live[rid], began[rid] = e.requests[rid], []
+        elif act < 0.5 and live:
+            rid = rng.choice(sorted(live))
+            n = rng.randint(0, len(live[rid].output))
+            if live[rid].status != "finished" and len(live) < 9 and n < live[rid].params.max_new_tokens:
+                for b in e.fork(rid, count=rng.randint(1, 2), num_output=n):
+                    live[b], began[b] = e.requests[b], live[rid].output[:n]
+        elif act < 0.6 and live:
+            rid = rng.choice(sorted(live))
+            e.abort(rid)
+            del live[rid]
+        if e.has_work:
+            e.step()
+        e.runner.manager.check()
+    while e.has_work:
+        e.step()
+        e.runner.manager.check()
+    assert e.runner.manager.paged[0].pool.num_free == free
+    for rid, r in live.items():
+        assert r.status == "finished" and len(r.output) == r.params.max_new_tokens and r.output[:len(began[rid])] == began[rid]
+
+
 def test_branches_are_preempted_like_others(folders):
     """Few pages: branches give way and are computed again; shared pages stay with who holds them."""
     from pytriton_llama_amd.engine import SamplingParams
