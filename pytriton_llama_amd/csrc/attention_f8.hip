@@ -896,6 +896,19 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
           for (int r = 0; r < RT; ++r) st[r][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, qf[r][kk].v, st[r][kt], 0, 0, 0);
         }
       }
+      auto transposed = [&](const bf16_t* x) {
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)x);
+      };
+      // half of the values are on their way while the softmax is made (us, rows behind keys: 2,048 behind 2,048 of 128 163 160, 1,024 behind
+      // 1,000 49.4 48.4, 512 behind 1,024 of 64 22.2 21.7, 2,048 behind 3,000 107.6 108.5; keys before the conversion as well: 138)
+      Frag8 early[RT == 1 ? 2 * ND : 1];
+      if constexpr (RT == 1) {
+#pragma unroll
+        for (int dt = 0; dt < 2 * ND; ++dt) {
+          early[dt].s[0] = transposed(Vb + value_at(dt));
+          early[dt].s[1] = transposed(Vb + 16 * D + value_at(dt));
+        }
+      }
       Frag8 p[RT][2];
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
@@ -931,16 +944,17 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
       }
       // (two row tiles leave no registers for values that are read early)
       if constexpr (RT == 2) __builtin_amdgcn_sched_barrier(0);
-      auto transposed = [&](const bf16_t* x) {
-        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)x);
-      };
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
 #pragma unroll
         for (int dt = 0; dt < 2 * ND; ++dt) {
           Frag8 a;
-          a.s[0] = transposed(Vb + 32 * half * D + value_at(dt));
-          a.s[1] = transposed(Vb + (32 * half + 16) * D + value_at(dt));
+          if (RT == 1 && half == 0) {
+            a = early[dt];
+          } else {
+            a.s[0] = transposed(Vb + 32 * half * D + value_at(dt));
+            a.s[1] = transposed(Vb + (32 * half + 16) * D + value_at(dt));
+          }
 #pragma unroll
           for (int r = 0; r < RT; ++r) o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, p[r][half].v, o[r][dt], 0, 0, 0);
         }
