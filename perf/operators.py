@@ -313,8 +313,9 @@ def _attention_own(s):
         ops.attention_decode_f8(out, s.q, *cache, s.q_start, s.ctx_len, s.block_table, s.n, s.scale, case["window"],
                                 tickets=s.tickets)
     else:
-        rows, groups = ops.attention_prefill_mfma_plan(s.q.device, case["heads"], case["dim"], s.blocks_64[0].numel(),
-                                                       s.blocks_128[0].numel(), s.longest_k)
+        keys = min(s.longest_k, case["window"]) if case["window"] else s.longest_k
+        rows, groups = ops.attention_prefill_f8_plan(s.q.device, case["heads"], case["dim"], s.blocks_64[0].numel(),
+                                                     s.blocks_128[0].numel(), keys)
         ops.attention_prefill_f8(out, s.q, *cache, s.q_start, s.ctx_len, s.block_table,
                                  *(s.blocks_128 if rows == 128 else s.blocks_64), s.scale, case["window"], rows, groups)
     return out
