@@ -808,12 +808,6 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
     const int wave_lo = window > 0 ? max(0, min_q - window + 1) : 0, wave_lo_last = window > 0 ? max(0, max_q - window + 1) : 0;
     f32x4_t o[RT][2 * ND + 1];
     float m_run[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      m_run[r] = -INFINITY;
-#pragma unroll
-      for (int t = 0; t <= 2 * ND; ++t) o[r][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
     const int k_lo = window > 0 ? max(0, first_q - window + 1) : 0, k_end = min(ctx, first_q + rows);
     const int k_begin = k_lo / BN * BN, n_all = max(0, (k_end - k_begin + BN - 1) / BN);
     int t_first = 0, n_tiles = n_all, n_parts = 1;   // this workgroup's tiles of the block
@@ -881,8 +875,9 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
       // what was read is in registers: the next tile's codes may come to its place (free here: the products read none of it)
       if constexpr (STAGED) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     };
-    auto tile = [&](int k0, const bf16_t* Kb, const bf16_t* Vb, auto masked_tag) __attribute__((always_inline)) {
-      constexpr bool MASKED = decltype(masked_tag)::value;
+    // MASKED: some row does not see some key. CAREFUL: and a value may be a NaN
+    auto tile = [&](int k0, const bf16_t* Kb, const bf16_t* Vb, auto masked_tag, auto careful_tag) __attribute__((always_inline)) {
+      constexpr bool MASKED = decltype(masked_tag)::value, CAREFUL = decltype(careful_tag)::value;
       f32x4_t st[RT][4];
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt) {
@@ -899,10 +894,11 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
       auto transposed = [&](const bf16_t* x) {
         return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)x);
       };
-      // half of the values are on their way while the softmax is made (us, rows behind keys: 2,048 behind 2,048 of 128 163 160, 1,024 behind
-      // 1,000 49.4 48.4, 512 behind 1,024 of 64 22.2 21.7, 2,048 behind 3,000 107.6 108.5; keys before the conversion as well: 138)
+      // half of the values are on their way while the softmax is made (us without and with it, rows behind keys, three runs of each within
+      // 0.1: 1,024 behind 1,000 of 128 49.5 48.6, 512 behind 1,024 of 64 22.4 22.0; 2,048 of 64 35.2 35.2, 2,048 behind 3,000 of 64 110.7
+      // 111.0, 2,048 of 128 65.5 65.2; keys before the conversion as well costs a quarter)
       Frag8 early[RT == 1 ? 2 * ND : 1];
-      if constexpr (RT == 1) {
+      if constexpr (RT == 1 && !CAREFUL) {
 #pragma unroll
         for (int dt = 0; dt < 2 * ND; ++dt) {
           early[dt].s[0] = transposed(Vb + value_at(dt));
@@ -942,6 +938,51 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
             for (int i = 0; i < 4; ++i)
               p[r][half].v[4 * t + i] = (__bf16)__builtin_amdgcn_exp2f(fmaf(st[r][2 * half + t][i], scale_log2, mc));
       }
+      if constexpr (CAREFUL) {
+        // a NaN goes in as zero, and a product of ones for NaNs with ones for the keys that a row sees counts those it is to have
+#pragma unroll
+        for (int dt = 0; dt < 2 * ND; ++dt) {
+          f32x4_t nans[RT];
+#pragma unroll
+          for (int r = 0; r < RT; ++r) nans[r] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            Frag8 a, is_nan;
+            a.s[0] = transposed(Vb + 32 * half * D + value_at(dt));
+            a.s[1] = transposed(Vb + (32 * half + 16) * D + value_at(dt));
+            auto split = [](uint32_t& x) {          // codes are finite or a NaN: one if the exponent's bits are all set
+              const uint32_t both = ((((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xffffu;
+              x &= ~both;
+              return both & 0x3f803f80u;
+            };
+            is_nan.u = make_uint4(split(a.u.x), split(a.u.y), split(a.u.z), split(a.u.w));
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+              Frag8 seen;
+              int first = k0 + 32 * half + 4 * lg;
+              asm("" : "+v"(first));              // (made anew for every piece of values: kept they take registers that the other products need)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const int k = first + 16 * (j >> 2) + (j & 3);
+                seen.v[j] = (__bf16)(k <= qpos[r] && k < k_end && k > qpos[r] - seen_back ? 1.0f : 0.0f);
+              }
+              o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, p[r][half].v, o[r][dt], 0, 0, 0);
+              nans[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(is_nan.v, seen.v, nans[r], 0, 0, 0);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[r][dt][i] = nans[r][i] > 0.f ? __uint_as_float(0x7fc00000u) : o[r][dt][i];
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            o[r][2 * ND] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones.v, p[r][half].v, o[r][2 * ND], 0, 0, 0);
+        return;
+      }
       // (two row tiles leave no registers for values that are read early)
       if constexpr (RT == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -972,12 +1013,21 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
       }
       if (wave_has_rows && k0 <= max_q && k0 + BN > wave_lo) {
         const bool need_mask = k0 + BN - 1 > min_q || k0 + BN > k_end || k0 < wave_lo_last;
-        if (need_mask) tile(k0, Ks[buffer], Vs[buffer], std::true_type{});
-        else tile(k0, Ks[buffer], Vs[buffer], std::false_type{});
+        if (need_mask) tile(k0, Ks[buffer], Vs[buffer], std::true_type{}, std::false_type{});
+        else tile(k0, Ks[buffer], Vs[buffer], std::false_type{}, std::false_type{});
       }
       if (!STAGED && t + 2 < n_tiles) { load(t + 2); load_page(t + 3); }
       __syncthreads();
     };
+    auto begin_sums = [&] {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        m_run[r] = -INFINITY;
+#pragma unroll
+        for (int t = 0; t <= 2 * ND; ++t) o[r][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      }
+    };
+    begin_sums();
     if (t_first < n_tiles) {
       load_page(t_first);
       load(t_first);
@@ -989,6 +1039,35 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
     for (int t = t_first; t < n_tiles; t += 2) {
       turn(t, 0);
       if (t + 1 < n_tiles) turn(t + 1, 1);
+    }
+    // A value that is a NaN makes one of every row that its tile's products go to, also of rows that do not see its key: zero times
+    // NaN is one. Where sums are NaNs the block is taken again with the careful products (by the workgroup's waves
+    // together); where they are not, all that costs is to look at them once a block (us without and with it, 32 heads: 2,048 rows of 64
+    // 34.9 35.2, of 128 64.9 65.2, 1,531 behind 6,145 keys of 128 242.6 243.2; 1,024 behind 4,000 of 64, blocks of 128 rows whose registers
+    // are all taken, 72.8 75.0).
+    {
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int t = 0; t < 2 * ND; ++t) sum += (o[r][t][0] + o[r][t][1]) + (o[r][t][2] + o[r][t][3]);
+      // (the second buffer: its last reader has passed the last turn's barrier, its next writer comes behind another one)
+      int* const found = reinterpret_cast<int*>(Ks[1]);
+      const bool here = __any(sum != sum);
+      if (lane == 0) found[wave] = here;
+      __syncthreads();
+      if (__builtin_amdgcn_readfirstlane(found[0] | found[1] | found[2] | found[3])) {
+        begin_sums();
+        for (int t = t_first; t < n_tiles; ++t) {
+          const int k0 = k_begin + t * BN;
+          load_page(t);
+          load(t);
+          convert(t, Ks[0], Vs[0]);
+          __syncthreads();
+          if (wave_has_rows && k0 <= max_q && k0 + BN > wave_lo) tile(k0, Ks[0], Vs[0], std::true_type{}, std::true_type{});
+          __syncthreads();
+        }
+      }
     }
     if constexpr (CUT) {
       if (n_parts > 1) {

@@ -358,6 +358,32 @@ def test_prefill(ops, Hq, Hkv, D, P, window, rows, groups):
     s.check(matrix_cores=True)
 
 
+@pytest.mark.parametrize("rows,groups", [(64, 0), (64, 2), (128, 0), (128, 2)])
+@pytest.mark.parametrize("Hq,Hkv,D,P,window", [(8, 2, 64, 16, 0), (4, 2, 128, 32, 0), (3, 1, 96, 16, 40), (4, 4, 32, 64, 0), (4, 2, 128, 16, 70)])
+def test_prefill_of_numbers_that_are_none(ops, Hq, Hkv, D, P, window, rows, groups):
+    """A value that is a NaN is one in its column for the rows that see its key, a key that is one in all columns; other rows of the
+    block, before it or with a window that has passed it, are what they are without it."""
+    s = Step(torch.bfloat16, Hq, Hkv, D, P, [(70, 203), (1, 40), (200, 431), (64, 64), (5, 1500)], window, seed=D, spread=1.5)
+    last = Hkv - 1
+    for seq, key, head, d in [(0, 150, 0, 0), (0, 202, last, D - 1), (2, 231, last, 17), (2, 300, 0, 31), (2, 430, 0, 3), (3, 1, last, 5),
+                              (3, 40, 0, 16), (4, 1497, last, 30)]:
+        s.vc.view(torch.uint8)[s.table[seq][key // P], head, key % P, d] = 0xff if d % 2 else 0x7f
+        s.v[s.table[seq][key // P], head, key % P, d] = math.nan
+    s.kc.view(torch.uint8)[s.table[3][50 // P], last, 50 % P, 9] = 0x7f
+    s.k[s.table[3][50 // P], last, 50 % P, 9] = math.nan
+    s.device()
+    ops.attention_prefill_f8(s.out, s.qd, *s.cache, *s.tables, *s.blocks(rows), s.scale, window, rows, groups)
+    want = plain_f8.attention(s.q[:s.q_start[-1]], s.k, s.v, s.q_start, s.ctx, s.table, s.scale, window)[0]
+    nan, got = torch.isnan(want), s.out[:s.q_start[-1]].cpu()
+    assert nan.any() and not nan.all() and torch.equal(torch.isnan(got), nan)
+    # (the other numbers: against the same without the NaNs, whose rows and columns are left out)
+    for x in (s.k, s.v):
+        x.nan_to_num_(0.0)
+    s.out[:s.q_start[-1]] = torch.where(nan, plain_f8.attention(s.q[:s.q_start[-1]], s.k, s.v, s.q_start, s.ctx, s.table, s.scale,
+                                                                 window)[0].to(got.dtype), got).cuda()
+    s.check(matrix_cores=True)
+
+
 @pytest.mark.parametrize("rows", [64, 128])
 def test_prefill_behind_decoding_sequences_with_a_sink(ops, rows):
     s = Step(torch.bfloat16, 8, 4, 64, 16, [(1, 40), (1, 700), (33, 90), (150, 150)], 0, seed=7).device()
