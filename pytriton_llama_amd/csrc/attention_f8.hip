@@ -149,6 +149,7 @@ extern "C" int ptl_attention_generic_f8(void* out, long out_stride, const void* 
   if (n_work <= 0) return PTL_OK;
   if (Hq <= 0 || Hkv <= 0 || Hq % Hkv || Hq > 65535 || D <= 0 || D > 640 || page_size <= 0 || n_work >= 1 << 26 || window < 0)
     return PTL_ERR_ARG;
+  if (((uintptr_t)k | (uintptr_t)v) % (D % 16 == 0 ? 16 : D % 4 == 0 ? 4 : 1)) return PTL_ERR_ARG;
   const F8Cache cache{k, v, k_scale, v_scale};
   const F8Tables tab{q_start, ctx_len, block_table, bt_stride};
   const long groups = 16l * n_work * Hq;

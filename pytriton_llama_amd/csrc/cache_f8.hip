@@ -373,7 +373,7 @@ extern "C" int ptl_rope_store_f8(void* q_out, const void* q, const void* k, cons
   if (T <= 0) return PTL_OK;
   if (Hq <= 0 || Hkv <= 0 || D <= 0 || (D & 1) || D > 640 || page_size <= 0 || (long)page_size * D >= 1l << 30) return PTL_ERR_ARG;
   if (slots && (!k_cache || !v_cache || !k_scale || !v_scale)) return PTL_ERR_ARG;
-  if (((uintptr_t)k_cache | (uintptr_t)v_cache) % 16) return PTL_ERR_ARG;
+  if (((uintptr_t)k_cache | (uintptr_t)v_cache) % (D % 16 == 0 ? 16 : D % 4 == 0 ? 4 : 2)) return PTL_ERR_ARG;
   if (partials && (T > SCALED_ROWS || count <= 0 || size <= 0)) return PTL_ERR_ARG;
   const RowFactor factor{partials, count, partials ? 1.0f / (float)size : 0.f, eps};
   const int in_all = slots ? (int)min((long)pages * page_size, 0x7fffffffl) : 0;

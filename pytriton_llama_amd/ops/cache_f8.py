@@ -62,8 +62,10 @@ def _cache(what: str, Hkv: int, D: int, k_cache, v_cache, k_scale, v_scale):
     if k_cache.dtype != CACHE_F8 or v_cache.dtype != CACHE_F8:
         raise KernelError(f"{what}: caches must be float8_e4m3fn, got {k_cache.dtype} and {v_cache.dtype}")
     k, v = k_cache.data_ptr(), v_cache.data_ptr()
-    if not k_cache.is_contiguous() or not v_cache.is_contiguous() or (k | v) % 16:
-        raise KernelError(f"{what}: caches must be contiguous and 16-byte aligned")
+    # (what the kernels read at once lies in one row: a layer of a pool may begin at any of its multiples of D bytes)
+    need = 16 if D % 16 == 0 else 4 if D % 4 == 0 else 2 - D % 2
+    if not k_cache.is_contiguous() or not v_cache.is_contiguous() or (k | v) % need:
+        raise KernelError(f"{what}: caches must be contiguous and {need}-byte aligned")
     for t in (k_scale, v_scale):
         if t.dtype != torch.float32 or t.shape != shape[:2] or not t.is_contiguous():
             raise KernelError(f"{what}: scales must be contiguous float32 [{shape[0]}, {Hkv}]")

@@ -60,3 +60,16 @@ def test_the_plan_of_prompt_portions(monkeypatch):
     assert plan(128, 1024, 8192, True) == (64, 16) and plan(128, 1152, 8192, True) == (128, 9) and plan(128, 1152, 4000, True) == (64, 18)
     assert plan(64, 2048, 100000, True) == (64, 32) and plan(64, 4096, 100000, True) == (128, 32)
     assert ops.attention_prefill_f8_plan("cuda", 1024, 64, 2, 1, 64) == (64, 2)
+
+
+@pytest.mark.parametrize("D,need", [(64, 16), (48, 16), (12, 4), (8, 4), (10, 2), (33, 1)])
+def test_a_layer_of_a_pool_begins_at_a_multiple_of_its_rows(D, need):
+    """Pages of odd sizes: the layers of one pool begin where the pages before them end; what lies between rows is refused."""
+    pool, scale = torch.zeros(3, 5, 1, 3, D).to(ops.CACHE_F8), torch.ones(3, 5, 1)
+    for layer in range(3):
+        pages, page_size, at = cache_f8._cache("a call", 1, D, pool[layer], pool[layer], scale[layer], scale[layer])
+        assert (pages, page_size) == (5, 3) and at[0] == pool.data_ptr() + layer * 15 * D
+    if need > 1:
+        off = pool.flatten()[need // 2:need // 2 + 15 * D].view(5, 1, 3, D)
+        with pytest.raises(ops.KernelError, match=f"{need}-byte"):
+            cache_f8._cache("a call", 1, D, pool[0], off, scale[0], scale[0])

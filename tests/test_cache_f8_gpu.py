@@ -393,6 +393,37 @@ def test_prefill_behind_decoding_sequences_with_a_sink(ops, rows):
     s.check(sink, first=2, matrix_cores=True)
 
 
+@pytest.mark.parametrize("dtype,Hkv,D,P", [(torch.float32, 1, 10, 3), (torch.bfloat16, 3, 34, 1), (torch.float32, 1, 12, 5), (torch.bfloat16, 1, 2, 1),
+                                           (torch.float32, 1, 20, 7)])
+def test_layers_of_a_pool_of_odd_pages(ops, dtype, Hkv, D, P):
+    """Layers that begin at a multiple of 2 or 4 bytes: stored, grown and read as in a cache of their own."""
+    layers, pages, n = 3, 7, 5 * P + 1
+    g = torch.Generator().manual_seed(D)
+    codes = torch.zeros(2, layers, pages, Hkv, P, D, device="cuda", dtype=torch.uint8).view(F8)
+    scales = torch.zeros(2, layers, pages, Hkv, device="cuda")
+    table = torch.randperm(pages, generator=g).tolist()
+    slots = torch.tensor([table[i // P] * P + i % P for i in range(n)], dtype=torch.int32)
+    pos = torch.arange(n, dtype=torch.int32)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")   # noqa: E731
+    for layer in range(layers):
+        alone = [torch.zeros(pages, Hkv, P, D, device="cuda", dtype=torch.uint8).view(F8) for _ in range(2)] + [
+            torch.zeros(pages, Hkv, device="cuda") for _ in range(2)]
+        pooled = [codes[0, layer], codes[1, layer], scales[0, layer], scales[1, layer]]
+        x = (torch.randn(n, 4 * Hkv, D, generator=g) * torch.exp(2 * torch.randn(n, 1, 1, generator=g))).to(dtype).cuda()
+        outs = []
+        for cache in (alone, pooled):
+            for a, b in ((0, 2 * P + 1), (2 * P + 1, n)):              # (the second call begins inside of a page)
+                q = ops.rope_store_f8(x[a:b, :2 * Hkv], x[a:b, 2 * Hkv:3 * Hkv], x[a:b, 3 * Hkv:], pos[a:b].cuda(), None,
+                                      slots[a:b].cuda(), *cache)
+            out = torch.empty_like(q)
+            ops.attention_generic_f8(out, q, *cache, i32([0, b - a]), i32([n]), i32([table]), i32([0] * -(-(b - a) // 16)),
+                                     i32(list(range(0, b - a, 16))), D ** -0.5)
+            outs.append(out)
+        assert torch.equal(outs[0], outs[1]) and not torch.isnan(outs[0]).any()
+        for a, b in zip(alone, pooled):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 # ---- copies ----------------------------------------------------------------------------------------
 POOLS = [[(3, 20, (2, 16, 64), torch.bfloat16)], [(2, 9, (3, 5, 7), torch.float32), (2, 9, (3,), torch.float32)],
          [(4, 600, (2, 16, 32), F8), (4, 600, (2, 16, 32), F8), (4, 600, (2,), torch.float32), (4, 600, (2,), torch.float32)],
