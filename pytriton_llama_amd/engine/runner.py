@@ -28,7 +28,8 @@ class ModelRunner:
         self.model = model
         self.device = model.device
         if self.device.type == "cuda":
-            ops.library.require(model.kernel_libraries() + (("cache_f8", "attention_f8") if cache_dtype is not None else ()))
+            # (cache_f8 has the copies of pages too, which requests that branch need over any cache)
+            ops.library.require(model.kernel_libraries() + ("cache_f8",) + (("attention_f8",) if cache_dtype is not None else ()))
         self.manager = CacheManager(model.cache_layers_in(cache_dtype), page_size, num_pages, max_num_seqs)
         self.storage = CacheStorage(self.manager, model.dtype, self.device)
         # decode-only steps replay a HIP graph when the longest request is known
@@ -87,14 +88,14 @@ class ModelRunner:
             for n in new:
                 copies += self.manager.fork(request, n, num_tokens)
                 made.append(n)
+            for g in range(len(self.manager.paged)):
+                self.storage.copy_pages(g, [s for h, s, _ in copies if h == g], [d for h, _, d in copies if h == g])
+            for n in made:
+                self.storage.copy_slot(self.manager.slot_of[request], self.manager.slot_of[n])
         except Exception:
             for n in made:
                 self.manager.free(n)
             raise
-        for g in range(len(self.manager.paged)):
-            self.storage.copy_pages(g, [s for h, s, _ in copies if h == g], [d for h, _, d in copies if h == g])
-        for n in made:
-            self.storage.copy_slot(self.manager.slot_of[request], self.manager.slot_of[n])
 
     def end(self, request: Hashable) -> None:
         """The request is finished: what it holds is given back."""

@@ -8,6 +8,7 @@ from pytriton_llama_amd.cache import RELEASED, CacheManager, CannotShare, OutOfP
 from pytriton_llama_amd.cache.storage import CacheStorage
 from pytriton_llama_amd.config import EngineConfig, build_model
 from pytriton_llama_amd.engine.request import Request, SamplingParams
+from pytriton_llama_amd.engine.runner import ModelRunner
 from pytriton_llama_amd.engine.scheduler import Scheduler
 from pytriton_llama_amd.parts import StateSpec, paged_kv_spec
 from tiny_configs import tiny
@@ -211,3 +212,56 @@ def test_the_command_line_refuses_no_samples(samples, capsys):
     with pytest.raises(SystemExit):
         cli.main(["--checkpoints_dir", "nowhere", "--samples", samples])
     assert "--samples" in capsys.readouterr().err
+
+
+# ---- the runner's part ---------------------------------------------------------------------------
+class Copies:
+    """Stands for the device memory: what was asked for, or an error at the copy named ``fails``."""
+
+    def __init__(self, fails=None):
+        self.fails, self.pages, self.slots = fails, [], []
+
+    def copy_pages(self, group, src, dst):
+        if self.fails == "pages":
+            raise OSError("no such kernel")
+        self.pages += [(group, s, d) for s, d in zip(src, dst)]
+
+    def copy_slot(self, src, dst):
+        if self.fails == "slot":
+            raise OSError("no such kernel")
+        self.slots.append((src, dst))
+
+
+def host_runner(manager, storage):
+    r = object.__new__(ModelRunner)
+    r.manager, r.storage = manager, storage
+    return r
+
+
+@pytest.mark.parametrize("fails", ["pages", "slot"])
+def test_branches_whose_copies_fail_hold_nothing(fails):
+    m = CacheManager([FULL], page_size=4, num_pages=8, max_num_seqs=4)
+    live(m, "a", 6)
+    with pytest.raises(OSError):
+        host_runner(m, Copies(fails)).fork("a", ["b", "c"], 5)
+    assert not m.is_live("b") and not m.is_live("c") and m.num_free_slots == 3 and m.paged[0].pool.num_free == 6
+    m.check()
+
+
+@pytest.mark.parametrize("cache_dtype", [None, F8])
+def test_the_kernel_that_copies_pages_is_loaded_with_the_model(monkeypatch, cache_dtype):
+    """Whatever the cache is held in: the first branch comes between two steps."""
+    import types
+
+    from pytriton_llama_amd import ops
+
+    class Asked(Exception):
+        pass
+
+    def require(names):
+        raise Asked(tuple(names))
+    monkeypatch.setattr(ops.library, "require", require)
+    model = types.SimpleNamespace(dtype=torch.bfloat16, device=torch.device("cuda"), kernel_libraries=lambda: ("norm",))
+    with pytest.raises(Asked) as asked:
+        ModelRunner(model, 16, 4, 2, cache_dtype=cache_dtype)
+    assert "cache_f8" in asked.value.args[0] and ("attention_f8" in asked.value.args[0]) == (cache_dtype is not None)
