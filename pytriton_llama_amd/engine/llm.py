@@ -206,7 +206,7 @@ class Engine:
             raise ValueError(f"request {request_id!r} has no log-probabilities of the {n} tokens its branch starts with")
         branches = []
         for p in params:
-            b = Request(self._new_id(), req.prompt_array, p, req.output[:n], req.output_logprobs[:n])
+            b = Request(self._new_id(), req.prompt_array, p, req.output[:n], req.output_logprobs[:n] if p.logprobs else [])
             self.scheduler.check(b)
             branches.append(b)
         # every branch computes one token at least, the one whose logits it samples from

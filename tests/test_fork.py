@@ -1,4 +1,5 @@
 """Requests that branch: who holds which page, on the CPU. And which models hold their cache in 8 bits."""
+import itertools
 import random
 
 import pytest
@@ -7,6 +8,7 @@ import torch
 from pytriton_llama_amd.cache import RELEASED, CacheManager, CannotShare, OutOfPages, OutOfSlots
 from pytriton_llama_amd.cache.storage import CacheStorage
 from pytriton_llama_amd.config import EngineConfig, build_model
+from pytriton_llama_amd.engine.llm import Engine
 from pytriton_llama_amd.engine.request import Request, SamplingParams
 from pytriton_llama_amd.engine.runner import ModelRunner
 from pytriton_llama_amd.engine.scheduler import Scheduler
@@ -265,3 +267,57 @@ def test_the_kernel_that_copies_pages_is_loaded_with_the_model(monkeypatch, cach
     with pytest.raises(Asked) as asked:
         ModelRunner(model, 16, 4, 2, cache_dtype=cache_dtype)
     assert "cache_f8" in asked.value.args[0] and ("attention_f8" in asked.value.args[0]) == (cache_dtype is not None)
+
+
+# ---- the engine's part ---------------------------------------------------------------------------
+class HostEngine(Engine):
+    """The engine's requests, scheduler, cache manager and branches; a step is its book-keeping alone. ``computed``: how many rows
+    each step computed of what request at what position; a token is a rule of what comes before it and the request's seed."""
+
+    def __init__(self, specs=(FULL,), page=4, pages=400, seqs=8, budget=4096, eos=(), **more):
+        self.scheduler = Scheduler(CacheManager(list(specs), page, pages, seqs), seqs, budget, eos_token_ids=eos, **more)
+        self.manager, self.copies = self.scheduler.manager, Copies()
+        self.runner = host_runner(self.manager, self.copies)
+        self.requests, self._ids, self._inflight = {}, itertools.count(), None
+        self.computed = []
+
+    def add_request(self, prompt, params=None, request_id=None):
+        rid = self._new_id()
+        req = self.requests[rid] = Request(rid, prompt, params or SamplingParams())
+        self.scheduler.add(req)
+        return rid
+
+    def step(self):
+        plan, sampled = self.scheduler.schedule(), {}
+        for e in plan.entries:
+            r = e.request
+            if not self.manager.is_live(r.id):
+                self.manager.admit(r.id)
+            assert self.manager.append(r.id, e.num_tokens) == e.start
+            self.computed += [(r.id, p) for p in range(e.start, e.start + e.num_tokens)]
+            if e.samples:
+                sampled[r.id] = hash((tuple(r.tokens), r.params.seed)) % 1000
+        for e in plan.entries:
+            self.manager.release_behind_window(e.request.id)
+        outs = self.scheduler.update(plan, sampled)
+        for o in outs:
+            if self.requests[o.request].params.logprobs:
+                self.requests[o.request].output_logprobs.append(-1.0)
+        self.manager.check()
+        return outs
+
+    def all_back(self):
+        assert not self.has_work and not self.requests and self.manager.num_free_slots == self.manager.max_num_seqs
+        assert all(g.pool.num_free == g.pool.num_pages for g in self.manager.paged)
+
+
+def test_a_branch_without_log_probabilities_has_none_of_its_request():
+    e = HostEngine()
+    rid = e.add_request(range(9), SamplingParams(max_new_tokens=8, logprobs=True))
+    for _ in range(3):
+        e.step()
+    with_them, without = e.fork(rid, [SamplingParams(max_new_tokens=6, logprobs=True), SamplingParams(max_new_tokens=6)], 2)
+    reqs = [e.requests[r] for r in (rid, with_them, without)]
+    while e.has_work:
+        e.step()
+    assert [len(r.output_logprobs) for r in reqs] == [8, 6, 0] and [len(r.output) for r in reqs] == [8, 6, 6]
