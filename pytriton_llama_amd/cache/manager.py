@@ -7,7 +7,8 @@ gives them back when the whole batch is done
 Here the unit is a page of ``page_size`` tokens, pages are taken when a request's
 tokens need them and go back on the free list when the request ends or, for a
 group whose queries read a window or a chunk of the positions, when every later query has moved
-past them. Requests that branch from one another share the full pages they have in common (``fork``). All of it is
+past them. Requests that branch from one another share the full pages they have in common (``fork``); one that waits for
+a state slot may have its pages already (it is *parked*). All of it is
 host-side bookkeeping: no device call, no synchronisation.
 
 Cache layers with the same needs form a group; a group has a page pool and, for
@@ -156,18 +157,24 @@ class CacheManager:
     def is_live(self, req) -> bool:
         return req in self.slot_of
 
+    def is_parked(self, req) -> bool:
+        """Whether ``req`` has pages and no state slot."""
+        return req in self.num_tokens and req not in self.slot_of
+
     @property
     def num_free_slots(self) -> int:
         return len(self._free_slots)
 
     def admit(self, req) -> int:
-        """Give ``req`` a state slot and empty block tables."""
+        """Give ``req`` a state slot and empty block tables (a parked one keeps those it has)."""
         if req in self.slot_of:
             raise RuntimeError(f"request {req!r} is already live")
         if not self._free_slots:
             raise OutOfSlots(f"all {self.max_num_seqs} state slots are taken")
         slot = self._free_slots.pop()
         self.slot_of[req] = slot
+        if req in self.num_tokens:
+            return slot
         self.num_tokens[req] = 0
         for g in self.paged:
             g.tables[req] = []
@@ -206,17 +213,18 @@ class CacheManager:
         self.num_tokens[req] = start + n_new
         return start
 
-    def fork(self, req, new, num_tokens: Optional[int] = None) -> List[Tuple[int, int, int]]:
-        """Make ``new`` a live request that has what ``req`` has in the cache, its first ``num_tokens``
+    def fork(self, req, new, num_tokens: Optional[int] = None, parked: bool = False) -> List[Tuple[int, int, int]]:
+        """Make ``new`` a live request that has what ``req`` (live or parked) has in the cache, its first ``num_tokens``
         tokens (None: all). Full pages are shared: nobody writes them again, and each is free once
         both have given it back. A last page that is not full is the new request's own: returns the
         copies to be made, (group, page to read, page to write). A state slot is taken; where the
-        model has state, the caller copies it (all tokens only). Changes nothing where it raises:
+        model has state, the caller copies it (all tokens only). ``parked``: without a slot, which ``admit``
+        gives it later (not for models with state, which lies in the slot). Changes nothing where it raises:
         CannotShare if pages the new request will read are gone, or state is asked for that was, OutOfPages,
         OutOfSlots."""
-        if req not in self.slot_of:
+        if req not in self.num_tokens:
             raise RuntimeError(f"request {req!r} is not live")
-        if new in self.slot_of:
+        if new in self.num_tokens:
             raise RuntimeError(f"request {new!r} is already live")
         have = self.num_tokens[req]
         n = have if num_tokens is None else int(num_tokens)
@@ -224,7 +232,9 @@ class CacheManager:
             raise ValueError(f"request {req!r} has {have} tokens in the cache, {n} wanted")
         if self.states and n != have:
             raise CannotShare(f"the state of request {req!r} is that of {have} tokens, not of {n}")
-        if not self._free_slots:
+        if self.states and parked:
+            raise CannotShare(f"request {new!r} has no place for state without a slot")
+        if not parked and not self._free_slots:
             raise OutOfSlots(f"all {self.max_num_seqs} state slots are taken")
         full, rest = divmod(n, self.page_size)
         for g in self.paged:
@@ -235,7 +245,8 @@ class CacheManager:
                 raise CannotShare(f"request {req!r} has given back pages that {n} tokens need")
             if rest and not g.pool.num_free:
                 raise OutOfPages(f"request {new!r} needs a page of {g.spec} for what it does not share")
-        self.slot_of[new] = self._free_slots.pop()
+        if not parked:
+            self.slot_of[new] = self._free_slots.pop()
         self.num_tokens[new] = n
         copies = []
         for gi, g in enumerate(self.paged):
@@ -287,12 +298,13 @@ class CacheManager:
         return n
 
     def free(self, req) -> None:
-        """The request is over: its pages and its slot go back."""
-        if req not in self.slot_of:
+        """The request is over: its pages and its slot, if it has one, go back."""
+        if req not in self.num_tokens:
             raise RuntimeError(f"request {req!r} is not live (freed twice?)")
         for g in self.paged:
             g.pool.give_back([p for p in g.tables.pop(req) if p >= 0])
-        self._free_slots.append(self.slot_of.pop(req))
+        if req in self.slot_of:
+            self._free_slots.append(self.slot_of.pop(req))
         del self.num_tokens[req]
 
     def block_table(self, req, group: int) -> List[int]:
@@ -323,6 +335,8 @@ class CacheManager:
                                      f"!= {g.pool.num_pages} pages")
             if len(set(g.pool._free)) != len(g.pool._free):
                 raise AssertionError(f"group {gi}: a page is on the free list twice")
+        if not set(self.slot_of) <= set(self.num_tokens) or any(set(g.tables) != set(self.num_tokens) for g in self.paged):
+            raise AssertionError("requests with a slot, with tokens and with block tables are not the same")
         slots = list(self.slot_of.values())
         if len(set(slots)) != len(slots) or set(slots) & set(self._free_slots) \
                 or len(slots) + len(self._free_slots) != self.max_num_seqs:

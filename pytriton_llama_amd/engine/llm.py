@@ -9,7 +9,7 @@ from typing import Dict, Hashable, Iterator, List, Optional, Sequence, Union
 import numpy as np
 import torch
 
-from ..cache import CacheManager, CacheStorage, CannotShare, OutOfPages, OutOfSlots
+from ..cache import CacheManager, CacheStorage
 from ..config import EngineConfig, build_model, read_config_json
 from ..sampling import Sampler
 from ..weights import load_random_weights, load_weights
@@ -183,8 +183,10 @@ class Engine:
         the first ``num_output`` tokens of its output (None: all it has), each by itself. ``params``: theirs
         (one, or one each; None: the request's own); max_new_tokens counts the output they start
         with. A branch draws numbers of its own unless its params name a seed: one that shares the seed
-        repeats the request. What the request has in the cache is shared where that is possible
-        (CacheManager.fork) and there is room to run; otherwise the branch waits and is computed from its tokens,
+        repeats the request. What the request has in the cache is shared by as many branches as there are
+        pages for, if it can be (CacheManager.fork: a window may have passed by pages that a branch needs, and the state of models
+        that have one is there behind the last token of the last step that was launched only, not of earlier ones); those that
+        no place is free for wait with their share. A branch that gets none waits too and is computed from its tokens,
         like a preempted request. (A page in 8 bits that is copied keeps the scale of all it held, later tokens of the
         request's too: numbers below 2^-14 of the page's largest may be rounded otherwise than in a run by itself.)
         Returns the new requests' ids."""
@@ -211,21 +213,16 @@ class Engine:
             branches.append(b)
         # every branch computes one token at least, the one whose logits it samples from
         share = min(req.num_computed, len(req.prompt) + n - 1)
-        shared = False
-        if share > 0 and self.runner.manager.is_live(request_id) \
-                and len(self.scheduler.running) + count <= self.scheduler.max_num_seqs:
-            try:
-                self.runner.fork(request_id, [b.id for b in branches], share)
-                shared = True
-            except (CannotShare, OutOfPages, OutOfSlots):
-                pass
-        if shared:
-            for b in branches:
-                b.num_computed = share
-            self.scheduler.adopt(branches)
-        else:
-            for b in branches:
-                self.scheduler.add(b)
+        places = max(0, self.scheduler.max_num_seqs - len(self.scheduler.running))
+        made = 0
+        if share > 0 and (self.runner.manager.is_live(request_id) or self.runner.manager.is_parked(request_id)):
+            made = self.runner.fork(request_id, [b.id for b in branches], share, places)
+        for b in branches[:made]:
+            b.num_computed = share
+        self.scheduler.adopt(branches[:min(made, places)])
+        self.scheduler.park(branches[places:made])
+        for b in branches[made:]:
+            self.scheduler.add(b)
         for b in branches:
             self.requests[b.id] = b
         return [b.id for b in branches]

@@ -7,7 +7,7 @@ from typing import Hashable, List, Optional, Sequence
 import torch
 
 from .. import ops
-from ..cache import CacheManager, CacheStorage
+from ..cache import CacheManager, CacheStorage, CannotShare, OutOfPages, OutOfSlots
 from .batch import StepEntry, build_context
 
 
@@ -78,26 +78,35 @@ class ModelRunner:
         return logits
 
     @torch.inference_mode()
-    def fork(self, request: Hashable, new: Sequence[Hashable], num_tokens: Optional[int] = None) -> None:
-        """Admit the requests ``new`` with what ``request`` has in the cache, its first ``num_tokens``
-        tokens (None: all): full pages are shared, the last one and the state copied, on the device and
-        behind the steps launched so far. All of them or, where this raises (as CacheManager.fork), none."""
+    def fork(self, request: Hashable, new: Sequence[Hashable], num_tokens: Optional[int] = None,
+             slots: Optional[int] = None) -> int:
+        """Give the requests ``new`` what ``request`` has in the cache, its first ``num_tokens`` tokens (None:
+        all): full pages are shared, the last one and the state copied, on the device and behind the steps
+        launched so far. The first ``slots`` of them (None: all) are live then, the others parked. Returns how many
+        there was room for, from the first on (see CacheManager.fork); where a copy fails it raises, and none has
+        anything."""
         copies: List[tuple] = []
         made: List[Hashable] = []
         try:
-            for n in new:
-                copies += self.manager.fork(request, n, num_tokens)
+            for i, n in enumerate(new):
+                try:
+                    copies += self.manager.fork(request, n, num_tokens, parked=slots is not None and i >= slots)
+                except (CannotShare, OutOfPages, OutOfSlots):
+                    break
                 made.append(n)
             for g in range(len(self.manager.paged)):
                 self.storage.copy_pages(g, [s for h, s, _ in copies if h == g], [d for h, _, d in copies if h == g])
+            slot_of = self.manager.slot_of
             for n in made:
-                self.storage.copy_slot(self.manager.slot_of[request], self.manager.slot_of[n])
+                if n in slot_of and request in slot_of:           # (parked ones are of models without state)
+                    self.storage.copy_slot(slot_of[request], slot_of[n])
         except Exception:
             for n in made:
                 self.manager.free(n)
             raise
+        return len(made)
 
     def end(self, request: Hashable) -> None:
         """The request is finished: what it holds is given back."""
-        if self.manager.is_live(request):
+        if self.manager.is_live(request) or self.manager.is_parked(request):
             self.manager.free(request)

@@ -12,7 +12,10 @@ step it decides which requests run how many tokens:
   steps and shares them with decodes;
 * waiting requests are admitted in order of arrival while a state slot, a place
   in the batch and the pages of their first portion are there;
-* when a running request cannot get the page it needs, the most recently
+* a branch of another request may wait with what it shares of that one's pages; while pages
+  are short, such waiting requests lose theirs first, the last one first, and are computed from
+  their tokens;
+* when a running request still cannot get the page it needs, the most recently
   admitted running request is preempted: its pages and slot are given back, it
   returns to the front of the waiting queue and is computed again from its
   prompt plus the tokens it had generated (which are kept). If the request in
@@ -94,11 +97,38 @@ class Scheduler:
             req.status = RUNNING
             self.running.append(req)
 
+    def park(self, reqs: Sequence[Request]) -> None:
+        """Take over branches that have pages but no slot yet: they wait in order of arrival, with what they have."""
+        for req in reqs:
+            self.check(req)
+            if not self.manager.is_parked(req.id) or not 0 < req.num_computed < req.num_tokens:
+                raise ValueError(f"request {req.id!r} is not a branch that waits with its pages")
+        for req in reqs:
+            req.status = WAITING
+            self.waiting.append(req)
+
     @property
     def has_work(self) -> bool:
         return bool(self.waiting or self.running)
 
     # ---- planning one step -------------------------------------------------------
+    def _take_parked(self, but: Optional[Request] = None) -> bool:
+        """Give back the pages of the last request that waits with some; False when there is none (beside ``but``)."""
+        for req in reversed(self.waiting):
+            if req is not but and self.manager.is_parked(req.id):
+                self.manager.free(req.id)
+                req.num_computed = 0
+                return True
+        return False
+
+    def _parked_may_do(self, req: Request, n: int, reserve: Sequence[int]) -> bool:
+        """Whether n tokens of ``req`` could get their pages if all who wait with some gave them back (by the lengths of their tables:
+        what they share with running requests would not be free)."""
+        parked = [r.id for r in self.waiting if r is not req and self.manager.is_parked(r.id)]
+        return bool(parked) and all(
+            need + kept <= g.pool.num_free + sum(len(g.tables[r]) for r in parked)
+            for g, need, kept in zip(self.manager.paged, self.manager.pages_needed(req.id, n), reserve))
+
     def _preempt(self, victim: Request, plan: StepPlan, reserve: List[int]) -> None:
         for e in list(plan.entries):
             if e.request is victim:
@@ -119,6 +149,8 @@ class Scheduler:
         """Plan n tokens of a running request, preempting later arrivals while
         pages are short. False when the request itself had to give way."""
         while not self.manager.can_append(req.id, n, reserve):
+            if self._take_parked():
+                continue
             victim = self.running[-1]
             self._preempt(victim, plan, reserve)
             if victim is req:
@@ -152,7 +184,11 @@ class Scheduler:
             if req in plan.preempted:
                 break                           # just preempted: it waits at least one step
             n = min(req.remaining, self.prefill_chunk, budget)
-            if not self.manager.can_append(req.id, n, reserve):
+            fits = self.manager.can_append(req.id, n, reserve)
+            if not fits and self._parked_may_do(req, n, reserve):
+                while not fits and self._take_parked(but=req):
+                    fits = self.manager.can_append(req.id, n, reserve)
+            if not fits:
                 break
             self.waiting.popleft()
             req.status = RUNNING
@@ -230,5 +266,7 @@ class Scheduler:
                 self.manager.free(req.id)
         elif req in self.waiting:
             self.waiting.remove(req)
+            if self.manager.is_parked(req.id):
+                self.manager.free(req.id)
         req.status = FINISHED
         req.finish_reason = "aborted"

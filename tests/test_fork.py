@@ -321,3 +321,155 @@ def test_a_branch_without_log_probabilities_has_none_of_its_request():
     while e.has_work:
         e.step()
     assert [len(r.output_logprobs) for r in reqs] == [8, 6, 0] and [len(r.output) for r in reqs] == [8, 6, 6]
+
+
+def prompt_rows(e, length, but=None):
+    """Rows computed at positions of the prompt that are before its last (not those of request ``but``)."""
+    return sum(p < length - 1 for r, p in e.computed if r != but)
+
+
+@pytest.mark.parametrize("count", [1, 6, 7, 8, 30])
+def test_branches_beyond_the_places_keep_their_share(count):
+    """Eight places, two of them taken: whatever the number of branches, the prompt is computed once."""
+    e = HostEngine()
+    other = e.add_request(range(5), SamplingParams(max_new_tokens=40))
+    rid = e.add_request(range(101), SamplingParams(max_new_tokens=9))
+    for _ in range(3):
+        e.step()
+    made = e.fork(rid, SamplingParams(max_new_tokens=9), count)
+    reqs = [e.requests[r] for r in [rid] + made]
+    assert sum(r.status == "running" for r in reqs[1:]) == min(count, 6)
+    assert all(r.num_computed == reqs[0].num_computed for r in reqs)
+    more = e.fork(made[-1], SamplingParams(max_new_tokens=5), 2, num_output=0)      # (of one that may itself be waiting)
+    e.manager.check()
+    e.abort(made[0])
+    while e.has_work:
+        e.step()
+    assert prompt_rows(e, 101, but=other) == 100
+    assert all(len(r.output) == 9 for r in reqs[:1] + reqs[2:]) and len(e.requests[other].output) == 40
+    assert [len(e.requests[r].output) for r in more] == [5, 5]
+    e.requests.clear()
+    e.all_back()
+
+
+def test_waiting_branches_give_way_to_whom_runs():
+    """Too few pages for all that wait: running requests are not preempted for them, an earlier request that waits gets in, and
+    the branches are computed from their tokens then."""
+    e = HostEngine(pages=16, seqs=2)
+    rid = e.add_request(range(22), SamplingParams(max_new_tokens=18))          # (6 pages, 10 at its end)
+    e.step()
+    made = e.fork(rid, SamplingParams(max_new_tokens=18), 6, num_output=0)     # (a page more each)
+    assert [e.requests[r].status for r in made] == ["running"] + ["waiting"] * 5
+    assert e.manager.paged[0].pool.num_free == 16 - 6 - 6
+    late = e.add_request(range(3), SamplingParams(max_new_tokens=2))
+    reqs = [e.requests[r] for r in [rid] + made + [late]]
+    while reqs[0].status != "finished":
+        e.step()
+    assert reqs[0].num_preemptions == reqs[1].num_preemptions == 0
+    while e.has_work:
+        e.step()
+    assert [len(r.output) for r in reqs] == [18] * 7 + [2]
+    e.requests.clear()
+    e.all_back()
+
+
+def test_a_request_ahead_of_waiting_branches_gets_their_pages():
+    e = HostEngine(pages=12, seqs=2)
+    rid = e.add_request(range(10), SamplingParams(max_new_tokens=6))           # (3 pages; a page more for a branch)
+    e.step()
+    first = e.add_request(range(30), SamplingParams(max_new_tokens=4))         # (8 pages)
+    made = e.fork(rid, SamplingParams(max_new_tokens=6), 6, num_output=0)
+    for r in made[1:]:
+        assert e.manager.is_parked(r)
+    e.abort(made[0])
+    reqs = [e.requests[r] for r in [rid, first] + made[1:]]
+    e.step()
+    assert reqs[1].status == "running" and not e.manager.is_parked(made[-1])
+    while e.has_work:
+        e.step()
+    assert [len(r.output) for r in reqs] == [6, 4] + [6] * 5
+    e.requests.clear()
+    e.all_back()
+
+
+def test_waiting_branches_keep_their_pages_where_those_would_not_do():
+    e = HostEngine(pages=30, seqs=3)
+    running = e.add_request(range(60), SamplingParams(max_new_tokens=20))      # (15 pages to begin with)
+    rid = e.add_request(range(10), SamplingParams(max_new_tokens=20))          # (3)
+    e.step()
+    filler = e.add_request(range(4), SamplingParams(max_new_tokens=3))
+    e.step()
+    large = e.add_request(range(99), SamplingParams(max_new_tokens=2))         # (25: not while the others run)
+    made = e.fork(rid, SamplingParams(max_new_tokens=20), 4, num_output=0)
+    while e.requests[filler].status != "finished":
+        e.step()
+    for _ in range(3):
+        e.step()
+    assert e.requests[large].status == "waiting" and all(e.manager.is_parked(r) for r in made)
+    reqs = [e.requests[r] for r in [running, rid, filler, large] + made]
+    while e.has_work:
+        e.step()
+    assert [len(r.output) for r in reqs] == [20, 20, 3, 2] + [20] * 4
+    e.requests.clear()
+    e.all_back()
+
+
+def test_parked_requests_of_the_manager():
+    m = CacheManager([FULL], page_size=4, num_pages=9, max_num_seqs=1)
+    live(m, "a", 9)
+    with pytest.raises(OutOfSlots):
+        m.fork("a", "b")
+    m.fork("a", "b", parked=True)
+    m.fork("b", "c", 8, parked=True)
+    assert m.is_parked("b") and not m.is_live("b") and not m.is_parked("a") and not m.is_parked("x")
+    m.check()
+    with pytest.raises(OutOfSlots):
+        m.admit("b")
+    m.free("a")
+    m.admit("b")
+    assert m.is_live("b") and m.num_tokens["b"] == 9 and m.append("b", 2) == 9
+    m.check()
+    for name in "bc":
+        m.free(name)
+    assert m.paged[0].pool.num_free == 9
+    with pytest.raises(RuntimeError):
+        m.free("c")
+    m.check()
+    s = CacheManager([FULL, StateSpec((3,))], page_size=4, num_pages=8, max_num_seqs=3)
+    live(s, "a", 9)
+    with pytest.raises(CannotShare):
+        s.fork("a", "b", parked=True)
+    s.check()
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_branches_in_random_order(seed):
+    """Requests come, branch and are aborted, with few places and too few pages for all: every page is held by whom it is counted
+    for (checked after every step), all end with their tokens."""
+    rng = random.Random(seed)
+    e = HostEngine(page=rng.choice([1, 3, 8]), pages=60 if seed % 2 else 200, seqs=rng.randint(1, 5), budget=rng.choice([7, 64]), max_model_len=60)
+    live_ones = {}
+    for _ in range(300):
+        act = rng.random()
+        if act < 0.2 and len(live_ones) < 12:
+            rid = e.add_request([rng.randrange(100) for _ in range(rng.randint(1, 30))], SamplingParams(max_new_tokens=rng.randint(1, 24)))
+            live_ones[rid] = e.requests[rid]
+        elif act < 0.4 and live_ones:
+            r = live_ones[rng.choice(sorted(live_ones))]
+            n = rng.randint(0, len(r.output))
+            if r.status != "finished" and n < r.params.max_new_tokens and len(live_ones) < 20:
+                for b in e.fork(r.id, count=rng.randint(1, 4), num_output=n):
+                    live_ones[b] = e.requests[b]
+        elif act < 0.5 and live_ones:
+            rid = rng.choice(sorted(live_ones))
+            e.abort(rid)
+            del live_ones[rid]
+        elif e.has_work:
+            e.step()
+        e.manager.check()
+    while e.has_work:
+        e.step()
+    for r in live_ones.values():
+        assert r.status == "finished" and len(r.output) == r.params.max_new_tokens
+    e.requests.clear()
+    e.all_back()
