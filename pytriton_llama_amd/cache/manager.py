@@ -297,6 +297,12 @@ class CacheManager:
                 n += len(dead)
         return n
 
+    def park(self, req) -> None:
+        """Take the state slot of a live request, which keeps its pages (what state it had is gone)."""
+        if req not in self.slot_of:
+            raise RuntimeError(f"request {req!r} is not live")
+        self._free_slots.append(self.slot_of.pop(req))
+
     def free(self, req) -> None:
         """The request is over: its pages and its slot, if it has one, go back."""
         if req not in self.num_tokens:

@@ -195,6 +195,11 @@ class Engine:
             raise ValueError(f"request {request_id!r} is not one that can branch")
         if count < 1:
             raise ValueError("a request branches into one more at least")
+        return self._branch(req, params, count, num_output)
+
+    def _branch(self, req: Request, params, count: int, num_output: Optional[int]) -> List[Hashable]:
+        """``fork``, also of a request that is finished (and shares then if it kept its pages)."""
+        request_id = req.id
         n = len(req.output) if num_output is None else int(num_output)
         if not 0 <= n <= len(req.output):
             raise ValueError(f"request {request_id!r} has {len(req.output)} tokens of output, {n} wanted")
@@ -355,29 +360,37 @@ class Engine:
     def generate_samples(self, prompts: Sequence[Sequence[int]], count: int,
                          params: Union[SamplingParams, Sequence[SamplingParams], None] = None) -> List[List[Request]]:
         """``count`` finished requests for every prompt, each with tokens drawn by itself. A prompt is
-        computed once: when its first request has its first token the others branch off behind the
+        computed once, as long as there are pages for those that wait: when its first request has its first token
+        the others branch off behind the
         prompt. With a seed in a prompt's params its requests draw by seed, seed + 1, ..."""
         if count < 1:
             raise ValueError("one sample at least")
         ids = self._add_all(prompts, params)
         groups = {rid: [rid] for rid in ids}
-        waiting = set(ids) if count > 1 else set()
-        ended: Dict[Hashable, List[SamplingParams]] = {}
-        while self.has_work or ended:
-            for rid, each in ended.items():           # (its only token ended it: the prompt is computed again)
-                groups[rid] += [self.add_request(self.requests[rid].prompt_array, p) for p in each]
-            ended.clear()
-            for o in self.step():
-                if o.request not in waiting:
-                    continue
-                waiting.discard(o.request)
-                req = self.requests[o.request]
-                seed = req.params.seed
-                each = [dataclasses.replace(req.params, seed=None if seed is None else seed + i) for i in range(1, count)]
-                if req.status == FINISHED:
-                    ended[o.request] = each
-                else:
-                    groups[o.request] += self.fork(o.request, each, count - 1, num_output=0)
+        waiting = {rid: self.requests[rid] for rid in ids} if count > 1 else {}
+        manager = self.runner.manager
+
+        def branched(req):
+            req.keeps_pages = False
+            if req.status == FINISHED and manager.is_parked(req.id):
+                manager.free(req.id)
+        for req in waiting.values():
+            req.keeps_pages = True                    # (its only token may end it)
+        try:
+            while self.has_work:
+                for o in self.step():
+                    req = waiting.pop(o.request, None)
+                    if req is None:
+                        continue
+                    try:
+                        seed = req.params.seed
+                        each = [dataclasses.replace(req.params, seed=None if seed is None else seed + i) for i in range(1, count)]
+                        groups[o.request] += self._branch(req, each, count - 1, 0)
+                    finally:
+                        branched(req)
+        finally:
+            for req in waiting.values():
+                branched(req)
         return [[self.requests.pop(r) for r in groups[rid]] for rid in ids]
 
     def generate_stream(self, prompts, params=None) -> Iterator[List[StepOutput]]:

@@ -43,6 +43,7 @@ class Request:
     status: str = WAITING
     finish_reason: Optional[str] = None
     num_preemptions: int = 0
+    keeps_pages: bool = False         # its pages are not given back when it is finished: who set this does that
 
     def __post_init__(self):
         # the prompt as a list and as an array: portions of it go to the step without a conversion

@@ -232,7 +232,8 @@ class Scheduler:
     # ---- after the step ------------------------------------------------------------
     def update(self, plan: StepPlan, sampled: Dict[Hashable, int]) -> List[StepOutput]:
         """Record what the step computed; ``sampled`` maps the id of every entry
-        that samples to its new token. Finished requests give back what they hold."""
+        that samples to its new token. Finished requests give back what they hold (but for pages that
+        they were told to keep)."""
         outs: List[StepOutput] = []
         for e in plan.entries:
             req = e.request
@@ -255,7 +256,10 @@ class Scheduler:
                 req.finish_reason = reason
                 self.running.remove(req)
                 if self.manager.is_live(req.id):
-                    self.manager.free(req.id)
+                    if req.keeps_pages:
+                        self.manager.park(req.id)
+                    else:
+                        self.manager.free(req.id)
             outs.append(StepOutput(req.id, tok, reason is not None, reason))
         return outs
 

@@ -473,3 +473,61 @@ def test_branches_in_random_order(seed):
         assert r.status == "finished" and len(r.output) == r.params.max_new_tokens
     e.requests.clear()
     e.all_back()
+
+
+# ---- samples -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("new", [1, 7])
+@pytest.mark.parametrize("count", [1, 2, 8, 9, 16, 40])
+def test_samples_compute_a_prompt_once(count, new):
+    e = HostEngine(pages=600)
+    group = e.generate_samples([range(1000)], count, SamplingParams(max_new_tokens=new, seed=4))[0]
+    assert prompt_rows(e, 1000) == 999
+    assert [len(r.output) for r in group] == [new] * count and [r.params.seed for r in group] == [4 + i for i in range(count)]
+    assert all(r.output == HostEngine(pages=600).generate([range(1000)], r.params)[0] for r in group[:3])
+    e.all_back()
+
+
+@pytest.mark.parametrize("prompts,count,seqs", [(64, 4, 64), (10, 3, 4), (5, 5, 1)])
+def test_samples_of_many_prompts_compute_each_once(prompts, count, seqs):
+    e = HostEngine(pages=4000, seqs=seqs)
+    lengths = [17 + 3 * i for i in range(prompts)]
+    groups = e.generate_samples([range(n) for n in lengths], count, SamplingParams(max_new_tokens=5, seed=1))
+    firsts = {g[0].id: n for g, n in zip(groups, lengths)}
+    owner = {r.id: g[0].id for g in groups for r in g}
+    assert sum(p < firsts[owner[r]] - 1 for r, p in e.computed) == sum(n - 1 for n in lengths)
+    assert all(len(g) == count and all(len(r.output) == 5 for r in g) for g in groups)
+    e.all_back()
+
+
+def test_samples_that_their_first_token_may_end():
+    """Some prompts' first request ends with its first token, others not; too few pages for all that wait."""
+    for eos in (range(0, 1000, 3), range(1000)):
+        e = HostEngine(pages=14, seqs=2, eos=tuple(eos), budget=9)
+        groups = e.generate_samples([range(n) for n in (1, 4, 21, 5, 30)], 4, SamplingParams(max_new_tokens=6, seed=3))
+        for group in groups:
+            for r in group:
+                assert r.output == HostEngine(eos=tuple(eos)).generate([r.prompt], r.params)[0]
+        e.all_back()
+
+
+def test_samples_that_are_interrupted_hold_nothing_for_good():
+    class Stop(Exception):
+        pass
+    for when in range(1, 6):
+        e = HostEngine(pages=60, seqs=3)
+        real, calls = e.step, []
+
+        def step():
+            calls.append(1)
+            if len(calls) == when:
+                raise Stop
+            return real()
+        e.step = step
+        with pytest.raises(Stop):
+            e.generate_samples([range(9), range(14), range(6), range(3)], 3, SamplingParams(max_new_tokens=2))
+        e.step = real
+        while e.has_work:
+            e.step()
+        assert not any(r.keeps_pages for r in e.requests.values())
+        e.requests.clear()
+        e.all_back()
