@@ -153,6 +153,12 @@ class CacheManager:
         self.slot_of: Dict[Hashable, int] = {}
         self.num_tokens: Dict[Hashable, int] = {}
 
+    @property
+    def only_goes_on(self) -> bool:
+        """Whether what a request has can be shared as it is only, not what it had some tokens before: there is state, or
+        pages are given back."""
+        return bool(self.states) or any(g.spec.gives_back for g in self.paged)
+
     # ---- requests ------------------------------------------------------------
     def is_live(self, req) -> bool:
         return req in self.slot_of

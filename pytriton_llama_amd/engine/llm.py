@@ -362,7 +362,9 @@ class Engine:
         """``count`` finished requests for every prompt, each with tokens drawn by itself. A prompt is
         computed once, as long as there are pages for those that wait: when its first request has its first token
         the others branch off behind the
-        prompt. With a seed in a prompt's params its requests draw by seed, seed + 1, ..."""
+        prompt; where the model has state or a window, when all of the prompt but its last token has been computed (with
+        state, one that finds no free place then computes the prompt itself). With a seed in a prompt's params its requests
+        draw by seed, seed + 1, ..."""
         if count < 1:
             raise ValueError("one sample at least")
         ids = self._add_all(prompts, params)
@@ -371,21 +373,23 @@ class Engine:
         manager = self.runner.manager
 
         def branched(req):
-            req.keeps_pages = False
+            req.keeps_pages, req.stops_at = False, None
             if req.status == FINISHED and manager.is_parked(req.id):
                 manager.free(req.id)
         for req in waiting.values():
             req.keeps_pages = True                    # (its only token may end it)
+            if manager.only_goes_on and len(req.prompt) > 1:
+                req.stops_at = len(req.prompt) - 1
         try:
             while self.has_work:
-                for o in self.step():
-                    req = waiting.pop(o.request, None)
-                    if req is None:
-                        continue
+                self.step()
+                for rid in [r for r, req in waiting.items()
+                            if req.output or (req.stops_at is not None and req.num_computed == req.stops_at)]:
+                    req = waiting.pop(rid)
                     try:
                         seed = req.params.seed
                         each = [dataclasses.replace(req.params, seed=None if seed is None else seed + i) for i in range(1, count)]
-                        groups[o.request] += self._branch(req, each, count - 1, 0)
+                        groups[rid] += self._branch(req, each, count - 1, 0)
                     finally:
                         branched(req)
         finally:

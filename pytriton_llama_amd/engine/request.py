@@ -43,6 +43,7 @@ class Request:
     status: str = WAITING
     finish_reason: Optional[str] = None
     num_preemptions: int = 0
+    stops_at: Optional[int] = None    # so many tokens are run through the model and no more until this is None again
     keeps_pages: bool = False         # its pages are not given back when it is finished: who set this does that
 
     def __post_init__(self):
@@ -71,8 +72,9 @@ class Request:
 
     @property
     def remaining(self) -> int:
-        """Tokens not yet run through the model."""
-        return self.num_tokens - self.num_computed
+        """Tokens not yet run through the model (that are to be)."""
+        n = self.num_tokens if self.stops_at is None else min(self.num_tokens, self.stops_at)
+        return n - self.num_computed
 
 
 @dataclass

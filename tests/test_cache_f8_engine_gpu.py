@@ -329,6 +329,63 @@ def test_a_model_with_state_branches_at_its_end_only(tmp_path_factory, gpu_devic
     assert [r.output for r in reqs] == [want] * 3
 
 
+def test_samples_of_a_model_with_state(gpu_device):
+    """With steps launched ahead and recorded, as by default: the prompt is computed once, its state copied for each branch; a
+    request that branches while it decodes is a token further in its state than in its output, and its branches are computed anew."""
+    import virusun_configs
+    from pytriton_llama_amd.config import EngineConfig
+    from pytriton_llama_amd.engine import Engine, SamplingParams
+    cfg = next(iter(virusun_configs.VIRUSUN.values()))[0]
+    e = Engine(cfg, EngineConfig(dtype="float32", page_size=8, num_pages=60, max_num_seqs=6, max_model_len=96,
+                                 timed_library_products=False), random_seed=3)
+    assert e.runner.manager.states
+    copies, seen = [], []
+    real_copy, real_step = e.runner.storage.copy_slot, e.runner.step
+    e.runner.storage.copy_slot = lambda s, d: (copies.append((s, d)), real_copy(s, d))[1]
+    e.runner.step = lambda entries, feed=None: (seen.extend(len(x.tokens) for x in entries), real_step(entries, feed))[1]
+    prompts = list(random_sequences(e.model.vocab_size, [19, 2, 33, 1], seed=1).values())
+    p = SamplingParams(temperature=0.0, max_new_tokens=8, ignore_eos=True)
+    groups = e.generate_samples(prompts[:1], 4, p) + e.generate_samples(prompts[1:], 2, p)
+    assert len(copies) == 3 + 2 and sum(n for n in seen if n > 1) == 18 + 32
+    for prompt, group in zip(prompts, groups):
+        want = e.generate([prompt], p)[0]
+        assert all(r.output == want for r in group)
+    want = e.generate(prompts[:1], p)[0]
+    rid = e.add_request(prompts[0], p)
+    for _ in range(4):
+        e.step()
+    reqs = [e.requests[r] for r in [rid] + e.fork(rid)]
+    while e.has_work:
+        e.step()
+        e.runner.manager.check()
+    assert [r.output for r in reqs] == [want] * 2
+
+
+@pytest.mark.parametrize("cache_dtype", [None, "float8_e4m3fn"])
+@pytest.mark.parametrize("graphs", [False, True])
+def test_more_samples_than_places(folders, cache_dtype, graphs):
+    """Branches that wait with their pages: the prompt is computed once, tokens are those of requests of their own."""
+    from pytriton_llama_amd.engine import SamplingParams
+    e = engine(folders["C"], cache_dtype=cache_dtype, graphs=graphs, seqs=3, pages=80)
+    prompts = list(random_sequences(300, [37, 9], seed=9).values())
+    seen = []
+    real = e.runner.step
+    e.runner.step = lambda entries, feed=None: (seen.extend(len(x.tokens) for x in entries), real(entries, feed))[1]
+    for p in (SamplingParams(temperature=0.0, max_new_tokens=7, ignore_eos=True), SamplingParams(temperature=0.0, max_new_tokens=1)):
+        seen.clear()
+        groups = e.generate_samples(prompts, 8, p)
+        assert sum(n for n in seen if n > 1) == 37 + 9
+        for prompt, group in zip(prompts, groups):
+            want = e.generate([prompt], p)[0]
+            assert all(r.output == want for r in group) and len(group) == 8
+    p = SamplingParams(temperature=0.9, max_new_tokens=9, seed=5, ignore_eos=True)
+    for prompt, group in zip(prompts, e.generate_samples(prompts, 8, p)):
+        each = [SamplingParams(temperature=0.9, max_new_tokens=9, seed=5 + i, ignore_eos=True) for i in range(8)]
+        assert [r.output for r in group] == e.generate([prompt] * 8, each)
+    e.runner.manager.check()
+    assert not e.has_work and not e.requests and e.runner.manager.paged[0].pool.num_free == 80
+
+
 def test_the_command_line(folders):
     prompt = random_sequences(300, [12], seed=8)["r0"]
     args = [sys.executable, os.path.join(ROOT, "cli.py"), "--checkpoints_dir", folders["C"], "--temperature", "0", "--max_gen_len", "6",

@@ -531,3 +531,44 @@ def test_samples_that_are_interrupted_hold_nothing_for_good():
         assert not any(r.keeps_pages for r in e.requests.values())
         e.requests.clear()
         e.all_back()
+
+
+@pytest.mark.parametrize("length", range(1, 25))
+@pytest.mark.parametrize("specs", [(FULL, WIN), (FULL, StateSpec((3,))), (WIN, StateSpec((3,)))], ids=["window", "state", "both"])
+def test_samples_of_models_that_only_go_on(specs, length):
+    """A window may have passed by the page that holds the prompt's last token but one, and state cannot go back by a token: the
+    branches are made before the prompt's last token."""
+    e = HostEngine(specs=specs, seqs=5, budget=10)
+    other = e.add_request(range(3), SamplingParams(max_new_tokens=30))
+    group = e.generate_samples([range(length)], 4, SamplingParams(max_new_tokens=6, seed=2))[0]
+    assert prompt_rows(e, length, but=other) == length - 1
+    assert len(e.copies.slots) == (3 if length > 1 else 0)
+    for r in group:
+        assert r.output == HostEngine().generate([r.prompt], r.params)[0]
+    while e.has_work:
+        e.step()
+    e.requests.clear()
+    e.all_back()
+
+
+def test_samples_with_state_beyond_the_places_compute_the_prompt_themselves():
+    e = HostEngine(specs=(FULL, StateSpec((3,))), seqs=3)
+    group = e.generate_samples([range(50)], 7, SamplingParams(max_new_tokens=4, seed=2))[0]
+    assert prompt_rows(e, 50) == 49 * 5 and len(e.copies.slots) == 2
+    for r in group:
+        assert r.output == HostEngine().generate([r.prompt], r.params)[0]
+    e.all_back()
+
+
+def test_a_request_that_stops_is_let_alone():
+    e = HostEngine(budget=4)
+    a, b = e.add_request(range(7), SamplingParams(max_new_tokens=3)), e.add_request(range(5), SamplingParams(max_new_tokens=9))
+    e.requests[a].stops_at = 6
+    for _ in range(6):
+        e.step()
+    assert e.requests[a].num_computed == 6 and not e.requests[a].output and len(e.requests[b].output) > 2
+    e.requests[a].stops_at = None
+    reqs = [e.requests[a], e.requests[b]]
+    while e.has_work:
+        e.step()
+    assert [len(r.output) for r in reqs] == [3, 9]
