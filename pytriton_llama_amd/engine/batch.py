@@ -84,6 +84,8 @@ class StepContext:
     lens_are_bounds: bool = False              # q_lens and ctx_lens are such bounds
     tickets: Optional[torch.Tensor] = None     # int32 zeros, ops.TICKET a single-token sequence and kv head: the workgroups of
                                                # a launch that share a sequence's keys count in them who is done, and leave zeros
+    block_tickets: Optional[torch.Tensor] = None   # the same for blocks of prompt rows that a launch cuts along their keys:
+                                               # made by the first layer that needs them (parts/attention.py)
     rotations: Optional[Rotations] = None      # while a model's forward runs: the cosines and sines of the rows
 
 

@@ -260,6 +260,23 @@ def attention_prefill_f8_plan(device: torch.device, num_heads: int, head_dim: in
     return rows, max(1, blocks if blocks <= 2 * t else t)
 
 
+def _cut_into(device: torch.device, num_heads: int, head_dim: int, blocks: int, groups: int, block_rows: int, table_keys: int) -> int:
+    """Parts a head that ``attention_prefill_f8`` cuts its blocks into, some; 0: it leaves them whole. table_keys: keys that a row of
+    the block table has room for."""
+    if groups != blocks or blocks > 64 or table_keys <= 64 * WORTH_TILES:
+        return 0
+    resident = _prefill_resident(device, num_heads, head_dim)
+    # (blocks of 64 rows that fill more than half of it are as fast whole, of 128 rows five sixths: csrc/attention_f8.hip has the figures)
+    return resident if (2 * blocks <= resident if block_rows == 64 else 6 * blocks <= 5 * resident) else 0
+
+
+def attention_prefill_f8_tickets(device: torch.device, num_heads: int, head_dim: int, blocks: int, groups: int, block_rows: int,
+                                 table_keys: int) -> int:
+    """How many tickets ``attention_prefill_f8`` counts in for so many blocks and groups, over a block table whose rows have room
+    for ``table_keys`` keys (0: none)."""
+    return TICKET * blocks * num_heads if _cut_into(device, num_heads, head_dim, blocks, groups, block_rows, table_keys) else 0
+
+
 def attention_prefill_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                          v_scale: torch.Tensor, q_start: torch.Tensor, ctx_len: torch.Tensor, block_table: torch.Tensor,
                          work_seq: torch.Tensor, work_qoff: torch.Tensor, scale: float, window: int = 0, block_rows: int = 64,
@@ -268,7 +285,8 @@ def attention_prefill_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
     of ``block_rows`` (64 or 128) rows, those with the most keys first; ``groups`` workgroups a head share it (0: one for
     every block). Where blocks have a workgroup each and these fill less than the GPU, blocks are cut along their keys, on the device and
     by the contexts that it finds there.
-    ``tickets``: zeros that such launches on one stream may share, TICKET * blocks * query heads (else they are made)."""
+    ``tickets``: zeros that such launches on one stream may share, as many as ``attention_prefill_f8_tickets`` says (else they are
+    made)."""
     what = "attention_prefill_f8"
     stream = _launch_stream(what, out, q, k_cache, v_cache, k_scale, v_scale, q_start, ctx_len, block_table, sink, work_seq, work_qoff,
                             tickets)
@@ -286,15 +304,11 @@ def attention_prefill_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
     if n == 0:
         return
     groups = min(n, groups, 65535) if groups > 0 else min(n, 65535)
-    cap, work, work_at, tickets_at = 0, None, None, None
-    if groups == n <= 64 and block_table.shape[1] * page_size > 64 * WORTH_TILES:
-        # (blocks of 64 rows that fill more than half of it are as fast whole, of 128 rows five sixths: csrc/attention_f8.hip has the figures)
-        resident = _prefill_resident(q.device, Hq, D)
-        if 2 * n <= resident if block_rows == 64 else 6 * n <= 5 * resident:
-            cap = resident
-            work = torch.empty((n + cap) * Hq * block_rows * (D + 8), dtype=torch.float32, device=q.device)
-            tickets = _tickets(tickets, TICKET * n * Hq, q, what)
-            work_at, tickets_at = work.data_ptr(), tickets.data_ptr()
+    cap, work_at, tickets_at = _cut_into(q.device, Hq, D, n, groups, block_rows, block_table.shape[1] * page_size), None, None
+    if cap:
+        work = torch.empty((n + cap) * Hq * block_rows * (D + 8), dtype=torch.float32, device=q.device)
+        tickets = _tickets(tickets, TICKET * n * Hq, q, what)
+        work_at, tickets_at = work.data_ptr(), tickets.data_ptr()
     _check(_entry("ptl_attention_prefill_f8")(*args, work_seq.data_ptr(), work_qoff.data_ptr(), n, groups, cap, work_at, tickets_at,
                                               block_rows, Hq, Hkv, D, page_size, int(window), sink_at, scale, stream), what)
 

@@ -290,5 +290,11 @@ class PagedAttention(Part):
         rows, groups = ops.attention_prefill_f8_plan(
             q.device, self.num_heads, D, ctx.work[PORTIONS_64][0].numel(), ctx.work[PORTIONS_128][0].numel(),
             min(keys, window) if window else keys, ctx.lens_are_bounds)
-        ops.attention_prefill_f8(out, q, *held, *tables, *ctx.work[PORTIONS_128 if rows == 128 else PORTIONS_64], self.scale, window,
-                                 rows, groups, sink=self.sink)
+        work = ctx.work[PORTIONS_128 if rows == 128 else PORTIONS_64]
+        # (zeros that all layers of the step share, and all replays of a recorded one: a launch leaves them so)
+        need = ops.attention_prefill_f8_tickets(q.device, self.num_heads, D, work[0].numel(), groups, rows,
+                                                group.block_table.shape[1] * cache.page_size)
+        tickets = getattr(ctx, "block_tickets", None)
+        if need and (tickets is None or tickets.numel() < need):
+            tickets = ctx.block_tickets = torch.zeros(need, dtype=torch.int32, device=q.device)
+        ops.attention_prefill_f8(out, q, *held, *tables, *work, self.scale, window, rows, groups, sink=self.sink, tickets=tickets)

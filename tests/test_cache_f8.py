@@ -73,3 +73,47 @@ def test_a_layer_of_a_pool_begins_at_a_multiple_of_its_rows(D, need):
         off = pool.flatten()[need // 2:need // 2 + 15 * D].view(5, 1, 3, D)
         with pytest.raises(ops.KernelError, match=f"{need}-byte"):
             cache_f8._cache("a call", 1, D, pool[0], off, scale[0], scale[0])
+
+
+def test_layers_of_a_step_share_the_tickets_of_their_blocks(monkeypatch):
+    """Made once, by the first layer whose blocks are cut, and as many as the call counts in; none where blocks stay whole."""
+    import types
+
+    from pytriton_llama_amd.parts import attention
+    monkeypatch.setattr(cache_f8, "compute_units", lambda device: 256)
+    calls = []
+    monkeypatch.setattr(ops, "attention_prefill_f8", lambda *args, tickets=None, **more: calls.append((args, tickets)))
+
+    def step(rows, pages, layers):
+        calls.clear()
+        lists = {w: (torch.zeros(-(-rows // w.block_rows), dtype=torch.int32),) * 2 for w in (attention.PORTIONS_64, attention.PORTIONS_128)}
+        ctx = types.SimpleNamespace(num_decode_seqs=0, num_seqs=1, ctx_lens=[16 * pages], work=lists, lens_are_bounds=False, q_start=None,
+                                    ctx_len=None)
+        group = types.SimpleNamespace(block_table=torch.zeros(1, pages, dtype=torch.int32))
+        for heads in layers:
+            part = attention.PagedAttention(64, heads, 8, 64)
+            codes, scales = torch.zeros(1, 8, 16, 64).to(ops.CACHE_F8), torch.zeros(1, 8)
+            cache = types.SimpleNamespace(k=codes, v=codes, k_scale=scales, v_scale=scales, page_size=16)
+            q = torch.zeros(rows, heads, 64, dtype=torch.bfloat16)
+            part.attend(torch.empty_like(q), q, cache, ctx, group)
+        return [t for _, t in calls]
+
+    a, b, c = step(500, 200, (32, 32, 8))                    # (four blocks of 128 rows)
+    assert a is b is c and a.numel() == ops.TICKET * 4 * 32 and a.dtype == torch.int32 and not a.any()
+    few, many = step(200, 200, (8, 64))[-2:]                 # (a later layer that needs more)
+    assert few.numel() == ops.TICKET * 4 * 8 and many.numel() == ops.TICKET * 4 * 64
+    assert step(500, 20, (32,)) == [None] and step(1500, 120, (32,)) == [None]
+
+
+@pytest.mark.parametrize("heads", [1, 8, 32, 40])
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+def test_parts_of_blocks_are_within_what_the_kernel_takes(monkeypatch, heads, dim):
+    monkeypatch.setattr(cache_f8, "compute_units", lambda device: 256)
+    for rows in (64, 128):
+        for blocks in (1, 2, 5, 12, 13, 20, 64, 65):
+            parts = cache_f8._cut_into("cuda", heads, dim, blocks, blocks, rows, 4096)
+            assert 0 <= parts <= 4096 and (parts == 0 or blocks <= min(64, parts))
+            assert cache_f8._cut_into("cuda", heads, dim, blocks, blocks, rows, 768) == 0
+            assert cache_f8._cut_into("cuda", heads, dim, blocks, blocks + 1, rows, 4096) == 0
+            n = ops.attention_prefill_f8_tickets("cuda", heads, dim, blocks, blocks, rows, 4096)
+            assert n == (ops.TICKET * blocks * heads if parts else 0)
