@@ -38,14 +38,16 @@ def pages_that_fit(usable_bytes: int, bytes_per_page: int, state_bytes: int, cap
 def graph_pool_bytes(model, engine: EngineConfig) -> int:
     """Memory the recorded steps' shared pool is allowed for when the cache is sized from free
     memory: the intermediate results of the largest step that is recorded (a portion of up to
-    2,048 tokens beside max_num_seqs decoding rows) and its float32 logits. (The logits that the
+    2,048 tokens beside max_num_seqs decoding rows), its float32 logits and the parts that attention over a cache in 8
+    bits cuts its keys into. (The logits that the
     graphs of further size classes keep come from what gpu_memory_fraction leaves free.) Nothing
     when steps are not recorded."""
     if not (engine.use_graphs and model.graph_capturable()):
         return 0
     from .graphs import PORTION_BUCKETS
     tokens = min(PORTION_BUCKETS[-1], engine.max_num_batched_tokens) + engine.max_num_seqs
-    return tokens * model.widest_step_row_bytes() + (engine.max_num_seqs + 1) * model.vocab_size * 4
+    parts = model.workspace_bytes_in(engine.cache_dtype, engine.device, engine.page_size, engine.max_num_seqs, engine.dtype)
+    return tokens * model.widest_step_row_bytes() + (engine.max_num_seqs + 1) * model.vocab_size * 4 + parts
 
 
 def pages_from_memory(model, engine: EngineConfig) -> int:

@@ -96,6 +96,14 @@ class CausalLM:
             layers[c] = mixer.cache_spec_in(dtype)
         return layers
 
+    def workspace_bytes_in(self, cache_dtype: Optional[torch.dtype], device, page_size: int, num_seqs: int, engine_dtype: torch.dtype) -> int:
+        """What a mixer's launches make at most, beside their results, over a cache in ``cache_dtype`` (one layer's at a time)."""
+        if cache_dtype is None:
+            return 0
+        mixers = [getattr(b, "mixer", None) for b in self.blocks]
+        return max((m.workspace_bytes_in(cache_dtype, device, page_size, num_seqs, engine_dtype)
+                    for m in mixers if hasattr(m, "workspace_bytes_in")), default=0)
+
     def kernel_libraries(self) -> Tuple[str, ...]:
         libs: Tuple[str, ...] = ()
         for part in [self.embedding, *self.blocks, self.final_norm, self.head]:

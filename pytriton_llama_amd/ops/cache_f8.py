@@ -197,6 +197,11 @@ MOST_PARTS_F8 = 128        # parts of a (sequence, kv head) pair (csrc/attention
 WHOLE_KEYS_F8 = 512        # keys of a pair that is never cut
 
 
+def _decode_parts(device: torch.device, num_heads: int, num_kv_heads: int) -> int:
+    """Parts of all sequences' keys, some: a workgroup a compute unit."""
+    return max(1, min(MOST_PARTS_F8, compute_units(device) // (num_kv_heads * -(-(num_heads // num_kv_heads) // 16))))
+
+
 def attention_decode_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                         v_scale: torch.Tensor, q_start: torch.Tensor, ctx_len: torch.Tensor, block_table: torch.Tensor, n_seq: int,
                         scale: float, window: int = 0, sink: Optional[torch.Tensor] = None,
@@ -220,7 +225,7 @@ def attention_decode_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tenso
         _tickets(tickets, 0, q, what)                        # (checks)
     if block_table.shape[1] * page_size > WHOLE_KEYS_F8:
         tiles = -(-(Hq // Hkv) // 16)
-        cap = max(1, min(MOST_PARTS_F8, compute_units(q.device) // (Hkv * tiles)))     # a workgroup a compute unit
+        cap = _decode_parts(q.device, Hq, Hkv)
         heads = (n_seq + cap) * Hq                                                   # (room for parts: csrc/attention_f8.hip)
         parts = torch.empty(heads * (D + 2), dtype=torch.float32, device=q.device)
         tickets = _tickets(tickets, TICKET * n_seq * Hkv * tiles, q, what)
@@ -275,6 +280,19 @@ def attention_prefill_f8_tickets(device: torch.device, num_heads: int, head_dim:
     """How many tickets ``attention_prefill_f8`` counts in for so many blocks and groups, over a block table whose rows have room
     for ``table_keys`` keys (0: none)."""
     return TICKET * blocks * num_heads if _cut_into(device, num_heads, head_dim, blocks, groups, block_rows, table_keys) else 0
+
+
+def attention_f8_workspace_bytes(device: torch.device, num_heads: int, num_kv_heads: int, head_dim: int, num_seqs: int) -> int:
+    """The most that one call of ``attention_decode_f8`` with up to ``num_seqs`` sequences, or of ``attention_prefill_f8``, makes for the
+    parts that it cuts keys into."""
+    cap = _decode_parts(device, num_heads, num_kv_heads)
+    most = (num_seqs + cap) * num_heads * (head_dim + 2)
+    for rows in (64, 128):
+        blocks = max((n for n in range(1, 65) if _cut_into(device, num_heads, head_dim, n, n, rows, 1 << 30)), default=0)
+        if blocks:
+            parts = _cut_into(device, num_heads, head_dim, blocks, blocks, rows, 1 << 30)
+            most = max(most, (blocks + parts) * num_heads * rows * (head_dim + 8))
+    return 4 * most
 
 
 def attention_prefill_f8(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,

@@ -82,6 +82,12 @@ class PagedAttention(Part):
             raise ValueError(f"a cache in 8 bits takes even head sizes, got {self.head_dim}")
         return paged_kv_spec(self.num_kv_heads, self.head_dim, self.window, dtype)
 
+    def workspace_bytes_in(self, cache_dtype: torch.dtype, device, page_size: int, num_seqs: int, engine_dtype: torch.dtype) -> int:
+        """What a step's attention makes at most beside its result over a cache in ``cache_dtype``."""
+        if cache_dtype != ops.CACHE_F8 or not ops.attention_f8_fits(engine_dtype, self.num_heads, self.num_kv_heads, self.head_dim, page_size):
+            return 0
+        return ops.attention_f8_workspace_bytes(device, self.num_heads, self.num_kv_heads, self.head_dim, num_seqs)
+
     @property
     def graph_capturable(self) -> bool:
         return self.position is None or getattr(self.position, "graph_capturable", True)

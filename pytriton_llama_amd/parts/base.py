@@ -18,6 +18,8 @@ norm:            forward(x, residual) -> (y, new_residual)    residual may be No
 mixer:           cache_spec() -> PagedSpec | StateSpec | None
                  cache_spec_in(dtype) -> PagedSpec   (optional) the same held in another type than
                  the engine's (torch.float8_e4m3fn: 8 bits); its forward then finds that in the view
+                 workspace_bytes_in(cache dtype, device, page_size, num_seqs, engine dtype) -> int   (optional)
+                 what a step makes at most for its launches over such a cache
                  forward(x, ctx, cache) -> y      x, y: [T, hidden]
                  work_lists() -> WorkList, ...   (optional) how its kernels cut the query rows
 feed-forward:    forward(x) -> y

@@ -117,3 +117,46 @@ def test_parts_of_blocks_are_within_what_the_kernel_takes(monkeypatch, heads, di
             assert cache_f8._cut_into("cuda", heads, dim, blocks, blocks + 1, rows, 4096) == 0
             n = ops.attention_prefill_f8_tickets("cuda", heads, dim, blocks, blocks, rows, 4096)
             assert n == (ops.TICKET * blocks * heads if parts else 0)
+
+
+@pytest.mark.parametrize("heads,kv,dim,seqs", [(32, 8, 64, 8), (32, 8, 128, 64), (8, 1, 96, 300), (2, 2, 32, 1), (40, 2, 128, 5), (1024, 8, 64, 3)])
+def test_the_workspace_of_every_call_is_within_what_is_said(monkeypatch, heads, kv, dim, seqs):
+    """What the faces would make for calls of all numbers of blocks and sequences, by the sizes that they ask torch for."""
+    monkeypatch.setattr(cache_f8, "compute_units", lambda device: 256)
+    most = ops.attention_f8_workspace_bytes("cuda", heads, kv, dim, seqs)
+    made = [0]
+    real = torch.empty
+
+    def empty(n, **more):
+        made[0] = max(made[0], 4 * n)
+        return real(1)
+    monkeypatch.setattr(cache_f8, "_launch_stream", lambda *a: 0)
+    monkeypatch.setattr(cache_f8, "_entry", lambda name: lambda *a: 0)
+    monkeypatch.setattr(cache_f8.torch, "empty", empty)
+    codes, scales = torch.zeros(1, kv, 16, dim).to(ops.CACHE_F8), torch.zeros(1, kv)
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32)   # noqa: E731
+    for blocks in (1, 2, 3, 5, 8, 12, 13, 16, 20, 33, 64, 65):
+        for rows in (64, 128):
+            q = torch.zeros(1, heads, dim, dtype=torch.bfloat16)
+            ops.attention_prefill_f8(q, q, codes, codes, scales, scales, i32(2), i32(1), i32(100).view(1, 100), i32(blocks), i32(blocks), 1.0,
+                                     0, rows)
+    for n in {1, seqs}:
+        q = torch.zeros(n, heads, dim, dtype=torch.bfloat16)
+        ops.attention_decode_f8(q, q, codes, codes, scales, scales, i32(n + 1), i32(n), i32(100 * n).view(n, 100), n, 1.0)
+    assert 0 < made[0] <= most <= 2 * made[0]
+
+
+def test_the_recorded_steps_pool_counts_the_parts_of_keys(monkeypatch):
+    from pytriton_llama_amd.config import EngineConfig, build_model
+    from pytriton_llama_amd.engine import llm
+    from tiny_configs import tiny
+    monkeypatch.setattr(cache_f8, "compute_units", lambda device: 256)
+    model = build_model(tiny("B")[0])
+    model.dtype = torch.bfloat16
+    config = dict(dtype="bfloat16", device="cpu", page_size=16, max_num_seqs=4, max_model_len=4096, use_graphs=True)
+    plain, eight = (llm.graph_pool_bytes(model, EngineConfig(**config, cache_dtype=c)) for c in (None, "fp8"))
+    mixer = model.blocks[0].mixer
+    assert eight - plain == ops.attention_f8_workspace_bytes("cpu", mixer.num_heads, mixer.num_kv_heads, mixer.head_dim, 4) > 0
+    config["page_size"] = 8                                   # (the general kernel has no parts)
+    assert llm.graph_pool_bytes(model, EngineConfig(**config, cache_dtype="fp8")) == llm.graph_pool_bytes(model, EngineConfig(**config))
+    assert llm.graph_pool_bytes(model, EngineConfig(**{**config, "use_graphs": False}, cache_dtype="fp8")) == 0
