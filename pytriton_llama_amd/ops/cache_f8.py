@@ -245,22 +245,33 @@ def _prefill_resident(device: torch.device, num_heads: int, head_dim: int) -> in
 
 def attention_prefill_f8_plan(device: torch.device, num_heads: int, head_dim: int, blocks_of_64: int, blocks_of_128: int,
                               max_keys: int = 0, bound: bool = False):
-    """(block_rows, groups) for ``attention_prefill_f8``; arguments as of ``attention_prefill_mfma_plan``, which it follows but where few
-    blocks have many keys each: blocks of 128 rows, cut along their keys, from 4 of them on where the longest sequence has 512
-    keys for each; 192 at head sizes above 64 if the blocks of 64 rows have no workgroup each at once. us in blocks of 64 and of 128
-    rows, 32 heads, rows behind keys: 1,024 behind 1,000 of 128 50 57, 900 behind 4,000 128 123, 512 behind 8,000 122 109, 500 behind 3,000
-    (4 blocks) 62 64, 200 behind 3,000 (2) 38 45; 1,100 behind 1,500 103 80, 1,536 behind 500 66 71, 1,531 behind 1,000 97 86, 2,048
-    alone 65 72; 1,024 behind 4,000 of 64 80 73, 2,048 behind 8,000 231 216, 2,048 behind 3,000 107 113, 1,500 behind 2,500 73 81.
+    """(block_rows, groups) for ``attention_prefill_f8``; arguments as of ``attention_prefill_mfma_plan``, which it follows but where
+    blocks have many keys each. With t = the workgroups of a head that run at once, four blocks of 128 rows or more, and max_keys the
+    longest sequence's, blocks have 128 rows
+      where blocks of 64 are cut (2 of them fill no more than t): above head size 64 from 3,000 keys a workgroup on (blocks * max_keys / t);
+      where each has a workgroup: from 4,800 keys on;
+      where they are more than t: from 400 keys for each block of 128 rows on, above head size 64 from 192.
+    us in blocks of 64 and of 128 rows, heads x head size, rows behind keys. Cut: 8 x 64 512 behind 6,000 30 41, 2,048 behind 6,000 65 72; 16 x 64
+    1,024 behind 4,000 46 54; 32 x 64 512 behind 6,000 58 66; 16 x 128 512 behind 6,000 63 66, 1,024 behind 4,000 78 87; 8 x 128 2,048 behind 6,000
+    110 110; 32 x 128 500 behind 3,000 62 64, 512 behind 6,000 100 89, behind 8,000 122 109. A workgroup each: 16 x 64 2,048 behind 2,000 57 62, behind
+    6,000 120 102; 32 x 64 1,024 behind 1,000 32 42, behind 4,000 79 75; 64 x 64 512 behind 6,000 106 91; 16 x 128 2,048 behind 2,000 90 97, behind
+    6,000 185 175; 32 x 128 1,024 behind 1,000 49 58, 900 behind 4,000 128 123; 64 x 128 512 behind 6,000 163 150. More: 32 x 64 2,048 behind 3,000
+    107 113, behind 6,000 188 179; 64 x 64 1,024 behind 4,000 124 124; 32 x 128 1,536 behind 500 67 72, 1,531 behind 1,000 97 86, 2,048 behind 2,000
+    160 140; 64 x 128 1,024 behind 1,000 87 77.
 
     ``bound``: max_keys is only a bound of what the sequences will have (a step that is recorded). Then blocks of 128 rows are for
     head sizes above 64, a bound from 4,096 on and blocks of 64 rows that have no workgroup each at once: 2,048 rows of 128 lose 7 us
     by them where the prompt begins and win 24 behind 2,048 keys; 1,024 rows lose 17 and win 8 behind 6,000."""
     t = max(1, _prefill_resident(device, num_heads, head_dim))
-    few = blocks_of_64 <= t
     if bound:
-        long = not few and head_dim > 64 and max_keys >= 4096
+        long = blocks_of_64 > t and head_dim > 64 and max_keys >= 4096
+    elif 2 * blocks_of_64 <= t:
+        long = head_dim > 64 and blocks_of_64 * max_keys >= 3000 * t
+    elif blocks_of_64 <= t:
+        long = max_keys >= 4800
     else:
-        long = blocks_of_128 >= 4 and max_keys >= (192 if head_dim > 64 and not few else 512) * blocks_of_128
+        long = max_keys >= (192 if head_dim > 64 else 400) * blocks_of_128
+    long = long and (bound or blocks_of_128 >= 4)
     rows, blocks = (128, blocks_of_128) if long or 4 * blocks_of_128 >= 5 * t else (64, blocks_of_64)
     return rows, max(1, blocks if blocks <= 2 * t else t)
 
