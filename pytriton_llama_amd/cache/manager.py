@@ -167,6 +167,10 @@ class CacheManager:
         """Whether ``req`` has pages and no state slot."""
         return req in self.num_tokens and req not in self.slot_of
 
+    def holds(self, req) -> bool:
+        """Whether ``req`` is live or parked: it has something to give back."""
+        return req in self.num_tokens
+
     @property
     def num_free_slots(self) -> int:
         return len(self._free_slots)

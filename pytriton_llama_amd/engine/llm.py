@@ -222,7 +222,7 @@ class Engine:
         share = min(req.num_computed, len(req.prompt) + n - 1)
         places = max(0, self.scheduler.max_num_seqs - len(self.scheduler.running))
         made = 0
-        if share > 0 and (self.runner.manager.is_live(request_id) or self.runner.manager.is_parked(request_id)):
+        if share > 0 and self.runner.manager.holds(request_id):
             made = self.runner.fork(request_id, [b.id for b in branches], share, places)
         for b in branches[:made]:
             b.num_computed = share

@@ -108,5 +108,5 @@ class ModelRunner:
 
     def end(self, request: Hashable) -> None:
         """The request is finished: what it holds is given back."""
-        if self.manager.is_live(request) or self.manager.is_parked(request):
+        if self.manager.holds(request):
             self.manager.free(request)

@@ -135,7 +135,7 @@ class Scheduler:
                 plan.entries.remove(e)
                 for g, n in enumerate(self.manager.pages_needed(victim.id, e.num_tokens)):
                     reserve[g] -= n
-        if self.manager.is_live(victim.id):
+        if self.manager.holds(victim.id):          # (a branch whose first step has not run is parked still)
             self.manager.free(victim.id)
         self.running.remove(victim)
         victim.num_computed = 0
@@ -266,11 +266,9 @@ class Scheduler:
     def abort(self, req: Request) -> None:
         if req in self.running:
             self.running.remove(req)
-            if self.manager.is_live(req.id):
-                self.manager.free(req.id)
         elif req in self.waiting:
             self.waiting.remove(req)
-            if self.manager.is_parked(req.id):
-                self.manager.free(req.id)
+        if self.manager.holds(req.id):
+            self.manager.free(req.id)
         req.status = FINISHED
         req.finish_reason = "aborted"

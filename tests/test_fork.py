@@ -572,3 +572,33 @@ def test_a_request_that_stops_is_let_alone():
     while e.has_work:
         e.step()
     assert [len(r.output) for r in reqs] == [3, 9]
+
+
+@pytest.mark.parametrize("then", ["abort", "preempt"])
+def test_a_branch_whose_first_step_failed(then):
+    """It was planned, the step did not run: it has its pages and no slot, and gives them back like any other."""
+    e = HostEngine(pages=14, seqs=3)
+    rid = e.add_request(range(10), SamplingParams(max_new_tokens=12))
+    e.step()
+    made = e.fork(rid, SamplingParams(max_new_tokens=12), 3, num_output=0)
+    for r in made[:2]:
+        e.abort(r)
+    e.scheduler.schedule()                                   # (and an error in the step)
+    branch = e.requests[made[2]]
+    assert branch.status == "running" and e.manager.is_parked(branch.id)
+    if then == "abort":
+        e.abort(branch.id)
+    else:
+        e.manager.admit("filler")
+        e.manager.append("filler", 4 * e.manager.paged[0].pool.num_free)
+        while branch.num_preemptions == 0:
+            e.step()
+        assert not e.manager.holds(branch.id) or e.manager.num_tokens[branch.id] == branch.num_computed
+        e.manager.free("filler")
+    e.manager.check()
+    first = e.requests[rid]
+    while e.has_work:
+        e.step()
+    assert len(first.output) == 12 and (then == "abort" or len(branch.output) == 12)
+    e.requests.clear()
+    e.all_back()
