@@ -45,8 +45,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--prompt_ids", action="append", default=None,
                     help="prompt as token ids, e.g. '1,5,17' (repeatable)")
     ap.add_argument("--stream", type=_bool, default=True)
-    ap.add_argument("--cache_dtype", default=None, help="float8_e4m3fn: keys and values in 8 bits (default: as --dtype)")
-    ap.add_argument("--samples", type=int, default=1, help="completions of every prompt, which is computed once")
+    ap.add_argument("--cache_dtype", default=None, help="float8_e4m3fn: keys and values in 8 bits, half the memory; steps over few cached tokens and prompts get slower (default: as --dtype)")
+    ap.add_argument("--samples", type=int, default=1, help="completions of every prompt, which is computed once as long as there is room for what they share")
     return ap
 
 

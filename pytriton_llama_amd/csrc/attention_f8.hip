@@ -30,7 +30,7 @@ struct F8Tables {
 // 200 behind 700 153 71.
 //
 // What bounds it: few rows the chain of a turn, some 3 us (1 x 1,000 keys 7.8 us, 1 x 4,000 18.3, 8 x 2,048 27.2), many the vector units, which
-// have every key row anew for every query row (200 rows behind 700: 18 TFLOP/s).
+// have every key row anew for every query row (200 rows behind 700: 19 TFLOP/s).
 template <typename T, int NACC, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES)
 attn_generic_f8_kernel(T* __restrict__ out, long out_stride, const T* __restrict__ q, long q_stride, F8Cache cache, F8Tables tab,
@@ -223,13 +223,19 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) { return
 // of 128 14.2 13.4, 8 x 5,000 to 7,000 26.1 24.7, 32 x 100 to 5,000 61.7 47.4, 64 x 100 to 1,000 21.2 24.9. (Sixteen waves: 16 x 1,000 of
 // 64 8.2, 8 x 2,048 11.2, 64 x 61 to 2,610 25.)
 //
-// What bounds it: 2 x 120,000 keys of 128 take 89 us, 5.5 TB/s of codes in pieces of 2 KB (a copy reaches 4.8 both ways, a
-// plain stream of reads 7.1; three or four tiles a wave on their way instead of two change nothing: 89.7, 90.3). Few keys: a
+// What bounds it: 120,001 and 131,000 keys of 128 take 92 us, 5.6 TB/s of codes in pieces of 2 KB (a copy reaches 4.8 both ways, a
+// plain stream of reads 7.1; three or four tiles a wave on their way instead of two change nothing: 2 x 120,000 89, 90, 90). Few keys: a
 // chain of the context lengths, the table, the codes, and for a pair in parts of their way to memory and back, some 3 us.
 //
 // Both products are transposed, as in attention_decode.h:
 //   S^T[key, head] = K . Q^T        A = K: lane (ln, lg) has key ln's k-values, straight from memory
 //   O^T[d, head]  += V^T . P^T      B = P^T: what a lane has of S^T; A = V^T[d, key]
+// A weight is rounded to bfloat16 for the second product, as over a bfloat16 cache, and the denominator sums the rounded ones (a product
+// with ones), so that a row's weights add up to one: the result is off by at most 2 * 2^-8 of sum w |v|. Against 64 bits that makes an
+// error of 0.0017 to 0.0022 of the result where its rounding alone makes 0.0016 to 0.0017. Weights in two parts, the rounded one and
+// what it lacks, would leave that alone, with every second product twice: 64 x 61 to 2,610 of 64 22.1 23.4 us, 8 x 2,048
+// 11.2 11.4, 120,001 and 131,000 of 128 92.3 93.3, a prompt of 2,048 of 64 34.8 43.1, 1,531 rows behind 6,145 keys of 128 241 366.
+// Maxima, denominators and sums are float32.
 // For the second a lane needs one d of the 8 keys that its P^T values belong to. It loads D / 16 neighbouring elements of each of those
 // keys, which are D / 16 matrix instructions' d, and pairs the keys' halves up after the conversion (two
 // v_perm_b32 for two words): no LDS between memory and the matrix cores, and nothing to wait for but the loads.
@@ -629,9 +635,10 @@ extern "C" int ptl_attention_decode_f8(void* out, long out_stride, const void* q
 // keys that they see in tiles of 64. A tile's codes are turned into bfloat16 (with their scales) and lie in LDS in two buffers: in the
 // turn in which tile t is used, tile t + 1 is converted into the other buffer, and tile t + 2 sets out. With registers
 // between memory and the conversion it sets out at the turn's end: its codes then take no registers beside the products (us
-// before and behind the products, 32 heads: 2,048 rows of 64 36.9 35.2, 2,048 behind 2,048 of 128 in 128-row blocks 158 145; the conversion
-// between the two products instead of before them spills there, 353). Products, softmax and the layout of LDS are those of
-// attention_prefill.h: S^T = K Q^T, O^T += V^T P^T, sums of the rounded probabilities by one more product with ones.
+// before and behind the products, 32 heads, when this was built: 2,048 rows of 64 36.9 35.2, 2,048 behind 2,048 of 128 in 128-row blocks 158
+// 145; the conversion between the two products instead of before them spills there, 353). Products, softmax, its roundings and the layout of
+// LDS are those of attention_prefill.h and of the decode kernel above: S^T = K Q^T, O^T += V^T P^T, sums of the rounded weights by one
+// more product with ones.
 // Of a tile every wave brings 16 rows, which lie in one page: page and scales are the wave's, in scalar registers.
 //
 // CUT: few blocks. Their tiles, one block's behind the other's, are dealt out evenly to the workgroups that the GPU runs at once: a
@@ -643,7 +650,7 @@ extern "C" int ptl_attention_decode_f8(void* out, long out_stride, const void* q
 // 8,000 of 128 250 109, 1,100 behind 6,000 (9, 16) 253 180, 1,531 behind 6,145 (12, 16) 279 243, 1,600 behind 6,000 (13) 272 255, 1,700 (14)
 // 278 277, 2,048 behind 2,048 (16) 141 163; 1,000 behind 8,000 of 64 (8, 24) 183 114.
 //
-// What bounds it: 1,531 rows behind 6,145 keys, 32 heads of 128, take 243 us in blocks of 128 rows that are cut: 173 GFLOP, 713 TFLOP/s,
+// What bounds it: 1,531 rows behind 6,145 keys, 32 heads of 128, take 242 us in blocks of 128 rows that are cut: 173 GFLOP, 715 TFLOP/s,
 // 46 % of what a large product of matrices reaches. The conversion of a tile, done once for each of the blocks that read it, and the
 // softmax share the vector units (the same attention over a bfloat16 cache, without the conversion and not cut: 250).
 struct PrefillF8Parts {
@@ -662,8 +669,8 @@ attn_prefill_f8_kernel(bf16_t* __restrict__ out, long out_stride, const bf16_t* 
   constexpr int D = 32 * ND, BN = 64, ROWS = 64 * RT;
   constexpr int PIECES = D / 8;                     // 8-element pieces of a row: 8 codes, 16 bytes of bfloat16
   // two row tiles: registers are short, so codes go to LDS without one in between, to a place of the wave's own (its 16 rows are whole
-  // kilobytes, 64 lanes of 16 bytes). us with and without, 32 heads of 128: 1,531 rows behind 6,145 keys 274 284, 2,048 behind 2,048
-  // 139 145; with one row tile 332 312, 185 171.
+  // kilobytes, 64 lanes of 16 bytes). us with and without, 32 heads of 128, before blocks were cut: 1,531 rows behind 6,145 keys 274 284 (cut,
+  // with: 241), 2,048 behind 2,048 139 145; with one row tile 332 312, 185 171.
   constexpr bool STAGED = RT == 2 && D % 64 == 0;
   __shared__ __attribute__((aligned(16))) bf16_t Ks[2][BN * D], Vs[2][BN * D];
   __shared__ __attribute__((aligned(16))) uint8_t staged[STAGED ? 4 : 1][2][STAGED ? 16 * D : 16];

@@ -39,7 +39,7 @@ __device__ __forceinline__ uint32_t two_codes(float a, float b) {
 // waves write one scale. Up to DIRECT rows every row has its tasks, and the waves of rows that begin nothing leave. Beyond, a
 // workgroup makes the list of the rows that begin a run (of LISTED rows at a time) and its waves take their share of the
 // tasks; with a workgroup for every row 2,048 rows, 8 kv heads of 128, took 71 us, from lists they took 17.6, and where the four tasks of a
-// workgroup are of one run, whose angles they make together, they take 15.1.
+// workgroup are of one run, whose angles they make together, they take 15.0.
 // A wave takes the rows of its run a chunk at a time, holds their numbers of a head and finds the largest; a run of one chunk (16 rows
 // of 128) is then written from the registers, a longer one read and rotated again. Behind them the workgroups that rotate the queries, a
 // row a wave.
