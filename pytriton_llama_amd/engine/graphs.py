@@ -34,6 +34,7 @@ replay reads are written by ordinary copies before it.
 """
 from __future__ import annotations
 
+import gc
 from typing import Dict, List, Sequence
 
 import torch
@@ -93,8 +94,16 @@ def capture_forward(model, storage, ctx, device, pool=None, timed_products: bool
     torch.cuda.current_stream().wait_stream(side)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph, pool=pool), ops.timed_library_products(timed_products):
-        logits = model.forward(ctx, storage)
+    # No garbage is collected while the step is recorded: what an engine that nobody holds any more has on the GPU (its graphs,
+    # events, pinned buffers), if it lies in a cycle, would be given back then, which is not allowed during a recording and ends the process.
+    collects = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph, pool=pool), ops.timed_library_products(timed_products):
+            logits = model.forward(ctx, storage)
+    finally:
+        if collects:
+            gc.enable()
     return graph, logits
 
 

@@ -1,3 +1,4 @@
+import gc
 import os
 import sys
 
@@ -9,6 +10,14 @@ sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu)")
+
+
+@pytest.fixture(autouse=True, scope="module")
+def no_garbage_for_the_next_module():
+    """Engines that a module's tests left in cycles go before another module records a graph of its own (what they have on the GPU
+    cannot be given back during a recording)."""
+    yield
+    gc.collect()
 
 
 @pytest.fixture(scope="session")
