@@ -96,10 +96,13 @@ def capture_forward(model, storage, ctx, device, pool=None, timed_products: bool
     graph = torch.cuda.CUDAGraph()
     # No garbage is collected while the step is recorded: what an engine that nobody holds any more has on the GPU (its graphs,
     # events, pinned buffers), if it lies in a cycle, would be given back then, which is not allowed during a recording and ends the process.
-    collects = gc.isenabled()
+    # And the recording begins outside of inference mode, the forward runs in it where the caller does: the first recording of a
+    # process makes tensors for torch's random numbers, and if those are inference tensors nobody records outside of that mode any more.
+    collects, inference = gc.isenabled(), torch.is_inference_mode_enabled()
     gc.disable()
     try:
-        with torch.cuda.graph(graph, pool=pool), ops.timed_library_products(timed_products):
+        with torch.inference_mode(False), torch.cuda.graph(graph, pool=pool), torch.inference_mode(inference), \
+                ops.timed_library_products(timed_products):
             logits = model.forward(ctx, storage)
     finally:
         if collects:

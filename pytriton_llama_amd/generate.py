@@ -89,7 +89,7 @@ class GenerateText:
     def generate_samples(self, prompt_tokens: List[List[int]], count: int, max_gen_len: int, temperature: float = 0.6,
                          top_p: float = 0.9, logprobs: bool = False
                          ) -> Tuple[List[List[List[int]]], Optional[List[List[List[float]]]]]:
-        """As ``generate``, ``count`` times for every prompt, which is computed once: the tokens (and with
+        """As ``generate``, ``count`` times for every prompt, which is computed once (Engine.generate_samples): the tokens (and with
         ``logprobs`` their log-probabilities) of every sample of every prompt."""
         params = [self._params(max_gen_len, temperature, top_p, len(p), logprobs) for p in prompt_tokens]
         groups = self.engine.generate_samples(prompt_tokens, count, params)
